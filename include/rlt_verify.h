@@ -760,6 +760,69 @@ RLT_API int rlt_delta_scan(const void* q, const void* k, const void* v, int64_t 
 RLT_API int rlt_step_metadata(int32_t* words, const int64_t* at, const int64_t* records, int portions, int sequences, int planes, int width,
                       int short_sequences, int64_t rows, int64_t dummy_slot);
 
+/* ------------------------------------------------------------------------
+ * A step's rows on the device: pages claimed from a stack of free ones and the slot of every row.  No counterpart in the reference, whose
+ * scheduler does both on the host.
+ *   cu[s] = sum of the counts before s (below zero: zero);  new_lengths[s] = lengths[s] + counts[s]
+ *   row r of request s: position lengths[s] + r - cu[s], page tables[s][position / block_size], offset position % block_size
+ * With `held` (pages that each request holds) request s first gets max(ceil(new_lengths[s] / block_size) - held[s], 0) pages, appended to its
+ * table row at held[s]; page k of the call, in the order of the requests and their entries, is free_pages[free_count - 1 - k]; held and
+ * free_count are updated.  Rows behind the last request's: row_seq and write_blocks -1, position and offset 0.  Refused as a whole (status 1,
+ * cu and active_rows 0, new_lengths = lengths, state unchanged): more than `rows` rows, more pages than are free, a length below zero or
+ * beyond table_width * block_size, held below zero or beyond table_width, free_count below zero or beyond free_capacity.
+ * lengths, counts, new_lengths, held: int32 [requests], at most 8192.  tables: int32 [requests][table_width].  free_pages: int32
+ * [free_capacity].  cu: int32 [requests + 1].  positions, row_seq: int32 [rows].  write_blocks, write_offsets: int64 [rows].  free_count,
+ * active_rows, status: one int32.  held may be NULL (with free_pages and free_count): the tables are complete.
+ *
+ * rlt_return_pages: request s keeps the pages of its first lengths[s] tokens.  Page k of those given back goes to place
+ * free_count + total - 1 - k, so that the call undoes the claims of the step before it.  status 1 and nothing changed where free_capacity
+ * would be passed or held is out of range. */
+RLT_API int rlt_step_slots(const int32_t* lengths, const int32_t* counts, int requests, int32_t* tables, int table_width, int block_size,
+                   int32_t* held, const int32_t* free_pages, int free_capacity, int32_t* free_count, int rows, int32_t* cu,
+                   int32_t* new_lengths, int32_t* positions, int32_t* row_seq, int64_t* write_blocks, int64_t* write_offsets,
+                   int32_t* active_rows, int32_t* status, rlt_stream_t stream);
+RLT_API int rlt_return_pages(const int32_t* lengths, int requests, const int32_t* tables, int table_width, int block_size, int32_t* held,
+                     int32_t* free_pages, int free_capacity, int32_t* free_count, int32_t* status, rlt_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * A paged cache in 8 bits: e4m3 codes [pages][block_size][kv_heads][head_dim <= 256] (block_stride and token_stride in BYTES, the
+ * [kv_heads, head_dim] tail contiguous) and fp32 scales [pages][kv_heads] (row stride scale_stride, in elements), keys and values alike;
+ * value = code * scale.  No counterpart in the reference, whose caches hold the model's dtype.
+ * Rows are packed: rows cu_rows[s] .. cu_rows[s + 1] - 1 (int32 [sequences + 1]) are the last ones of sequence s, whose length with them is
+ * lengths[s] (int32 [sequences]); page p of sequence s is block_tables[s][p] (int32 [sequences][table_width]).
+ *
+ * rlt_quantized_kv_write: k, v [rows][kv_heads][head_dim] of `dtype`, row strides in elements.  Per page that gets rows and head, K and V
+ * apart: e the smallest exponent in [-100, 100] with max |finite x| <= 448 * 2^e over the new rows; scale = 2^e where offset 0 is written,
+ * else max(2^e, old scale rounded up to a power of two), and where that is larger than the old one the tokens in front of the new rows are
+ * rounded again; code = e4m3(x / scale), to nearest even, saturating; what is not finite becomes NaN.  A page that is written belongs to one
+ * sequence of the call.  Rows at negative positions, behind cu_rows[sequences], beyond their table row or in pages outside the cache are
+ * not stored.
+ *
+ * rlt_quantized_attention: out[r, h] = sum_t softmax_t(scale * q[r, h] . K[t, h / g]) V[t, h / g], row i of the n_s of a sequence over
+ * t < lengths[s] - n_s + i + 1, with window > 0 the last `window` of those; a row that sees no key gives zeros, rows behind
+ * cu_rows[sequences] are left alone.  A length beyond table_width * block_size (at most 2^26) is cut to it; a page outside the cache reads as zeros.  q, out:
+ * [rows][q_heads][head_dim] with row strides.  max_new: the longest portion (it chooses the kernel, and nothing depends on its being
+ * exact).  A row's bits depend on its own query, keys and values only.  workspace: rlt_quantized_attention_workspace_bytes(...) bytes, 16-byte
+ * aligned, private to the call until its work on `stream` completes.
+ *
+ * rlt_quantized_kv_expand: the tokens of every sequence in `dtype` as 16-token pages, [sequences * pages_width][16][kv_heads][head_dim], page p
+ * of sequence s at s * pages_width + p, which page_tables (int32 [sequences][pages_width]) then names; slots and entries behind a length
+ * are not written.  pages_width * 16 >= table_width * block_size. */
+RLT_API int rlt_quantized_kv_write(void* key_cache, void* value_cache, float* key_scale, float* value_scale, int64_t block_stride,
+                           int64_t token_stride, int64_t scale_stride, int64_t num_blocks, int block_size, int kv_heads, int head_dim,
+                           const void* k, int64_t k_stride, const void* v, int64_t v_stride, int dtype, const int32_t* block_tables,
+                           const int32_t* lengths, const int32_t* cu_rows, int sequences, int table_width, int rows, rlt_stream_t stream);
+RLT_API size_t rlt_quantized_attention_workspace_bytes(int rows, int q_heads, int head_dim, int block_size, int table_width, int window);
+RLT_API int rlt_quantized_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const void* key_cache, const void* value_cache,
+                            const float* key_scale, const float* value_scale, int64_t block_stride, int64_t token_stride,
+                            int64_t scale_stride, int64_t num_blocks, int block_size, int q_heads, int kv_heads, int head_dim, int dtype,
+                            const int32_t* block_tables, const int32_t* lengths, const int32_t* cu_rows, int sequences, int table_width,
+                            int rows, int max_new, float scale, int window, void* workspace, size_t workspace_bytes, rlt_stream_t stream);
+RLT_API int rlt_quantized_kv_expand(const void* key_cache, const void* value_cache, const float* key_scale, const float* value_scale,
+                            int64_t block_stride, int64_t token_stride, int64_t scale_stride, int64_t num_blocks, int block_size,
+                            int kv_heads, int head_dim, const int32_t* block_tables, const int32_t* lengths, int sequences, int table_width,
+                            void* key_pages, void* value_pages, int32_t* page_tables, int pages_width, int dtype, rlt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

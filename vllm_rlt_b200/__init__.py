@@ -24,6 +24,7 @@ from .layers import (block_epilogue, clamped_glu, gated_unit, head_gate, head_mi
                      soft_cap, stream_mix)
 from .looped_lm import LoopedLM, LoopedLMConfig, seeded_state_dict
 from .postnorm_lm import PostNormLM, PostNormLMConfig
+from .quantized_kv import QuantizedKV, StepSlots, quantized_attention, quantized_kv_write, return_pages, step_slots
 from .recurrent import causal_conv, conv_heads, decay_scan, decay_table, delta_scan, gated_norm, ssd_scan
 from .registry import load_model, register_model, registered_architectures
 from .runner import (B200SpeculativeRunner, KVCacheManagerView, ModelRunnerOutput, Request, SamplingParams, ScheduledRequest,
@@ -52,4 +53,5 @@ __all__ = [
     "SandwichLM", "SandwichLMConfig", "YarnScaling", "conv_heads", "gated_unit", "head_gate", "packed_attention", "soft_cap",
     "PostNormLM", "PostNormLMConfig", "delta_scan", "head_mix", "norm_rotate", "paired_rows",
     "talking_attention", "talking_decode", "talking_prompt",
+    "QuantizedKV", "StepSlots", "quantized_attention", "quantized_kv_write", "return_pages", "step_slots",
 ]

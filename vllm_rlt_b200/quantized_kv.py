@@ -1,0 +1,228 @@
+"""A paged key/value cache in 8 bits, and a step's pages and slots on the GPU.
+
+`QuantizedKV` is one layer's cache: e4m3 codes `[pages, block, kv_heads, dim]` and a float32 scale for each page and head.  A step over it:
+
+    slots = step_slots(lengths, counts, tables, block, rows, held=held, free_pages=free_pages, free_count=free_count)
+    quantized_kv_write(cache, k, v, tables, slots.lengths, slots.cu)
+    out = quantized_attention(q, cache, tables, slots.lengths, slots.cu, max_new)
+
+The rows of a step are packed: rows cu[s] .. cu[s + 1] - 1 are sequence s's last ones, at positions lengths[s] - n_s .. lengths[s] - 1, and
+everything is read on the device, so a step of a fixed number of rows can be captured in a CUDA graph and replayed with other lengths.
+"""
+
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import _capi
+
+CODE_DTYPE = torch.float8_e4m3fn
+
+
+@dataclass(frozen=True)
+class QuantizedKV:
+    """One layer's keys and values in 8 bits: a value is its code times the scale of its page and head.
+
+    key / value: float8_e4m3fn `[pages, block, kv_heads, dim]` of one layout, pages and tokens with any stride, the `[kv_heads, dim]` tail
+    contiguous; dim at most 256.  key_scale / value_scale: float32 `[pages, kv_heads]` of one layout, heads side by side."""
+
+    key: torch.Tensor
+    value: torch.Tensor
+    key_scale: torch.Tensor
+    value_scale: torch.Tensor
+
+    @classmethod
+    def allocate(cls, pages: int, block: int, kv_heads: int, dim: int, device="cuda") -> "QuantizedKV":
+        """An empty cache, keys and values in one allocation (a page of both is then one copy)."""
+        codes = torch.zeros(2, pages, block, kv_heads, dim, dtype=CODE_DTYPE, device=device)
+        scales = torch.zeros(2, pages, kv_heads, dtype=torch.float32, device=device)
+        return cls(codes[0], codes[1], scales[0], scales[1])
+
+    def check(self) -> None:
+        key, value, ks, vs = self.key, self.value, self.key_scale, self.value_scale
+        if key.dim() != 4 or value.shape != key.shape or key.stride() != value.stride() or key.dtype != CODE_DTYPE or value.dtype != CODE_DTYPE:
+            raise ValueError("key and value must be float8_e4m3fn [pages, block, kv_heads, dim] of one layout")
+        if (key.shape[3] > 1 and key.stride(3) != 1) or (key.shape[2] > 1 and key.stride(2) != key.shape[3]):
+            raise ValueError("the [kv_heads, dim] tail of the cache must be contiguous")
+        if not 0 < key.shape[3] <= 256 or key.shape[1] == 0 or key.shape[2] == 0:
+            raise ValueError("a cache needs tokens, heads, and a dim of 1 .. 256")
+        if ks.dtype != torch.float32 or vs.dtype != torch.float32 or ks.shape != (key.shape[0], key.shape[2]) or vs.shape != ks.shape \
+                or ks.stride() != vs.stride() or (ks.shape[1] > 1 and ks.stride(1) != 1):
+            raise ValueError("scales must be float32 [pages, kv_heads] of one layout with unit inner stride")
+
+
+@dataclass(frozen=True)
+class StepSlots:
+    """A step's rows (device tensors).  Rows behind the last request's have row_seq -1, write_blocks -1 and zeros."""
+
+    cu: torch.Tensor              # int32 [n + 1]  rows cu[s] .. cu[s + 1] - 1 are request s's
+    lengths: torch.Tensor         # int32 [n]      tokens of the request with the step's
+    positions: torch.Tensor       # int32 [rows]
+    row_seq: torch.Tensor         # int32 [rows]   request of the row
+    write_blocks: torch.Tensor    # int64 [rows]   page and offset the row is stored at (`kv_write`, `rope_kv_write`)
+    write_offsets: torch.Tensor   # int64 [rows]
+    active_rows: torch.Tensor     # int32 []       cu[n]
+    status: torch.Tensor          # int32 []       0, or 1: refused, and nothing changed
+
+
+def _check_words(n: int, **tensors) -> None:
+    for name, t in tensors.items():
+        if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous int32 [{n}]")
+
+
+def _check_stack(tables, held, free_pages, free_count) -> None:
+    _check_words(tables.shape[0], held=held)
+    _check_words(1, free_count=free_count)
+    if free_pages.dtype != torch.int32 or free_pages.dim() != 1 or not free_pages.is_contiguous():
+        raise ValueError("free_pages must be contiguous int32 [pages]")
+
+
+def _check_tables(tables) -> None:
+    if tables.dtype != torch.int32 or tables.dim() != 2 or not tables.is_contiguous():
+        raise ValueError("tables must be contiguous int32 [requests, pages]")
+
+
+def step_slots(lengths, counts, tables, block: int, rows: int, *, held=None, free_pages=None, free_count=None) -> StepSlots:
+    """Slots of a step that stores `counts[s]` more tokens of request s behind the `lengths[s]` it has, in up to `rows` rows.
+
+    lengths / counts: int32 `[n]`, n at most 8192 (a count below zero is zero).  tables: int32 `[n, pages]`.  With `held` (int32 `[n]`, pages
+    that each request holds) missing pages are claimed first, from the end of the stack `free_pages` (int32 `[m]`, of which the first
+    free_count[0] are free), in the order of the requests: tables, held and free_count are updated in place.  Without it the tables have to
+    name every page already.  A step that does not fit (rows, free pages, a table's width), or a length or number of held or free pages that cannot
+    be, is refused as a whole: status 1, no rows, nothing changed.  A number of held pages may be larger than a request needs: a request
+    that was rolled back keeps its pages."""
+    _check_tables(tables)
+    n, width = tables.shape
+    _check_words(n, lengths=lengths, counts=counts)
+    if (held is None) != (free_pages is None) or (held is None) != (free_count is None):
+        raise ValueError("held, free_pages and free_count come together")
+    if held is not None:
+        _check_stack(tables, held, free_pages, free_count)
+    if block < 1 or rows < 0:
+        raise ValueError("block must be positive, rows not negative")
+    device = _capi.require_cuda(lengths, counts, tables, held, free_pages, free_count)
+    words = torch.empty(2 * n + 3 + 2 * rows, dtype=torch.int32, device=device)
+    cu, new_lengths, positions, row_seq, last = words.split((n + 1, n, rows, rows, 2))
+    write_blocks, write_offsets = torch.empty(2, rows, dtype=torch.int64, device=device).unbind()
+    active_rows, status = last.unbind()
+    with torch.cuda.device(device):
+        code = _capi.load().rlt_step_slots(
+            _capi.ptr(lengths), _capi.ptr(counts), n, _capi.ptr(tables), width, block, _capi.ptr(held), _capi.ptr(free_pages),
+            0 if free_pages is None else free_pages.numel(), _capi.ptr(free_count), rows, _capi.ptr(cu), _capi.ptr(new_lengths),
+            _capi.ptr(positions), _capi.ptr(row_seq), _capi.ptr(write_blocks), _capi.ptr(write_offsets), _capi.ptr(active_rows), _capi.ptr(status),
+            _capi.stream_of(words))
+    _capi.check(code, "step_slots")
+    return StepSlots(cu, new_lengths, positions, row_seq, write_blocks, write_offsets, active_rows, status)
+
+
+def return_pages(lengths, tables, block: int, *, held, free_pages, free_count):
+    """Request s keeps the pages of its first `lengths[s]` tokens (0: none) and gives the others back to the stack, so that what was claimed
+    last is claimed next; held, free_pages and free_count are updated in place, the tables stay.  Returns an int32 status on the device: 0, or
+    1 where the stack has no room (pages given back twice) or a number of held pages cannot be; then nothing has changed."""
+    _check_tables(tables)
+    n, width = tables.shape
+    _check_words(n, lengths=lengths)
+    _check_stack(tables, held, free_pages, free_count)
+    if block < 1:
+        raise ValueError("block must be positive")
+    device = _capi.require_cuda(lengths, tables, held, free_pages, free_count)
+    status = torch.empty((), dtype=torch.int32, device=device)
+    with torch.cuda.device(device):
+        code = _capi.load().rlt_return_pages(_capi.ptr(lengths), n, _capi.ptr(tables), width, block, _capi.ptr(held), _capi.ptr(free_pages),
+                                             free_pages.numel(), _capi.ptr(free_count), _capi.ptr(status), _capi.stream_of(status))
+    _capi.check(code, "return_pages")
+    return status
+
+
+def _check_step(tables, lengths, cu) -> None:
+    _check_tables(tables)
+    n = tables.shape[0]
+    _check_words(n, lengths=lengths)
+    _check_words(n + 1, cu=cu)
+
+
+def _row_stride(t) -> int:
+    """Elements between the rows of a [rows, heads, dim] tensor with a contiguous tail, which may be a slice of wider rows."""
+    if (t.shape[2] > 1 and t.stride(2) != 1) or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+        raise ValueError("the [heads, dim] tail of rows must be contiguous")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _cache_args(cache: QuantizedKV) -> tuple:
+    """Addresses, strides and pages of a cache; a dimension of one has the stride of a dense layout."""
+    key, scale = cache.key, cache.key_scale
+    pages, block, kv_heads, dim = key.shape
+    token = key.stride(1) if block > 1 else kv_heads * dim
+    return (_capi.ptr(key), _capi.ptr(cache.value), _capi.ptr(scale), _capi.ptr(cache.value_scale), key.stride(0) if pages > 1 else block * token, token,
+            scale.stride(0) if pages > 1 else kv_heads, pages)
+
+
+def quantized_kv_write(cache: QuantizedKV, k, v, tables, lengths, cu) -> None:
+    """Store a step's keys and values, `[rows, kv_heads, dim]` in float32, float16 or bfloat16 (rows may be slices of wider ones).
+
+    In every page that gets rows, and for every head, the scale becomes the smallest power of two (2^-100 .. 2^100) that brings the new rows'
+    largest element within the codes' 448, or stays the page's own where that is larger; where it grows, the tokens in front of the new rows
+    are rounded again.  A page whose offset 0 is written starts anew: what it held behind the new rows means nothing any more.  Codes are
+    rounded to the nearest, ties to even; elements that are not finite are stored as NaN and have no part in a scale.
+
+    A page that is written belongs to one sequence of the call.  Rows at negative positions, behind the last sequence, behind the end of
+    their table row or in a page that does not exist are not stored."""
+    cache.check()
+    _check_step(tables, lengths, cu)
+    pages, block, kv_heads, dim = cache.key.shape
+    if k.dim() != 3 or k.shape[1:] != (kv_heads, dim) or v.shape != k.shape or k.dtype not in _capi.DTYPE_CODES or v.dtype != k.dtype:
+        raise ValueError("k and v must be [rows, kv_heads, dim] of the cache's heads, in float32, float16 or bfloat16")
+    rows = k.shape[0]
+    k_stride, v_stride = _row_stride(k), _row_stride(v)
+    device = _capi.require_cuda(cache.key, cache.value, cache.key_scale, cache.value_scale, k, v, tables, lengths, cu)
+    if rows == 0 or pages == 0:
+        return
+    with torch.cuda.device(device):
+        code = _capi.load().rlt_quantized_kv_write(
+            *_cache_args(cache), block, kv_heads, dim, _capi.ptr(k), k_stride, _capi.ptr(v), v_stride, _capi.DTYPE_CODES[k.dtype], _capi.ptr(tables),
+            _capi.ptr(lengths), _capi.ptr(cu), tables.shape[0], tables.shape[1], rows, _capi.stream_of(k))
+    _capi.check(code, "quantized_kv_write")
+
+
+def quantized_attention(q, cache: QuantizedKV, tables, lengths, cu, max_new: int, *, scale: float | None = None, window: int = 0, out=None):
+    """Causal attention of a step's rows, `[rows, heads, dim]` in float32, float16 or bfloat16, over an 8-bit cache, in q's type.
+
+    Row i of the n_s rows of sequence s sees lengths[s] - n_s + i + 1 keys, with `window` the last so many of them; a row that sees none gives
+    zeros, a length that its table cannot address is cut to what it can, and rows behind the last sequence are left as they are in `out`
+    (undefined where `out` is not given).  scale: 1 / sqrt(dim) unless given.  max_new: the longest portion of the step, which decides on the
+    kernels; results do not depend on the other sequences of a call.  Heads are whole groups over the cache's.  Slots that no token was
+    stored in may hold anything."""
+    cache.check()
+    _check_step(tables, lengths, cu)
+    pages, block, kv_heads, dim = cache.key.shape
+    if q.dim() != 3 or q.shape[2] != dim or q.dtype not in _capi.DTYPE_CODES or q.shape[1] == 0 or q.shape[1] % kv_heads:
+        raise ValueError("q must be [rows, heads, dim] in float32, float16 or bfloat16, with whole groups of heads over the cache's")
+    if isinstance(window, bool) or not isinstance(window, int) or window < 0 or max_new < 0:
+        raise ValueError("window and max_new must be integers that are not negative")
+    device = _capi.require_cuda(q, cache.key, cache.value, cache.key_scale, cache.value_scale, tables, lengths, cu, out)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("out must have q's shape and dtype")
+    rows, heads, _ = q.shape
+    sequences, width = tables.shape
+    q_stride, out_stride = _row_stride(q), _row_stride(out)
+    if rows == 0 or sequences == 0:
+        return out
+    if width == 0:
+        raise ValueError("tables need at least one page per sequence")
+    window = min(window, 2 ** 31 - 1)
+    lib = _capi.load()
+    with torch.cuda.device(device):
+        nbytes = lib.rlt_quantized_attention_workspace_bytes(rows, heads, dim, block, width, window)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None   # a call's own: graphs and streams share none
+        code = lib.rlt_quantized_attention(
+            _capi.ptr(q), q_stride, _capi.ptr(out), out_stride, *_cache_args(cache), block, heads, kv_heads, dim, _capi.DTYPE_CODES[q.dtype],
+            _capi.ptr(tables), _capi.ptr(lengths), _capi.ptr(cu), sequences, width, rows, int(max_new),
+            float(1.0 / math.sqrt(dim) if scale is None else scale), window, _capi.ptr(workspace), nbytes, _capi.stream_of(q))
+    _capi.check(code, "quantized_attention")
+    return out
