@@ -145,16 +145,17 @@ quantized_merge_kernel(QuantizedAttentionArgs a) {
     float next = big;
 #pragma unroll
     for (int i = 0; i < 8; ++i) next = fmaxf(next, ml[i].x);          // the last part's again behind the end
-    const float zero = next == -INFINITY ? 0.0f : next, keep = exp2f(big - zero);
+    // l goes by 2^x in two steps: between parts whose values differ by far in size the factor may be 0 in fp32 where l times it is not
+    const float zero = next == -INFINITY ? 0.0f : next, root = exp2f(0.5f * (big - zero)), keep = root * root;
     big = next;
-    total *= keep;
+    total = total * root * root;
 #pragma unroll
     for (int j = 0; j < 2; ++j) { acc[j].x *= keep; acc[j].y *= keep; acc[j].z *= keep; acc[j].w *= keep; }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if (c0 + i >= parts) break;
-      const float f = exp2f(ml[i].x - zero);
-      total = fmaf(ml[i].y, f, total);
+      const float half = exp2f(0.5f * (ml[i].x - zero)), f = half * half;
+      total += ml[i].y * half * half;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         if (lane + 32 * j < quads) {
@@ -311,7 +312,8 @@ extern "C" RLT_API int rlt_quantized_attention(const void* q, int64_t q_stride, 
     return RLT_ERR_WORKSPACE;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  RLT_DISPATCH_DTYPE(dtype, T, status = launch_rows<T>(a, s));
+  status = quantized_tiles_supported(a) ? launch_quantized_tiles(a, max_new, s) : RLT_ERR_UNSUPPORTED;
+  if (status == RLT_ERR_UNSUPPORTED) RLT_DISPATCH_DTYPE(dtype, T, status = launch_rows<T>(a, s));
   if (status != RLT_OK || a.parts < 2) return status;
   RLT_DISPATCH_DTYPE(dtype, T, return launch_merge<T>(a, s));
 }
