@@ -171,11 +171,14 @@ def allowed(result, parts, dtype, dim, tiles):
     Half a step of the output's type, eps / 2 * |result|, and the weights' errors, each of which moves the output by at most its relative
     size times sum p |v| (twice where it enters the denominator too):
       scores: products of a row add up in fp32, dim roundings (the tensor cores cut instead of rounding: eps, not eps / 2) of at most
-              the sum of |q| |k|; with q brought to half precision at its largest element's size, an error of 2^-25 of that per element
-              (2^-12 |q| where q is normal in it is 0 for bf16 and fp16 rows): below 2^-24 of the sum for the sizes tested; times 2
+              the sum of |q| |k|; q as three parts of four bits at its largest element's size holds fp16's eleven bits and bf16's eight, and is
+              off by half of the last part's smallest step, 2^-10 / 1024 of a largest of 2^7: 2^-27 of it per element, which adds up to at
+              most eps of the sum for the sizes tested; times 2
       2^x:    two steps of fp32, 2^-22; the factor 2^(M_c - M) of a part again; sums of `count` terms in fp32: count * 2^-24; times 2
-      tiles:  weights are rounded to half precision, 2^-11 where they are normal in it; they are kept at 2^8 .. 2^15 for the row's largest
-              p * value scale, so that half a step of the smallest numbers is 2^-25 / 2^8 of it, per key, times the largest code 448."""
+      tiles:  weights are rounded to half precision, 2^-11, and held as three parts of four significant bits, of which eleven bits need no more
+              (a part leaves at most 2^-4 of what it took: 2^-4, 2^-8, then three bits for the last); the parts' smallest steps are those of
+              the codes, 2^-9 / 1024, half of it 2^-20, at a largest p * value scale of at least 2^6: 2^-26 of it, per key, times
+              the largest code 448."""
     spread, size, tiny, count = parts
     eps = torch.finfo(torch.float32).eps
     weight = 2 * (dim * eps * size + eps * size) + 2 * (4 * 2.0 ** -22 + count * eps / 2)
@@ -184,7 +187,7 @@ def allowed(result, parts, dtype, dim, tiles):
     total = spread * weight + torch.finfo(dtype).eps / 2 * result.abs() + torch.finfo(torch.float32).tiny
     if dtype == torch.float16:
         total = total + 2.0 ** -25                                   # half a step of its smallest numbers
-    return total + (tiny * 448 * 2.0 ** -33 if tiles else 0)
+    return total + (tiny * 448 * 2.0 ** -26 if tiles else 0)
 
 
 # ---- inputs -------------------------------------------------------------------------------------------

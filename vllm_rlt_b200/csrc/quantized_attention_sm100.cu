@@ -1,24 +1,26 @@
 // Attention over an 8-bit paged cache for short portions (decoding, verification): 64- and 128-wide heads, fp16 / bf16 queries, pages of whole
-// 16-token tiles.
+// 16-token tiles.  The codes are operands of the 5th-generation tensor cores as they lie in their pages: no conversion anywhere (converting
+// them to half precision took 77 % of the conversion pipe's time at 28 % of the memory's rate).
 //
-// Work.  An item is up to 16 query rows of one key/value head — (row, query head of the group) pairs of one sequence — over one part of its
-// context (kPartTokens at fixed positions).  Items are dealt to one CTA per SM in a fixed order that every CTA derives from the lengths: no work
-// list, no atomics, no second launch before the first byte is read.
+// Work.  An item is up to kRows query rows — (row, query head of the group) pairs of one sequence — of 128 bytes of heads (one 128-wide key/value
+// head or two 64-wide ones) over one part of the context (kPartTokens at fixed positions).  Items are dealt to one CTA per SM in an order that every
+// CTA derives from the lengths: no work list, no atomics, no launch before the first byte is read.
 //
-// Data flow.  A producer warp copies 32 tokens at a time (keys and values of two 16-token tiles, one TMA box each) into a ring of stages that runs
-// on across items, so the loads never stop; eight consumer warps take the stages in turn, by position.  Codes go from shared memory to the
-// tensor cores through one conversion: e4m3 is exact in half precision.
-//   S = Q K^T     m16n8k16, rows x tokens.  The head's elements are dealt to the products' k so that a lane's sixteen are one 16-byte load.
-//   O^T += V^T P^T   m16n8k16, elements x rows: S's accumulators are P^T's operand as they are, and V, which lies token by token, needs only a
-//                    byte permutation of two rows: the elements are dealt to the products' m like the head's elements above.
-// Queries are brought to half precision at their own row's power of two (bf16 and fp16 rows lose nothing but what is 2^-24 of the row's largest).
-// A key's scale multiplies its score; a value's scale goes into its weight's exponent, so a weight is 2^(s + log2 scale_v - R) and the sum l of the
-// weights divides it out again.  R is a row's reference: it moves only when a weight would pass 2^15, and then so that the largest is 2^8.
-// Weights are rounded to half precision (2^-11) for the second product; at 2^8 .. 2^15 for the largest, what is lost below half precision's
-// smallest numbers is 2^-33 of it.  Scores, R, l and O are fp32.
+// Products.  Keys and values are the M operands, so a handful of rows is the N and nothing is padded to a tensor tile:
+//   S^T = K Q^T        lanes = 128 tokens, columns = rows;       O^T += V^T P^T     lanes = 128 value elements, V^T read MN-major
+// Q and P have more bits than a code, so both are sums of three: x = h + m / 32 + l / 1024, each rounded to four significant bits, what is
+// left going to the next: the columns of an operand are the three parts of its rows, and the parts of a result are added in fp32.  A query row
+// is brought to its own power of two first (the largest element in 2^7 .. 2^8); bf16 and fp16 rows lose what is 2^-27 of that.
 //
-// The eight warps' results of an item are added in shared memory in the order of the warps, so a row's bits depend on positions only, not on
-// the batch, the other rows of its item or the part's length.
+// Softmax.  A key's scale multiplies its score; a value's goes into its weight's exponent, so a weight is
+// p = 2^(s + log2 scale_v - R) and l = sum p / scale_v.  R is a row's reference: it moves when a weight would pass 2^kHighest, and then so
+// that the largest is 2^kFresh.  Rounding p to three parts leaves 2^-12 of it, and below 2^-20 nothing: 2^-26 of a row's largest weight.
+// Scores, R, l and O are fp32.
+//
+// Roles.  Two groups of eight warps take tiles of 128 tokens in turn, each with scores, weights, references and sums of its own; one warp issues
+// S^T products, one O^T products, one the copies (a ring of tiles that runs on across items; keys give their place back before their values),
+// one prepares the queries of the next item.  The second group's sums are joined with the first's.  Which group a tile belongs to goes by its
+// position, so a row's bits do not depend on the batch or on the other rows of its item.
 //
 // Bound by the bytes of keys and values.
 #include <cuda.h>
@@ -29,122 +31,255 @@
 namespace rlt {
 namespace {
 
-constexpr int kConsumers = 8;
-constexpr int kThreads = (kConsumers + 4) * 32;  // whole warpgroups, so that registers can move from the producer's to the consumers'
-constexpr int kConsumerRegisters = 208, kProducerRegisters = 80;
-static_assert(kConsumers * 32 * kConsumerRegisters + 4 * 32 * kProducerRegisters <= kThreads * 168, "what a block of this size is launched with");
-constexpr int kSlots = 16;              // stages in the ring
-constexpr int kStageTokens = 32;
-constexpr int kBatch = 1024;            // sequences whose items are laid out at a time
-constexpr float kHighest = 15.0f;       // log2 of the largest weight that is kept
-constexpr float kFresh = 8.0f;          // log2 of the largest weight when a row's reference moves
-
-template <int kD, int kRowTiles>
-struct __align__(1024) Shared {
-  static constexpr int kRows = 8 * kRowTiles, kStride = kD + 4;
-  unsigned char stages[kSlots][2][2][16 * kD];      // [tile of the stage][lower / upper cache][token][element], swizzled by the copy
-  float sums[kConsumers][kRows][kStride];           // O, R, l of each warp
-  float4 scales[kSlots][2];                         // per tile: key scale, log2 of the value scale, its inverse
-  unsigned long long full[kSlots], empty[kSlots];
-  int items[kBatch + 1];                            // items in front of a sequence of the batch
-  int first[kBatch], count[kBatch], base[kBatch];   // its rows, and the keys its first row sees (below 1: none)
-};
+constexpr int kGroups = 2;
+constexpr int kGroupThreads = 256;      // two threads per token, each with half of the rows
+constexpr int kGroupWarps = kGroupThreads / 32;
+constexpr int kThreads = kGroups * kGroupThreads + 128;       // and copies, S^T, O^T, queries
+constexpr int kCopyWarp = 16, kScoreWarp = 17, kValueWarp = 18, kQueryWarp = 19;
+constexpr int kTile = 128;              // tokens
+constexpr int kTileBytes = kTile * 128; // of keys, or of values
+constexpr int kSlots = 10;              // tiles of keys or of values in the ring, in turn
+constexpr int kScaleSlots = 8;          // tiles' scales; see the copies
+constexpr int kBatch = 256;             // sequences whose items are laid out at a time
+constexpr int kClasses = kPartTokens / kTile + 1;
+constexpr float kHighest = 8.0f, kFresh = 6.0f;
+constexpr float kFaint = -100.0f;       // log2 of a weight whose product with 1 / scale_v may leave fp32
+constexpr float kWide = 30.0f;          // log2 of a value scale that makes that possible
 
 struct Item {
-  int s, first, count, base, kv_head, pair0, pairs, part;
-  int begin;        // first token of the first stage
-  int end;          // behind the last visible token of the part
-  int stages;
+  int s, first, count, base;
+  int unit;         // 128 bytes of heads
+  int pair0;        // the first pair of the item; pairs of every head of the unit
+  int pairs;
+  int part;
+  int from, end;    // tokens of the part that some row sees
+  int all_from, all_end;      // and those that every row sees
+  int begin;        // the first tile's first token
+  int tiles;
 };
+
+enum { kNowhere, kOutput, kZero, kPartial };
+
+template <int kRows>
+struct __align__(1024) Shared {
+  static constexpr int kN = kRows == 16 ? 48 : 32;    // three parts of every row, in whole sixteens
+  unsigned char ring[kSlots][kTileBytes];             // [token][128 bytes], swizzled by the copy: keys of a tile, its values, the next tile's keys ..
+  unsigned char q[2][kN * 128];                       // [item parity][part of a row][128 elements]
+  unsigned char p[kGroups][kN * 128];                 // [part of a row][128 tokens]
+  float sums[2][kRows][128];                          // [item parity]: O of the second group
+  float other_ref[2][kRows], other_l[2][kRows];       // its references and sums
+  float folded[kGroups][4][kRows];
+  uint32_t fresh[kGroups][2];                         // rows of a half without a reference yet
+  unsigned moved[kGroups][2];                         // the turn of a half's last move of a reference that had been there
+  float by[kGroups][kRows], root[kGroups][kRows];     // of a move of references: added to them; the root of what O and l are multiplied by
+  float factor[2][kRows];                             // of the joined result: the groups' O times these
+  uint32_t raw_q[kRows][64];                          // the next item's queries as they are
+  float row_scale[2][kRows];                          // of the scores, by item parity
+  int keys[2][kRows], low[2][kRows];                  // what a row sees
+  int64_t to[2][kRows];                               // where its result of the item goes: elements into the output, or floats into the partials
+  int kind[2][kRows];                                 // kNowhere, kOutput, kZero, kPartial
+  Item item[2];
+  uint32_t nan_value[kGroups][kRows][4];              // elements that a row gets NaN in
+  float4 scales[kScaleSlots][2][kTile / 16];          // by head and 16 tokens: key scale, log2 of the value scale, its inverse
+  int wide[kScaleSlots];                              // a value scale of the tile beyond 2^+-kWide
+  unsigned long long full[kSlots], empty[kSlots], q_full[2], q_empty[2], s_ready[kGroups], s_free[kGroups], p_ready[kGroups], o_done[kGroups];
+  uint32_t tmem_base;
+  // the work of a batch of sequences: cells (part, row tile) of whole parts in front of a sequence; then the last parts, largest first
+  int whole_before[kBatch + 1], last_before[kBatch + 1], order[kBatch];
+  int in_class[kClasses];
+  unsigned char size_class[kBatch];
+  int first[kBatch], count[kBatch], base[kBatch];     // a sequence's rows, and the keys its first row sees (below 1: none)
+};
+
+// Bounded wait for a phase of a barrier: false after about two seconds.  Few instructions: the roles' loops together have to stay within the
+// instruction caches (with unrolled polls at every wait they did not, and every phase took three to ten times as long).
+__device__ __forceinline__ bool wait_for(const unsigned long long* barrier, uint32_t parity) {
+  const uint32_t bar = smem_u32(barrier);
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long begin = clock64();
+#pragma unroll 1
+  while (!mbar_try_wait(bar, parity))
+    if (clock64() - begin > kWaitCycles) return false;
+  return true;
+}
 
 __device__ __forceinline__ int clamp_keys(int keys, int capacity) { return max(min(keys, capacity), 0); }
 
-// A sequence's parts and row tiles.
 struct Spread {
   int first_part, parts, tiles;
 };
-template <int kRows>
-__device__ __forceinline__ Spread spread_of(int count, int base, int group, int window, int capacity) {
+// A sequence's parts, and the row tiles of `each` pairs.
+__device__ __forceinline__ Spread spread_of(int each, int count, int base, int group, int window, int capacity) {
   Spread x;
   const int top = clamp_keys(base + count - 1, capacity), low = window > 0 ? max(clamp_keys(base, capacity) - window, 0) : 0;
   x.first_part = low / kPartTokens;
   x.parts = top > 0 ? (top - 1) / kPartTokens - x.first_part + 1 : 1;
-  x.tiles = (count * group + kRows - 1) / kRows;
+  x.tiles = (count * group + each - 1) / each;
   return x;
 }
 
-__device__ __forceinline__ void tma_tile_pair(uint32_t dst, const CUtensorMap* map, int token, int head, int page, uint32_t bar, uint64_t policy) {
-  asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, %4, %5, %6}], [%7], %8;"
-               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(token), "r"(head), "r"(0), "r"(page), "r"(bar), "l"(policy) : "memory");
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int token, int page, uint32_t bar, uint64_t policy) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, %4}], [%5], %6;"
+               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(token), "r"(page), "r"(bar), "l"(policy) : "memory");
 }
-__device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* map, int token, int head, int page, uint32_t bar, uint64_t policy) {
-  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, %4, %5}], [%6], %7;"
-               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(token), "r"(head), "r"(page), "r"(bar), "l"(policy) : "memory");
+// D[tmem] (+)= A[smem] * B[smem] of e4m3 codes, one elected thread; 32 codes of K.
+__device__ __forceinline__ void code_product(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+template <int kCount>
+__device__ __forceinline__ void load_columns(uint32_t at, float (&x)[kCount]) {
+  uint32_t r[kCount];
+  if constexpr (kCount == 8) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(at));
+  } else {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+  }
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) x[i] = __uint_as_float(r[i]);
+}
+template <int kCount>
+__device__ __forceinline__ void store_columns(uint32_t at, const float (&x)[kCount]) {
+  uint32_t r[kCount];
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) r[i] = __float_as_uint(x[i]);
+  if constexpr (kCount == 8) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+  } else {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+  }
+}
+// A group's barrier, with the OR of a predicate.
+__device__ __forceinline__ bool group_any(int group, bool mine) {
+  uint32_t any;
+  asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbarrier.cta.red.or.pred q, %2, %3, p;\nselp.u32 %0, 1, 0, q;\n}\n"
+               : "=r"(any) : "r"(mine ? 1u : 0u), "r"(1 + group), "n"(kGroupThreads) : "memory");
+  return any != 0;
+}
+// The second group's sums of an item are there: it goes on (at most an item, the queries see to that), the first one waits.
+__device__ __forceinline__ void sums_ready(unsigned parity) { asm volatile("bar.arrive %0, %1;" ::"r"(5 + parity), "n"(kGroups * kGroupThreads) : "memory"); }
+__device__ __forceinline__ void sums_wait(unsigned parity) { asm volatile("bar.sync %0, %1;" ::"r"(5 + parity), "n"(kGroups * kGroupThreads) : "memory"); }
+__device__ __forceinline__ void block_sync() { asm volatile("bar.sync 4, %0;" ::"n"(kThreads) : "memory"); }
+
+// Two numbers as packed codes of their three parts, x = h + m / 32 + l / 1024 for |x| <= 256: x in half precision (2^-11 of it, or 2^-25), then
+// h and m rounded by the conversion to a code; what each leaves, times 32, is exact in half precision.
+__device__ __forceinline__ void three_parts(float x0, float x1, uint32_t (&codes)[3]) {
+  const __half2 whole = __floats2half2_rn(x0, x1), minus = __float2half2_rn(-32.0f), times = __float2half2_rn(32.0f);
+  __half2 left = whole;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const __half2_raw raw = *reinterpret_cast<const __half2_raw*>(&left);
+    const __nv_fp8x2_storage_t code = __nv_cvt_halfraw2_to_fp8x2(raw, __NV_SATFINITE, __NV_E4M3);
+    codes[k] = code;
+    if (k < 2) {
+      const __half2_raw back = __nv_cvt_fp8x2_to_halfraw2(code, __NV_E4M3);
+      left = __hfma2(*reinterpret_cast<const __half2*>(&back), minus, __hmul2(left, times));
+    }
+  }
+}
+__device__ __forceinline__ void store_shared1(uint32_t at, uint32_t x) {
+  asm volatile("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %1;\nst.shared.u8 [%0], lo;\n}\n" ::"r"(at), "r"(x) : "memory");
+}
+__device__ __forceinline__ float4 load_shared16f(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
+  return v;
 }
 
-// Two codes (the low or the high half of a word) as packed half precision.
-__device__ __forceinline__ uint32_t halves_low(uint32_t w) {
-  uint32_t h;
-  asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %1;\ncvt.rn.f16x2.e4m3x2 %0, lo;\n}\n" : "=r"(h) : "r"(w));
-  return h;
+// Folds kCount values over the lanes of a warp, all of them at once: at every step a lane gives half of its values away and takes the other half's
+// partners.  Returns value row_after_fold(lane) of them, complete, in every lane.
+template <int kCount, bool kMax>
+__device__ __forceinline__ float fold_rows(float (&v)[kCount], int lane) {
+  auto op = [](float a, float b) { return kMax ? fmaxf(a, b) : a + b; };
+  int bit = 16;
+#pragma unroll
+  for (int half = kCount / 2; half > 0; half /= 2, bit /= 2) {
+    const bool upper = lane & bit;
+#pragma unroll
+    for (int i = 0; i < half; ++i) {
+      const float give = upper ? v[i] : v[i + half], stay = upper ? v[i + half] : v[i];
+      v[i] = op(stay, __shfl_xor_sync(0xffffffffu, give, bit));
+    }
+  }
+  float x = v[0];
+  for (; bit > 0; bit /= 2) x = op(x, __shfl_xor_sync(0xffffffffu, x, bit));
+  return x;
 }
-__device__ __forceinline__ uint32_t halves_high(uint32_t w) {
-  uint32_t h;
-  asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %1;\ncvt.rn.f16x2.e4m3x2 %0, hi;\n}\n" : "=r"(h) : "r"(w));
-  return h;
-}
-__device__ __forceinline__ uint4 load_shared16(uint32_t at) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
-  return v;
-}
-__device__ __forceinline__ uint2 load_shared8(uint32_t at) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
-  return v;
-}
+template <int kCount>
+__device__ __forceinline__ int row_after_fold(int lane) { return lane / (32 / kCount); }
 // 0x80 in every byte that is a NaN code.
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory"); }
-
-__device__ __forceinline__ void block_sync() { asm volatile("bar.sync 2, %0;" ::"n"(kThreads) : "memory"); }
-
-// The token of a 16-token tile that column or row i < 8 of a product stands for (and 8 more for the next eight).  For 64-wide heads two tokens
-// share a 128-byte line, and this order keeps the lanes of a load in different banks.
-template <int kD>
-__device__ __forceinline__ int token_of(int i) {
-  return kD == 64 ? static_cast<int>((0x65742130u >> (4 * i)) & 7u) : i;
-}
-
-template <typename T, int kD, int kRowTiles, bool kJoint>
+// kDim: 128, or 64 with two heads side by side, whose pairs are rows 0 .. kRows / 2 - 1 and kRows / 2 .. of an item.
+template <typename T, int kDim, int kRows>
 __global__ void __launch_bounds__(kThreads, 1)
 quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map, QuantizedAttentionArgs a, float scale_log2,
-                       int key_first) {
-  using Sm = Shared<kD, kRowTiles>;
-  constexpr int kRows = Sm::kRows, kTileBytes = 16 * kD, kSteps = kD / 16;      // k steps of S, m tiles of O^T
+                       int box) {
+  using Sm = Shared<kRows>;
+  constexpr int kHeads = 128 / kDim, kEach = kRows / kHeads, kN = Sm::kN;
+  constexpr uint32_t kScores = 0, kOutputs = kGroups * 64, kColumns = 256;      // tensor memory: 64 columns per group for each
   extern __shared__ unsigned char smem_raw[];
   Sm& sm = *reinterpret_cast<Sm*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const QuantizedCache& c = a.cache;
-  const int group = a.q_heads / c.kv_heads, capacity = a.step.width * c.block;
-  const uint32_t full = smem_u32(sm.full), empty = smem_u32(sm.empty);
+  const int group_heads = a.q_heads / c.kv_heads, capacity = a.step.width * c.block, units = (c.kv_heads + kHeads - 1) / kHeads;
 
+  if (warp == kScoreWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(kColumns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kSlots; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); }
+    for (int i = 0; i < kSlots; ++i) { mbar_init(smem_u32(&sm.full[i]), 1); mbar_init(smem_u32(&sm.empty[i]), 1); }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&sm.q_full[i]), 1);
+      mbar_init(smem_u32(&sm.q_empty[i]), 1 + kGroups * kGroupWarps);             // the products' completion, and each softmax warp
+      mbar_init(smem_u32(&sm.s_ready[i]), 1);
+      mbar_init(smem_u32(&sm.s_free[i]), kGroupWarps);
+      mbar_init(smem_u32(&sm.p_ready[i]), kGroupWarps);
+      mbar_init(smem_u32(&sm.o_done[i]), 1);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+#pragma unroll 1
+  for (int i = threadIdx.x; i < kGroups * kRows * 4; i += kThreads) (&sm.nan_value[0][0][0])[i] = 0u;
   grid_dependency_wait();
   grid_dependency_release();
+  tcgen05_before_sync();
+  __syncthreads();
+  tcgen05_after_sync();
+  const uint32_t tmem = sm.tmem_base;
 
-  unsigned stage = 0;          // stages of all items before the current one
+  unsigned done_items = 0, done_tiles = 0, done_of[kGroups] = {0u, 0u};   // items, tiles, and tiles of each group before the current item
   bool failed = false;
-  int batch = 0, sequences = 0;
+  int sequences = 0, whole = 0;      // of the batch: sequences, cells of whole parts
 
-  // The items of the next sequences, by all threads; their number.
-  auto lay_out = [&]() {
+  // Exclusive sums of value(i), i < n, into out[0 .. n], by one warp.
+  auto scan = [&](int n, int* out, auto value) {
+    int before = 0;
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const int mine = i0 + lane < n ? value(i0 + lane) : 0;
+      int sum = mine;
+#pragma unroll
+      for (int y = 1; y < 32; y <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, sum, y);
+        if (lane >= y) sum += o;
+      }
+      if (i0 + lane < n) out[i0 + lane] = before + sum - mine;
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (lane == 0) out[n] = before;
+  };
+  auto row_tiles = [&](int i) { return (sm.count[i] * group_heads + kEach - 1) / kEach; };
+
+  // The items of sequences batch .., by all threads; their number.  Cells of whole parts come first, then every sequence's last part, those with the
+  // most tiles first: dealt in this order, one CTA has about as many tiles as another.  The heads of a cell go to neighbouring CTAs at a time.
+  auto lay_out = [&](int batch) {
     sequences = min(a.step.sequences - batch, kBatch);
     block_sync();              // the batch before is done with
+#pragma unroll 1
     for (int i = threadIdx.x; i < sequences; i += kThreads) {
       int first, count;
       rows_of(a.step, batch + i, &first, &count);
@@ -152,513 +287,634 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       sm.first[i] = first;
       sm.count[i] = count;
       sm.base[i] = static_cast<int>(base < -0x20000000 ? -0x20000000 : (base > 0x20000000 ? 0x20000000 : base));
-      const Spread x = spread_of<kRows>(count, sm.base[i], group, a.window, capacity);
-      sm.items[i] = count > 0 ? x.parts * x.tiles * c.kv_heads : 0;
+      const Spread x = spread_of(kEach, count, sm.base[i], group_heads, a.window, capacity);
+      sm.whole_before[i] = count > 0 ? (x.parts - 1) * x.tiles : 0;
+      const int top = clamp_keys(sm.base[i] + count - 1, capacity);
+      sm.size_class[i] = static_cast<unsigned char>(top > 0 ? (top - 1) % kPartTokens / kTile + 1 : 0);
     }
     block_sync();
-    if (warp == 0) {
-      int before = 0;
+    if (warp < kClasses) {
+      int n = 0;
+#pragma unroll 1
+      for (int i0 = 0; i0 < sequences; i0 += 32) n += __popc(__ballot_sync(0xffffffffu, i0 + lane < sequences && sm.size_class[i0 + lane] == warp));
+      if (lane == 0) sm.in_class[warp] = n;
+    } else if (warp == kClasses) {
+      scan(sequences, sm.whole_before, [&](int i) { return sm.whole_before[i]; });
+    }
+    block_sync();
+    if (warp < kClasses) {
+      int at = 0;
+#pragma unroll 1
+      for (int k = kClasses - 1; k > warp; --k) at += sm.in_class[k];
+#pragma unroll 1
       for (int i0 = 0; i0 < sequences; i0 += 32) {
-        const int mine = i0 + lane < sequences ? sm.items[i0 + lane] : 0;
-        int sum = mine;
-#pragma unroll
-        for (int x = 1; x < 32; x <<= 1) {
-          const int o = __shfl_up_sync(0xffffffffu, sum, x);
-          if (lane >= x) sum += o;
-        }
-        if (i0 + lane < sequences) sm.items[i0 + lane] = before + sum - mine;
-        before += __shfl_sync(0xffffffffu, sum, 31);
+        const unsigned mine = __ballot_sync(0xffffffffu, i0 + lane < sequences && sm.size_class[i0 + lane] == warp);
+        if ((mine >> lane) & 1) sm.order[at + __popc(mine & ((1u << lane) - 1))] = i0 + lane;
+        at += __popc(mine);
       }
-      if (lane == 0) sm.items[sequences] = before;
     }
     block_sync();
-    return sm.items[sequences];
+    if (warp == 0) scan(sequences, sm.last_before, [&](int k) { return row_tiles(sm.order[k]); });
+    block_sync();
+    whole = sm.whole_before[sequences];
+    return (whole + sm.last_before[sequences]) * units;
   };
 
-  // The last sequence whose items start at or before i, 32 candidates at a time; then the item's place among its own.
-  auto item_at = [&](int i) {
-    int lo = 0, hi = sequences;
+  // The last i < n with before[i] <= x, 32 candidates at a time.
+  auto find = [&](const int* before, int n, int x) {
+    int lo = 0, hi = n;
+#pragma unroll 1
     while (hi - lo > 1) {
       const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-      const unsigned below = __ballot_sync(0xffffffffu, at < hi && sm.items[at] <= i);
+      const unsigned below = __ballot_sync(0xffffffffu, at < hi && before[at] <= x);
       lo += (31 - __clz(below)) * step;
       hi = min(lo + step, hi);
     }
-    Item x;
-    x.s = batch + lo; x.first = sm.first[lo]; x.count = sm.count[lo]; x.base = sm.base[lo];
-    const Spread spread = spread_of<kRows>(x.count, x.base, group, a.window, capacity);
-    const int local = i - sm.items[lo], rest = local / c.kv_heads, chunk = rest / spread.tiles;
-    x.kv_head = local - rest * c.kv_heads;
-    x.part = spread.first_part + chunk;
-    x.pair0 = (rest - chunk * spread.tiles) * kRows;
-    x.pairs = min(x.count * group - x.pair0, kRows);
-    const int top = clamp_keys(x.base + (x.pair0 + x.pairs - 1) / group, capacity);
-    const int low = a.window > 0 ? max(clamp_keys(x.base + x.pair0 / group, capacity) - a.window, 0) : 0;
-    const int from = max(low, x.part * kPartTokens);
-    x.end = min(top, (x.part + 1) * kPartTokens);
-    x.begin = from / kStageTokens * kStageTokens;
-    x.stages = x.end > from ? (x.end - x.begin + kStageTokens - 1) / kStageTokens : 0;
-    return x;
+    return lo;
   };
 
-  if (warp >= kConsumers) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegisters));
-    for (; batch < a.step.sequences; batch += kBatch) {
-      const int total = lay_out();
-      if (warp > kConsumers) continue;
-      // ---- producer: lane l holds pages and scales of the item's tiles l and l + 32 ----
+  auto item_at = [&](int batch, int i) {
+    const int cell = i / units, unit = i - cell * units;
+    int lo, local;
+    if (cell < whole) {
+      lo = find(sm.whole_before, sequences, cell);
+      local = cell - sm.whole_before[lo];
+    } else {
+      const int k = find(sm.last_before, sequences, cell - whole);
+      lo = sm.order[k];
+      local = cell - whole - sm.last_before[k];
+    }
+    Item x;
+    x.s = batch + lo; x.first = sm.first[lo]; x.count = sm.count[lo]; x.base = sm.base[lo];
+    const Spread spread = spread_of(kEach, x.count, x.base, group_heads, a.window, capacity);
+    const int chunk = cell < whole ? local / spread.tiles : spread.parts - 1;
+    x.unit = unit;
+    x.part = spread.first_part + chunk;
+    x.pair0 = (cell < whole ? local - chunk * spread.tiles : local) * kEach;
+    x.pairs = min(x.count * group_heads - x.pair0, kEach);
+    const int top = clamp_keys(x.base + (x.pair0 + x.pairs - 1) / group_heads, capacity);
+    const int low = a.window > 0 ? max(clamp_keys(x.base + x.pair0 / group_heads, capacity) - a.window, 0) : 0;
+    x.from = max(low, x.part * kPartTokens);
+    x.end = min(top, (x.part + 1) * kPartTokens);
+    x.all_from = max(a.window > 0 ? max(top - a.window, 0) : 0, x.from);
+    x.all_end = min(clamp_keys(x.base + x.pair0 / group_heads, capacity), x.end);
+    x.begin = x.from / kTile * kTile;
+    x.tiles = x.end > x.from ? (x.end - x.begin + kTile - 1) / kTile : 0;
+    return x;
+  };
+  auto group_of = [&](const Item& x, int j) { return (x.begin / kTile + j) & 1; };
+  auto tiles_of = [&](const Item& x, int group) { return (x.tiles + (group_of(x, 0) == group ? 1 : 0)) / 2; };
+  auto pass = [&](const Item& x) {
+    ++done_items;
+    done_tiles += x.tiles;
+    done_of[0] += tiles_of(x, 0);
+    done_of[1] += tiles_of(x, 1);
+  };
+
+#pragma unroll 1
+  for (int batch = 0; batch < a.step.sequences; batch += kBatch) {
+    const int total = lay_out(batch);
+    if (warp == kCopyWarp) {
+      static_assert(2 * kScaleSlots >= kSlots + 2, "tile n + kScaleSlots is copied after the values of tile n are done with");
+      // ---- copies: lane l has the pages of boxes l and l + 32 of an item (a part has up to 64 of 16 tokens), and the scales of its 16 tokens ----
       const uint64_t policy = policy_evict_first();
-      auto load_pages = [&](const Item& x, int (&page)[2]) {
+      int page[2], next_page[2];
+      float2 scales[kHeads][2], next_scales[kHeads][2];
+      auto load_pages = [&](const Item& x, int (&to)[2]) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int token = x.begin + 16 * (lane + 32 * k);
-          page[k] = x.stages > 0 && token < x.end ? a.step.tables[static_cast<int64_t>(x.s) * a.step.width + token / c.block] : -1;
+          to[k] = x.tiles > 0 && token < x.end && token + 16 > x.from ? a.step.tables[static_cast<int64_t>(x.s) * a.step.width + token / c.block] : -1;
         }
       };
       // a page outside the cache reads as zeros, which is what the copies of it bring too
-      auto load_scales = [&](const Item& x, const int (&page)[2], float (&ks)[2], float (&vs)[2]) {
+      auto load_scales = [&](const Item& x, const int (&of)[2], float2 (&to)[kHeads][2]) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const bool there = page[k] >= 0 && page[k] < c.num_pages;
-          ks[k] = there ? c.key_scale[page[k] * c.scale_stride + x.kv_head] : 0.0f;
-          vs[k] = there ? c.value_scale[page[k] * c.scale_stride + x.kv_head] : 0.0f;
+        for (int h = 0; h < kHeads; ++h) {
+          const int head = min(x.unit * kHeads + h, c.kv_heads - 1);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const bool there = of[k] >= 0 && of[k] < c.num_pages;
+            to[h][k].x = there ? c.key_scale[of[k] * c.scale_stride + head] : 0.0f;
+            to[h][k].y = there ? c.value_scale[of[k] * c.scale_stride + head] : 0.0f;
+          }
         }
       };
-      int page[2], next_page[2];
-      float ks[2], vs[2], next_ks[2], next_vs[2];
       Item x, next;
-      int i = blockIdx.x;
-      if (i < total) {
-        x = item_at(i);
-        load_pages(x, page);
-        load_scales(x, page, ks, vs);
-      }
-      while (i < total && !failed) {
-        const int i_next = i + gridDim.x;
+      x.tiles = 0;
+#pragma unroll 1
+      for (int i_next = blockIdx.x;; i_next += gridDim.x) {                // an item ahead of the copies
         const bool more = i_next < total;
         if (more) {
-          next = item_at(i_next);
+          next = item_at(batch, i_next);
           load_pages(next, next_page);
         }
-        bool scales_asked = false;
-        for (int j = 0; j < x.stages; ++j) {
-          const unsigned n = stage + j, slot = n % kSlots;
-          if (n >= kSlots && !mbar_wait(empty + 8 * slot, (n / kSlots - 1) & 1)) { failed = true; break; }
-          const int tile = 2 * j + (lane & 1), set = tile >> 5;
-          const bool mine = lane >> 1 == (j & 15) && x.begin + 16 * tile < x.end;
-          if (mine) {
-            // a scale that is no positive number within 2^-100 .. 2^100 is brought there: codes of a page of scale 0 then add nothing
-            const float v = fminf(fmaxf(set ? vs[1] : vs[0], 7.8886090522101181e-31f), 1.2676506002282294e30f);
-            sm.scales[slot][lane & 1] = make_float4(set ? ks[1] : ks[0], log2f(v), 1.0f / v, 0.0f);
+#pragma unroll 1
+        for (int j = 0; j < x.tiles && !failed; ++j) {
+          const unsigned n = done_tiles + j, scale_slot = n % kScaleSlots;
+          const int set = j >> 2, place = lane & 7;                        // tile j's 16-token pieces are 8j .. 8j + 7: lanes 8 (j & 3) .. of set j / 4
+          const int token = x.begin + j * kTile + 16 * place;
+          const bool holder = lane >> 3 == (j & 3);
+          const int id = set ? page[1] : page[0];
+          const bool copies = holder && token % box == 0 && token < x.end && token + box > x.from;
+          // the box's page is that of its first 16 tokens inside the visible range, which another lane may hold
+          const int skipped = token < x.from ? (x.from - token) / 16 : 0;
+          const int its_page = __shfl_sync(0xffffffffu, id, (lane & 24) + min(place + skipped, 7));
+          const uint32_t bytes = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, copies))) * box * 128;
+#pragma unroll
+          for (int values = 0; values < 2; ++values) {
+            const unsigned h = 2 * n + values, slot = h % kSlots;
+            if (h >= kSlots && !wait_for(&sm.empty[slot], (h / kSlots - 1) & 1)) { failed = true; break; }
+            if (values == 0) {
+              // The slots of the tile kScaleSlots before are free: its values gave theirs back before this tile's keys could be copied.
+              bool wide = false;
+              if (holder) {
+#pragma unroll
+                for (int k = 0; k < kHeads; ++k) {
+                  const float2 mine = set ? scales[k][1] : scales[k][0];
+                  // a scale that is no positive number within 2^-100 .. 2^100 is brought there: codes of a page of scale 0 then add nothing
+                  const float v = fminf(fmaxf(mine.y, 7.8886090522101181e-31f), 1.2676506002282294e30f);
+                  const int e = (__float_as_int(v) >> 23) - 127;
+                  const float significand = __int_as_float((__float_as_int(v) & 0x007fffff) | 0x3f800000);      // 1 for powers of two: exact then
+                  const float exponent = static_cast<float>(e) + __log2f(significand);
+                  wide |= fabsf(exponent) > kWide && token < x.end && token + 16 > x.from;
+                  sm.scales[scale_slot][k][place] = make_float4(mine.x, exponent, power_of_two(-e) * __frcp_rn(significand), 0.0f);
+                }
+              }
+              wide = __any_sync(0xffffffffu, wide);
+              if (lane == 0) sm.wide[scale_slot] = wide;
+            }
+            __syncwarp();                                                  // the scales are written
+            const uint32_t bar = smem_u32(&sm.full[slot]);
+            if (lane == 0) mbar_expect_tx(bar, bytes);
+            __syncwarp();
+            if (copies) tma_box(smem_u32(sm.ring[slot]) + place * 16 * 128, values ? &value_map : &key_map, x.unit * 128, token % c.block, its_page, bar, policy);
           }
           __syncwarp();
-          if (mine) {
-            const int token = x.begin + 16 * tile, at = token % c.block, id = set ? page[1] : page[0];
-            const uint32_t bar = full + 8 * slot, dst = smem_u32(&sm.stages[slot][lane & 1][0][0]);
-            if ((lane & 1) == 0) mbar_expect_tx(bar, (token + 16 < x.end ? 4 : 2) * kTileBytes);
-            if constexpr (kJoint) {
-              tma_tile_pair(dst, &key_map, at, x.kv_head, id, bar, policy);
-            } else {
-              tma_tile(dst, &key_map, at, x.kv_head, id, bar, policy);
-              tma_tile(dst + kTileBytes, &value_map, at, x.kv_head, id, bar, policy);
-            }
-          }
-          if (more && j == 2) { load_scales(next, next_page, next_ks, next_vs); scales_asked = true; }
         }
-        stage += x.stages;
         if (more) {
-          if (!scales_asked) load_scales(next, next_page, next_ks, next_vs);
-          x = next;
+          load_scales(next, next_page, next_scales);
 #pragma unroll
-          for (int k = 0; k < 2; ++k) { page[k] = next_page[k]; ks[k] = next_ks[k]; vs[k] = next_vs[k]; }
+          for (int k = 0; k < 2; ++k) {
+            page[k] = next_page[k];
+#pragma unroll
+            for (int h = 0; h < kHeads; ++h) scales[h][k] = next_scales[h][k];
+          }
         }
-        i = i_next;
+        done_tiles += x.tiles;
+        if (!more) break;
+        x = next;
       }
-    }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegisters));
-    for (; batch < a.step.sequences; batch += kBatch) {
-      const int total = lay_out();
-      // ---- consumers ----
-      for (int i = blockIdx.x; i < total; i += gridDim.x) {
-        const Item x = item_at(i);
-        // rows g and g + 8 of the item, as products of rows x tokens have them
-        int keys[2], low[2];
-        float row_scale[2];
-        uint32_t q[kSteps][kRowTiles * 2];
-#pragma unroll
-        for (int r = 0; r < kRowTiles; ++r) {
-          const int pair = x.pair0 + g + 8 * r;
-          const bool live = g + 8 * r < x.pairs;
-          const int row = (live ? pair : x.pair0) / group, head = x.kv_head * group + (live ? pair : x.pair0) - row * group;
-          keys[r] = live ? clamp_keys(x.base + row, capacity) : capacity;       // rows that are none see everything, and nothing is masked for them
-          low[r] = live && a.window > 0 ? max(keys[r] - a.window, 0) : 0;
-          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (x.first + row) * a.q_stride + static_cast<int64_t>(head) * kD + kD / 4 * t);
-          uint4 raw[kD / 32];
-#pragma unroll
-          for (int k = 0; k < kD / 32; ++k) raw[k] = live ? src[k] : make_uint4(0u, 0u, 0u, 0u);
-          float largest = 0.0f;
-#pragma unroll
-          for (int k = 0; k < kD / 32; ++k) {
-            const T* e = reinterpret_cast<const T*>(&raw[k]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) largest = fmaxf(largest, fabsf(Elem<T>::to_float(e[j])));
-          }
-          largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-          largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-          const int e = largest < INFINITY && largest > 0.0f ? min(max((__float_as_int(largest) >> 23) - 127, -126), 126) : 0;
-          const float down = power_of_two(-e);
-          row_scale[r] = scale_log2 * power_of_two(e);
-#pragma unroll
-          for (int k = 0; k < kD / 32; ++k) {
-            const T* el = reinterpret_cast<const T*>(&raw[k]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)            // element pairs 2j, 2j + 1: k step 2k + j / 2, first or second k half
-              q[2 * k + (j >> 1)][(j & 1) * kRowTiles + r] = pack2<false>(Elem<T>::to_float(el[2 * j]) * down, Elem<T>::to_float(el[2 * j + 1]) * down);
-          }
-        }
-        const int top_keys = clamp_keys(x.base + (x.pair0 + x.pairs - 1) / group, capacity), least_keys = clamp_keys(x.base + x.pair0 / group, capacity);
-        const int least_low = a.window > 0 ? max(least_keys - a.window, 0) : 0, top_low = a.window > 0 ? max(top_keys - a.window, 0) : 0;
-
-        float o[kSteps][kRowTiles][4];
-#pragma unroll
-        for (int m = 0; m < kSteps; ++m)
-#pragma unroll
-          for (int r = 0; r < kRowTiles; ++r) { o[m][r][0] = 0.f; o[m][r][1] = 0.f; o[m][r][2] = 0.f; o[m][r][3] = 0.f; }
-        float ref[kRowTiles], l[kRowTiles];
-#pragma unroll
-        for (int r = 0; r < kRowTiles; ++r) { ref[r] = -INFINITY; l[r] = 0.f; }
-        float largest_scale = -INFINITY;
-
-        const int first_stage = x.begin / kStageTokens;                  // of all the context's: the warp of a stage goes by its position
-        for (int j = (warp - first_stage) & (kConsumers - 1); j < x.stages; j += kConsumers) {
-          const unsigned n = stage + j, slot = n % kSlots;
-          if (failed ? !mbar_try_wait(full + 8 * slot, (n / kSlots) & 1) : !mbar_wait(full + 8 * slot, (n / kSlots) & 1)) failed = true;
-          if (!failed) {
-            const int token0 = x.begin + j * kStageTokens;
-            const bool two = token0 + 16 < x.end;
-            const uint32_t tile_at[2] = {smem_u32(&sm.stages[slot][0][0][0]), smem_u32(&sm.stages[slot][1][0][0])};
-            // scores, in log2 units and relative to the row's reference
-            float s[2][2][4];
-            float inverse[2], log2_scale[2];
-            bool far[2] = {false, false};        // values so much smaller than others' that their weights pass below fp32, but not their keys' share of l
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              if (u == 1 && !two) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) { s[1][0][k] = -INFINITY; s[1][1][k] = -INFINITY; }
-                inverse[1] = 0.0f;
-                break;
-              }
-              const uint32_t keys_at = tile_at[u] + (key_first ? 0 : kTileBytes);
-#pragma unroll
-              for (int k = 0; k < 4; ++k) { s[u][0][k] = 0.f; s[u][1][k] = 0.f; }
-#pragma unroll
-              for (int h = 0; h < kD / 64; ++h) {
-                uint32_t w[2][4];
-#pragma unroll
-                for (int n8 = 0; n8 < 2; ++n8) {
-                  const int token = token_of<kD>(g) + 8 * n8;
-                  const uint32_t chunk = kD == 128 ? static_cast<uint32_t>((2 * t + h) ^ (token & 7)) : static_cast<uint32_t>(t ^ ((token >> 1) & 3));
-                  const uint4 v = load_shared16(keys_at + token * kD + chunk * 16);
-                  w[n8][0] = v.x; w[n8][1] = v.y; w[n8][2] = v.z; w[n8][3] = v.w;
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  uint32_t qa[4];
-                  qa[0] = q[4 * h + k][0];
-                  qa[1] = kRowTiles == 2 ? q[4 * h + k][1] : 0u;
-                  qa[2] = q[4 * h + k][kRowTiles];
-                  qa[3] = kRowTiles == 2 ? q[4 * h + k][kRowTiles + 1] : 0u;
-#pragma unroll
-                  for (int n8 = 0; n8 < 2; ++n8) mma_16816<false>(s[u][n8], qa, halves_low(w[n8][k]), halves_high(w[n8][k]));
-                }
-              }
-              const float4 scales = sm.scales[slot][u];
-              inverse[u] = scales.z;
-              log2_scale[u] = scales.y;
-              largest_scale = fmaxf(largest_scale, scales.y);
-              far[u] = scales.y < largest_scale - 60.0f;
-#pragma unroll
-              for (int r = 0; r < kRowTiles; ++r) {
-                const float factor = row_scale[r] * scales.x, shift = scales.y - (ref[r] == -INFINITY ? 0.0f : ref[r]);
-#pragma unroll
-                for (int n8 = 0; n8 < 2; ++n8) {
-                  s[u][n8][2 * r] = fmaf(s[u][n8][2 * r], factor, shift);
-                  s[u][n8][2 * r + 1] = fmaf(s[u][n8][2 * r + 1], factor, shift);
-                }
-              }
-              const int tile0 = token0 + 16 * u;
-              if (tile0 + 16 > least_keys || tile0 < top_low) {
-#pragma unroll
-                for (int n8 = 0; n8 < 2; ++n8) {
-#pragma unroll
-                  for (int k = 0; k < 2; ++k) {
-                    const int token = tile0 + token_of<kD>(2 * t + k) + 8 * n8;
-#pragma unroll
-                    for (int r = 0; r < kRowTiles; ++r)
-                      if (token >= keys[r] || token < low[r]) s[u][n8][2 * r + k] = -INFINITY;
-                  }
-                }
-              }
-            }
-            // a row's reference moves when a weight would pass 2^kHighest
-            float top[kRowTiles];
-            bool moves = false;
-#pragma unroll
-            for (int r = 0; r < kRowTiles; ++r) {
-              top[r] = fmaxf(fmaxf(fmaxf(s[0][0][2 * r], s[0][0][2 * r + 1]), fmaxf(s[0][1][2 * r], s[0][1][2 * r + 1])),
-                             fmaxf(fmaxf(s[1][0][2 * r], s[1][0][2 * r + 1]), fmaxf(s[1][1][2 * r], s[1][1][2 * r + 1])));
-              moves |= top[r] > (ref[r] == -INFINITY ? -INFINITY : kHighest);
-            }
-            if (__any_sync(0xffffffffu, moves)) {
-#pragma unroll
-              for (int r = 0; r < kRowTiles; ++r) {
-                float most = top[r];
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                const bool fresh = ref[r] == -INFINITY, move = most > (fresh ? -INFINITY : kHighest);
-                const float by = move ? most - kFresh : 0.0f, root = move && !fresh ? exp2f(-0.5f * by) : 1.0f, keep = root * root;
-                if (move) ref[r] = (fresh ? 0.0f : ref[r]) + by;
-                l[r] = l[r] * root * root;            // in two steps: where a page of far larger values moved the reference, keep may be 0 in fp32 and l not
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                  for (int n8 = 0; n8 < 2; ++n8) { s[u][n8][2 * r] -= by; s[u][n8][2 * r + 1] -= by; }
-                const float keep0 = __shfl_sync(0xffffffffu, keep, 8 * t), keep1 = __shfl_sync(0xffffffffu, keep, 8 * t + 4);
-#pragma unroll
-                for (int m = 0; m < kSteps; ++m) { o[m][r][0] *= keep0; o[m][r][1] *= keep1; o[m][r][2] *= keep0; o[m][r][3] *= keep1; }
-              }
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              if (u == 1 && !two) break;
-              uint32_t p[kRowTiles][2];
-#pragma unroll
-              for (int r = 0; r < kRowTiles; ++r) {
-                const float p0 = fast_exp2(s[u][0][2 * r]), p1 = fast_exp2(s[u][0][2 * r + 1]), p2 = fast_exp2(s[u][1][2 * r]), p3 = fast_exp2(s[u][1][2 * r + 1]);
-                if (!far[u]) {
-                  l[r] = fmaf((p0 + p1) + (p2 + p3), inverse[u], l[r]);
-                } else {
-                  const float back = log2_scale[u];
-                  l[r] += (fast_exp2(s[u][0][2 * r] - back) + fast_exp2(s[u][0][2 * r + 1] - back)) +
-                          (fast_exp2(s[u][1][2 * r] - back) + fast_exp2(s[u][1][2 * r + 1] - back));
-                }
-                p[r][0] = pack2<false>(p0, p1);
-                p[r][1] = pack2<false>(p2, p3);
-              }
-              // values of tokens 2t, 2t + 1 and the same of the upper eight, elements g * kD / 8 ..
-              const uint32_t values_at = tile_at[u] + (key_first ? kTileBytes : 0);
-              uint32_t w[4][kD / 32];
-              int tokens[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const int token = tokens[k] = token_of<kD>(2 * t + (k & 1)) + 8 * (k >> 1);
-                if constexpr (kD == 128) {
-                  const uint4 v = load_shared16(values_at + token * kD + ((g ^ (token & 7)) << 4));
-                  w[k][0] = v.x; w[k][1] = v.y; w[k][2] = v.z; w[k][3] = v.w;
-                } else {
-                  const uint2 v = load_shared8(values_at + token * kD + (((g >> 1) ^ ((token >> 1) & 3)) << 4) + (g & 1) * 8);
-                  w[k][0] = v.x; w[k][1] = v.y;
-                }
-              }
-              const int tile0 = token0 + 16 * u;
-              if (tile0 + 16 > least_keys || tile0 < top_low) {
-                // Slots that no row of the item sees may hold anything, and a weight of zero times NaN is NaN: they are cleared.  NaN that some
-                // rows see and others do not goes to those that do, by a product of its own over ones.
-                uint32_t nans = 0;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const bool seen = tile0 + tokens[k] < top_keys && tile0 + tokens[k] >= least_low;
-#pragma unroll
-                  for (int j = 0; j < kD / 32; ++j) {
-                    if (!seen) w[k][j] = 0u;
-                    nans |= nan_codes(w[k][j]);
-                  }
-                }
-                if (__any_sync(0xffffffffu, nans != 0u)) {
-                  uint32_t sees[kRowTiles][2];
-#pragma unroll
-                  for (int r = 0; r < kRowTiles; ++r) {
-#pragma unroll
-                    for (int n8 = 0; n8 < 2; ++n8) {
-                      const int at0 = tile0 + token_of<kD>(2 * t) + 8 * n8, at1 = tile0 + token_of<kD>(2 * t + 1) + 8 * n8;
-                      sees[r][n8] = (at0 < keys[r] && at0 >= low[r] ? 0x3c00u : 0u) | (at1 < keys[r] && at1 >= low[r] ? 0x3c000000u : 0u);
-                    }
-                  }
-#pragma unroll
-                  for (int j = 0; j < kD / 32; ++j) {
-                    uint32_t ones[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                      const uint32_t marks = nan_codes(w[k][j]) >> 7;
-                      ones[k] = marks * 0x38u;
-                      w[k][j] &= ~(marks * 0xffu);
-                    }
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                      const uint32_t x0 = __byte_perm(ones[0], ones[1], half ? 0x7362 : 0x5140), x1 = __byte_perm(ones[2], ones[3], half ? 0x7362 : 0x5140);
-                      const uint32_t va[4] = {halves_low(x0), halves_high(x0), halves_low(x1), halves_high(x1)};
-#pragma unroll
-                      for (int r = 0; r < kRowTiles; ++r) {
-                        float hits[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma_16816<false>(hits, va, sees[r][0], sees[r][1]);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                          if (hits[k] > 0.0f) o[2 * j + half][r][k] = NAN;
-                      }
-                    }
-                  }
-                }
-              }
-#pragma unroll
-              for (int j = 0; j < kD / 32; ++j) {
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                  const uint32_t x0 = __byte_perm(w[0][j], w[1][j], half ? 0x7362 : 0x5140), x1 = __byte_perm(w[2][j], w[3][j], half ? 0x7362 : 0x5140);
-                  const uint32_t va[4] = {halves_low(x0), halves_high(x0), halves_low(x1), halves_high(x1)};
-#pragma unroll
-                  for (int r = 0; r < kRowTiles; ++r) mma_16816<false>(o[2 * j + half][r], va, p[r][0], p[r][1]);
-                }
-              }
-            }
-          }
-          __syncwarp();          // every lane's reads are done
-          if (lane == 0) mbar_arrive(empty + 8 * slot);
-        }
-
-        // the warps' sums, in the order of the warps
-        if (((warp - first_stage) & (kConsumers - 1)) < x.stages) {
-          constexpr int kMine = kD / 8;                                  // elements g * kMine .. of rows 2t, 2t + 1 of each tile
-#pragma unroll
-          for (int r = 0; r < kRowTiles; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            if (t == 0) {
-              sm.sums[warp][8 * r + g][kD] = failed ? 0.0f : ref[r];
-              sm.sums[warp][8 * r + g][kD + 1] = failed ? NAN : l[r];
-            }
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-              for (int m = 0; m < kSteps; m += 2)
-                *reinterpret_cast<float4*>(&sm.sums[warp][8 * r + 2 * t + k][g * kMine + 2 * m]) =
-                    make_float4(o[m][r][k], o[m][r][k + 2], o[m + 1][r][k], o[m + 1][r][k + 2]);
-          }
-        }
-        consumers_sync();
+    } else if (warp == kScoreWarp) {
+      // ---- S^T of a tile, once its keys and the item's queries are there and its group has read the scores of the tile before ----
+      constexpr uint32_t kIdesc = (1u << 4) | (static_cast<uint32_t>(kN >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
+#pragma unroll 1
+      for (int i = blockIdx.x; i < total && !failed; i += gridDim.x) {
+        const unsigned parity = done_items & 1;
+        bool ok = wait_for(&sm.q_full[parity], (done_items >> 1) & 1);
+        const Item x = sm.item[parity];
         {
-          constexpr int kPerRow = kConsumers * 32 / kRows, kEach = kD / kPerRow;
-          static_assert(kEach % 2 == 0, "whole pairs of elements per thread");
-          const int r = threadIdx.x / kPerRow, d0 = (threadIdx.x % kPerRow) * kEach;
-          if (r < x.pairs) {
-            const int pair = x.pair0 + r, row = pair / group, head = x.kv_head * group + pair - row * group;
-            const int row_keys = clamp_keys(x.base + row, capacity), row_low = a.window > 0 ? max(row_keys - a.window, 0) : 0;
-            const int first_part = row_low / kPartTokens, last_part = row_keys > 0 ? (row_keys - 1) / kPartTokens : first_part;
-            if (x.part >= first_part && x.part <= last_part) {
-              float big = -INFINITY;
+          const uint64_t q_desc = umma_desc(smem_u32(sm.q[parity]), 16, 1024);
+          unsigned of[kGroups] = {done_of[0], done_of[1]};
+#pragma unroll 1
+          for (int j = 0; j < x.tiles; ++j) {
+            const int group = group_of(x, j);
+            const unsigned h = 2 * (done_tiles + j), slot = h % kSlots, mine = group ? of[1] : of[0];
+            ok = ok && (mine == 0 || wait_for(&sm.s_free[group], (mine - 1) & 1));
+            ok = ok && wait_for(&sm.full[slot], (h / kSlots) & 1);
+            if (!__all_sync(0xffffffffu, ok)) { failed = true; break; }
+            tcgen05_after_sync();
+            const uint64_t k_desc = umma_desc(smem_u32(sm.ring[slot]), 16, 1024);
+            if (elect_one()) {
 #pragma unroll
-              for (int w = 0; w < kConsumers; ++w)
-                if (((w - first_stage) & (kConsumers - 1)) < x.stages) big = fmaxf(big, sm.sums[w][r][kD]);
-              const float zero = big == -INFINITY ? 0.0f : big;
-              float sum = 0.0f, acc[kEach];
+              for (int ks = 0; ks < 4; ++ks)
+                code_product(tmem + kScores + group * 64, k_desc + static_cast<uint64_t>(ks * 2), q_desc + static_cast<uint64_t>(ks * 2), kIdesc, ks > 0);
+              umma_commit(smem_u32(&sm.s_ready[group]));
+              umma_commit(smem_u32(&sm.empty[slot]));
+            }
+            __syncwarp();
+            if (group) ++of[1]; else ++of[0];
+          }
+        }
+        if (!__all_sync(0xffffffffu, ok)) failed = true;
+        if (elect_one()) umma_commit(smem_u32(&sm.q_empty[parity]));
+        __syncwarp();
+        pass(x);
+      }
+    } else if (warp == kValueWarp) {
+      // ---- O^T of a tile, once its group's weights are there; its completion gives the stage back ----
+      constexpr uint32_t kIdesc = (1u << 4) | (1u << 15) | (static_cast<uint32_t>(kN >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
+#pragma unroll 1
+      for (int i = blockIdx.x; i < total && !failed; i += gridDim.x) {
+        const unsigned parity = done_items & 1;
+        if (!__all_sync(0xffffffffu, wait_for(&sm.q_full[parity], (done_items >> 1) & 1))) { failed = true; break; }
+        const Item x = sm.item[parity];        // (held until the groups are done with the item, which needs these products)
+#pragma unroll 1
+        for (int j = 0; j < x.tiles; ++j) {
+          const int group = group_of(x, j);
+          const unsigned h = 2 * (done_tiles + j) + 1, slot = h % kSlots, mine = (group ? done_of[1] : done_of[0]) + j / 2;
+          if (!__all_sync(0xffffffffu, wait_for(&sm.full[slot], (h / kSlots) & 1) && wait_for(&sm.p_ready[group], mine & 1))) { failed = true; break; }
+          tcgen05_after_sync();
+          const uint64_t v_desc = umma_desc(smem_u32(sm.ring[slot]), kTileBytes, 1024), p_desc = umma_desc(smem_u32(sm.p[group]), 16, 1024);
+          if (elect_one()) {
 #pragma unroll
-              for (int k = 0; k < kEach; ++k) acc[k] = 0.0f;
+            for (int ks = 0; ks < 4; ++ks)
+              code_product(tmem + kOutputs + group * 64, v_desc + static_cast<uint64_t>(ks * 4096 >> 4), p_desc + static_cast<uint64_t>(ks * 2), kIdesc,
+                           (j >= 2 || ks > 0) ? 1u : 0u);
+            umma_commit(smem_u32(&sm.o_done[group]));
+            umma_commit(smem_u32(&sm.empty[slot]));
+          }
+          __syncwarp();
+        }
+        pass(x);
+      }
+    } else if (warp == kQueryWarp) {
+      // ---- the queries of an item in three parts, and what its rows see ----
+#pragma unroll 1
+      for (int i = blockIdx.x; i < total && !failed; i += gridDim.x) {
+        const Item x = item_at(batch, i);
+        const unsigned parity = done_items & 1;
+        if (done_items >= 2 && !__all_sync(0xffffffffu, wait_for(&sm.q_empty[parity], ((done_items >> 1) - 1) & 1))) { failed = true; break; }
+        constexpr int kMine = kDim / 32;            // elements of a lane
+        // lane r has row r's place in the item
+        const int my_head = x.unit * kHeads + lane % kRows / kEach, my_pair = x.pair0 + lane % kEach, my_row = my_pair / group_heads;
+        const bool my_live = lane % kEach < x.pairs && my_head < c.kv_heads;
+        const int64_t head = static_cast<int64_t>(my_head) * group_heads + my_pair - my_row * group_heads, at_row = x.first + my_row;
+        const int64_t my_source = my_live ? at_row * a.q_stride + head * kDim : -1;
+        // all rows on their way at once, a lane's kMine elements of each
+#pragma unroll 1
+        for (int r = 0; r < kRows; ++r) {
+          const int64_t source = __shfl_sync(0xffffffffu, my_source, r);
+          const T* src = static_cast<const T*>(a.q) + (source < 0 ? 0 : source) + lane * kMine;
+          asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(smem_u32(&sm.raw_q[r][lane * (kMine / 2)])), "l"(src), "n"(kMine * 2), "r"(source < 0 ? 0 : kMine * 2) : "memory");
+        }
+        asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
+        __syncwarp();
+#pragma unroll 1
+        for (int r = 0; r < kRows; ++r) {
+          {
+            uint32_t raw[kMine / 2];
 #pragma unroll
-              for (int w = 0; w < kConsumers; ++w) {
-                if (((w - first_stage) & (kConsumers - 1)) >= x.stages) continue;
-                const float* from = sm.sums[w][r];
-                const float root = exp2f(0.5f * (from[kD] - zero)), f = root * root;
-                sum += from[kD + 1] * root * root;
+            for (int w = 0; w < kMine / 2; ++w) raw[w] = sm.raw_q[r][lane * (kMine / 2) + w];
+            float v[kMine], largest = 0.0f;
+            bool odd = false;                       // a row with an element that is not finite has no scores that are: its references, and so its output, become NaN
 #pragma unroll
-                for (int k = 0; k < kEach; k += 2) {
-                  const float2 v = *reinterpret_cast<const float2*>(from + d0 + k);
-                  acc[k] = fmaf(v.x, f, acc[k]);
-                  acc[k + 1] = fmaf(v.y, f, acc[k + 1]);
-                }
-              }
-              const int64_t at = static_cast<int64_t>(x.first + row) * a.q_heads + head;
-              if (first_part == last_part) {
-                const float scale = row_keys > row_low ? 1.0f / sum : 0.0f;
-                uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (x.first + row) * a.out_stride + static_cast<int64_t>(head) * kD + d0);
+            for (int w = 0; w < kMine; ++w) {
+              v[w] = Elem<T>::to_float(reinterpret_cast<const T*>(raw)[w]);
+              largest = fmaxf(largest, fabsf(v[w]));
+              odd |= !(fabsf(v[w]) < INFINITY);
+            }
 #pragma unroll
-                for (int k = 0; k < kEach; k += 2) out[k / 2] = pack2<std::is_same<T, __nv_bfloat16>::value>(acc[k] * scale, acc[k + 1] * scale);
+            for (int y = 16; y > 0; y >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, y));
+            odd = __any_sync(0xffffffffu, odd);
+            const int e = largest > 0.0f && !odd ? max((__float_as_int(largest) >> 23) - 127 - 7, -126) : 0;
+            const float up = odd ? 0.0f : power_of_two(-e);
+            if (lane == 0) sm.row_scale[parity][r] = odd ? NAN : scale_log2 * power_of_two(e);
+            uint32_t codes[kMine / 2][3];
+#pragma unroll
+            for (int w = 0; w < kMine / 2; ++w) three_parts(odd ? 0.0f : v[2 * w] * up, odd ? 0.0f : v[2 * w + 1] * up, codes[w]);
+            // element lane * kMine of a 128-byte line whose 16-byte pieces are swizzled by the row; of two heads, the other's half of the line is zero
+            const uint32_t line = smem_u32(sm.q[parity]) + r * 128;
+            const int byte = (kHeads == 2 ? (r / kEach) * 64 : 0) + lane * kMine;
+            const uint32_t at = line + (byte ^ ((r & 7) << 4));
+#pragma unroll
+            for (int part = 0; part < 3; ++part) {
+              if constexpr (kDim == 128) {
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + part * kRows * 128), "r"(codes[0][part] | codes[kMine / 2 - 1][part] << 16) : "memory");
               } else {
-                float* partial = a.partials + (at * a.parts + x.part - first_part) * partial_stride(kD);
-#pragma unroll
-                for (int k = 0; k < kEach; k += 2) *reinterpret_cast<float2*>(partial + d0 + k) = make_float2(acc[k], acc[k + 1]);
-                if (d0 == 0) *reinterpret_cast<float2*>(partial + kD) = make_float2(big, sum);
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"(at + part * kRows * 128), "h"(static_cast<uint16_t>(codes[0][part])) : "memory");
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"((at ^ 64u) + part * kRows * 128), "h"(static_cast<uint16_t>(0)) : "memory");
               }
             }
           }
         }
-        consumers_sync();        // the sums are read before the next item's are written
-        stage += x.stages;
+        if (lane < kRows) {
+          const int sees = clamp_keys(x.base + my_row, capacity), low = a.window > 0 ? max(sees - a.window, 0) : 0;
+          const int first_part = low / kPartTokens, last_part = sees > 0 ? (sees - 1) / kPartTokens : first_part;
+          sm.keys[parity][lane] = my_live ? min(sees, x.end) : x.end;          // of the part; rows that are none see all of it, and nothing is masked for them
+          sm.low[parity][lane] = my_live ? max(low, x.from) : x.from;
+          int kind = kNowhere;
+          if (my_live && x.part >= first_part && x.part <= last_part) kind = first_part < last_part ? kPartial : (sees > low ? kOutput : kZero);
+          sm.kind[parity][lane] = kind;
+          sm.to[parity][lane] = kind == kPartial ? ((at_row * a.q_heads + head) * a.parts + x.part - first_part) * partial_stride(kDim) : at_row * a.out_stride + head * kDim;
+        }
+        if (lane == 0) sm.item[parity] = x;
+        fence_async_proxy();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.q_full[parity]));
+        pass(x);
+      }
+    } else {
+      // ---- softmax: a thread has a token and half of the rows (of two heads: one head's); in the end an element of the values and the same rows ----
+      constexpr int kMine = kRows / 2;
+      const int group = warp >> 3, half = (warp >> 2) & 1, own = threadIdx.x & (kTile - 1), row0 = half * kMine;
+      const int head_slot = kHeads == 2 ? half : 0;
+      const uint32_t lanes = (static_cast<uint32_t>((warp & 3) * 32) << 16) + group * 64 + row0;
+      const uint32_t scores_at = tmem + lanes + kScores, outputs_at = tmem + lanes + kOutputs;
+      // where this thread's weights go: rows of 128 tokens, 16-byte pieces swizzled by the row (a half's first row is a multiple of its rows)
+      const uint32_t weights = smem_u32(sm.p[group]) + row0 * 128 + (own & 15), piece = static_cast<uint32_t>((own >> 4) ^ (row0 & 7)) << 4;
+      const int folded_row = row0 + row_after_fold<kMine>(lane);
+      const bool folds = lane % (32 / kMine) == 0;
+#pragma unroll 1
+      for (int i = blockIdx.x; i < total; i += gridDim.x) {
+        const unsigned parity = done_items & 1;
+        failed = group_any(group, failed || !wait_for(&sm.q_full[parity], (done_items >> 1) & 1));
+        const Item x = sm.item[parity];
+        const int mine = tiles_of(x, group);
+        const unsigned before = group ? done_of[1] : done_of[0];
+        float ref[kMine], l[kMine];
+#pragma unroll
+        for (int r = 0; r < kMine; ++r) { ref[r] = 0.0f; l[r] = 0.0f; }
+        uint32_t fresh = (1u << kMine) - 1;          // rows without a reference yet
+        if (own == 0) { sm.fresh[group][half] = fresh; sm.moved[group][half] = 0xffffffffu; }      // (read behind barriers)
+        bool marked = false;                         // nan_value has something of this item
+        bool wide = false;                           // so has a tile had a scale beyond 2^+-kWide
+#pragma unroll 1
+        for (int k = 0; k < mine; ++k) {
+          const int j = 2 * k + (group_of(x, 0) == group ? 0 : 1);
+          const unsigned h = 2 * (done_tiles + j) + 1, turn = before + k, scale_slot = (done_tiles + j) % kScaleSlots;
+          const int token0 = x.begin + j * kTile, token = token0 + own;
+          // The tile's scales are there with its keys and its values.  Only the values can be waited for: they keep their place until this group's
+          // weights have met them, while that of the keys may have been filled again (and its barrier be a whole turn on).
+          if (!failed && !(wait_for(&sm.s_ready[group], turn & 1) && wait_for(&sm.full[h % kSlots], (h / kSlots) & 1))) failed = true;
+          __syncwarp();
+          tcgen05_after_sync();
+          float s[kMine], m[kMine], rest[kMine];
+          load_columns<kMine>(scores_at, s);
+          load_columns<kMine>(scores_at + kRows, m);
+          load_columns<kMine>(scores_at + 2 * kRows, rest);
+          const float4 scale = load_shared16f(smem_u32(&sm.scales[scale_slot][head_slot][own >> 4]));
+          wide |= sm.wide[scale_slot] != 0;
+          tmem_load_wait();
+          tcgen05_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sm.s_free[group]));
+#pragma unroll
+          for (int r = 0; r < kMine; r += 4) {
+            const float4 row_scale = load_shared16f(smem_u32(&sm.row_scale[parity][row0 + r]));
+            const float2 part = make_float2(0.03125f, 0.03125f), keys_scale = make_float2(scale.x, scale.x), exponent = make_float2(scale.y, scale.y);
+#pragma unroll
+            for (int i2 = 0; i2 < 4; i2 += 2) {
+              float2 raw = fma_pair(make_float2(rest[r + i2], rest[r + i2 + 1]), part, make_float2(m[r + i2], m[r + i2 + 1]));
+              raw = fma_pair(raw, part, make_float2(s[r + i2], s[r + i2 + 1]));
+              const float2 factor = mul_pair(i2 ? make_float2(row_scale.z, row_scale.w) : make_float2(row_scale.x, row_scale.y), keys_scale);
+              raw = fma_pair(raw, factor, sub_pair(exponent, make_float2(ref[r + i2], ref[r + i2 + 1])));
+              s[r + i2] = raw.x;
+              s[r + i2 + 1] = raw.y;
+            }
+          }
+          const bool ragged = token0 + kTile > x.all_end || token0 < x.all_from;
+          if (ragged) {
+#pragma unroll
+            for (int r = 0; r < kMine; ++r)
+              if (token >= sm.keys[parity][row0 + r] || token < sm.low[parity][row0 + r]) s[r] = -INFINITY;
+          }
+          float top = fmaxf(s[0], s[1]);
+#pragma unroll
+          for (int r = 2; r < kMine; r += 2) top = max3(top, s[r], s[r + 1]);
+          // (the first tile, and rows that have not seen a key: always; the other half's rows need it as well)
+          if (group_any(group, top > kHighest || fresh != 0)) {
+            {
+              float most[kMine];
+#pragma unroll
+              for (int r = 0; r < kMine; ++r) most[r] = s[r];
+              const float folded = fold_rows<kMine, true>(most, lane);
+              if (folds) sm.folded[group][warp & 3][folded_row] = folded;
+            }
+            group_any(group, false);
+            if (own < kMine) {                     // a row each
+              const int r = row0 + own;
+              const float most = fmaxf(fmaxf(sm.folded[group][0][r], sm.folded[group][1][r]), fmaxf(sm.folded[group][2][r], sm.folded[group][3][r]));
+              const bool first = (fresh >> own) & 1, move = most > (first ? -INFINITY : kHighest);
+              const float by = move ? most - kFresh : 0.0f;
+              sm.by[group][r] = by;
+              sm.root[group][r] = move ? (first ? 0.0f : fast_exp2(-0.5f * by)) : 1.0f;     // 0: there is nothing yet
+              if (move && first) atomicAnd(&sm.fresh[group][half], ~(1u << own));
+              if (move && !first) sm.moved[group][half] = turn;
+            }
+            group_any(group, false);
+            fresh = sm.fresh[group][half];
+#pragma unroll
+            for (int r = 0; r < kMine; ++r) {
+              const float by = sm.by[group][row0 + r], root = sm.root[group][row0 + r];
+              ref[r] += by;
+              s[r] -= by;
+              l[r] = l[r] * root * root;           // in two steps: where a page of far larger values moved the reference, the whole factor may be 0 in fp32 and l not
+            }
+            const bool moves = sm.moved[group][half] == turn;
+            if (moves && k > 0) {                  // the same for the warps of a half; the output is at rest once the product before is complete
+              if (!failed && !wait_for(&sm.o_done[group], (turn - 1) & 1)) failed = true;
+              __syncwarp();
+              tcgen05_after_sync();
+#pragma unroll
+              for (int part = 0; part < 3; ++part) {
+                float o[kMine];
+                load_columns<kMine>(outputs_at + part * kRows, o);
+                tmem_load_wait();
+#pragma unroll
+                for (int r = 0; r < kMine; ++r) o[r] *= sm.root[group][row0 + r] * sm.root[group][row0 + r];
+                store_columns<kMine>(outputs_at + part * kRows, o);
+              }
+              tmem_store_wait();
+              tcgen05_before_sync();
+            }
+          }
+          uint32_t codes[kMine / 2][3];
+#pragma unroll
+          for (int r = 0; r < kMine; r += 2) {
+            float2 p;
+            if (!wide) {
+              p = make_float2(fast_exp2(s[r]), fast_exp2(s[r + 1]));
+              const float2 sum = fma_pair(p, make_float2(scale.z, scale.z), make_float2(l[r], l[r + 1]));
+              l[r] = sum.x;
+              l[r + 1] = sum.y;
+            } else {
+              // a weight that is nothing beside the largest may still be a share of l, where its page's values are that much smaller
+              const bool faint0 = s[r] < kFaint, faint1 = s[r + 1] < kFaint;
+              p = make_float2(fast_exp2(faint0 ? s[r] - scale.y : s[r]), fast_exp2(faint1 ? s[r + 1] - scale.y : s[r + 1]));
+              l[r] = fmaf(p.x, faint0 ? 1.0f : scale.z, l[r]);
+              l[r + 1] = fmaf(p.y, faint1 ? 1.0f : scale.z, l[r + 1]);
+              if (faint0) p.x = 0.0f;
+              if (faint1) p.y = 0.0f;
+            }
+            three_parts(p.x, p.y, codes[r / 2]);
+          }
+          if (turn > 0) {                          // the product before has read the weights (it is long done)
+            if (!failed && !wait_for(&sm.o_done[group], (turn - 1) & 1)) failed = true;
+            __syncwarp();
+          }
+#pragma unroll
+          for (int r = 0; r < kMine; r += 2) {
+            const uint32_t at0 = weights + (piece ^ (r << 4)), at1 = weights + (piece ^ ((r + 1) << 4));
+#pragma unroll
+            for (int k3 = 0; k3 < 3; ++k3) {
+              store_shared1(at0 + (k3 * kRows + r) * 128, codes[r / 2][k3]);
+              store_shared1(at1 + (k3 * kRows + r + 1) * 128, codes[r / 2][k3] >> 8);
+            }
+          }
+          if (ragged) {
+            // Slots that no row of the item sees may hold anything, and a weight of zero times NaN is NaN: they are cleared.  NaN in a token that some
+            // rows see and others do not is cleared too, and kept for those that do.  The two threads of a token take 64 bytes each.
+            unsigned char* value = sm.ring[h % kSlots] + own * 128;
+            const bool seen = token >= x.from && token < x.end;
+#pragma unroll 1
+            for (int b = 4 * half; b < 4 * half + 4; ++b) {
+              uint4* at = reinterpret_cast<uint4*>(value + ((b ^ (own & 7)) << 4));
+              const uint4 w = *at;
+              if (!seen) {
+                *at = make_uint4(0u, 0u, 0u, 0u);
+              } else if (nan_codes(w.x) | nan_codes(w.y) | nan_codes(w.z) | nan_codes(w.w)) {
+                marked = true;
+                uint32_t* words = reinterpret_cast<uint32_t*>(at);
+#pragma unroll 1
+                for (int k4 = 0; k4 < 4; ++k4) {
+                  const uint32_t marks = nan_codes(words[k4]) >> 7;
+                  const uint32_t bits = (marks & 1) | ((marks >> 7) & 2) | ((marks >> 14) & 4) | ((marks >> 21) & 8);
+#pragma unroll 1
+                  for (int r = 0; r < kRows; ++r)
+                    if ((kHeads == 1 || r / kEach == b / 4) && token < sm.keys[parity][r] && token >= sm.low[parity][r])
+                      atomicOr(&sm.nan_value[group][r][b >> 1], bits << (16 * (b & 1) + 4 * k4));
+                  words[k4] &= ~(marks * 0xffu);
+                }
+              }
+            }
+          }
+          fence_async_proxy();
+          tcgen05_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sm.p_ready[group]));
+        }
+
+        // the group's sums: the second one leaves them in shared memory, the first joins them with its own
+        float o[kMine];
+#pragma unroll
+        for (int r = 0; r < kMine; ++r) o[r] = 0.0f;
+        if (mine > 0) {
+          const float total = fold_rows<kMine, false>(l, lane);
+          if (folds) sm.folded[group][warp & 3][folded_row] = total;
+          if (!failed && !wait_for(&sm.o_done[group], (before + mine - 1) & 1)) failed = true;
+          marked = group_any(group, marked);
+          __syncwarp();
+          tcgen05_after_sync();
+          float m[kMine], rest[kMine];
+          load_columns<kMine>(outputs_at, o);
+          load_columns<kMine>(outputs_at + kRows, m);
+          load_columns<kMine>(outputs_at + 2 * kRows, rest);
+          tmem_load_wait();
+          tcgen05_before_sync();
+#pragma unroll
+          for (int r = 0; r < kMine; ++r) {
+            o[r] = fmaf(fmaf(rest[r], 0.03125f, m[r]), 0.03125f, o[r]);
+            if (marked && (sm.nan_value[group][row0 + r][own >> 5] >> (own & 31)) & 1) o[r] = NAN;
+            l[r] = (sm.folded[group][0][row0 + r] + sm.folded[group][1][row0 + r]) + (sm.folded[group][2][row0 + r] + sm.folded[group][3][row0 + r]);
+            if (failed) { o[r] = NAN; l[r] = NAN; }
+          }
+          group_any(group, false);                 // folded and nan_value have been read
+          if (marked && own < kMine) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) sm.nan_value[group][row0 + own][b] = 0u;
+          }
+        }
+        if (group == 1) {
+          if (mine > 0) {
+#pragma unroll
+            for (int r = 0; r < kMine; ++r) {
+              sm.sums[parity][row0 + r][own] = o[r];
+              if (own == 0) {
+                sm.other_ref[parity][row0 + r] = (fresh >> r) & 1 ? -INFINITY : ref[r];
+                sm.other_l[parity][row0 + r] = l[r];
+              }
+            }
+          }
+          sums_ready(parity);
+        } else {
+          sums_wait(parity);
+          // a row's factors by one thread: 2^(R - max R) of each group, over the joined sum where this is the row's only part
+          const bool others = tiles_of(x, 1) > 0;
+          if (own < kMine) {
+            const int row = row0 + own, kind = sm.kind[parity][row];
+            float mine_ref = -INFINITY, mine_l = 0.0f;
+#pragma unroll
+            for (int r = 0; r < kMine; ++r) {
+              if (own == r) {
+                mine_ref = (fresh >> r) & 1 ? -INFINITY : ref[r];
+                mine_l = l[r];
+              }
+            }
+            const float other_ref = others ? sm.other_ref[parity][row] : -INFINITY, other_l = others ? sm.other_l[parity][row] : 0.0f;
+            const float big = fmaxf(mine_ref, other_ref), zero = big == -INFINITY ? 0.0f : big;
+            const float root0 = fast_exp2(0.5f * (mine_ref - zero)), root1 = fast_exp2(0.5f * (other_ref - zero));
+            const float sum = mine_l * root0 * root0 + other_l * root1 * root1;
+            const float scale = kind == kPartial ? 1.0f : (kind == kOutput ? __frcp_rn(sum) : 0.0f);
+            sm.factor[0][row] = root0 * root0 * scale;
+            sm.factor[1][row] = root1 * root1 * scale;
+            if (kind == kPartial) *reinterpret_cast<float2*>(a.partials + sm.to[parity][row] + kDim) = make_float2(big, sum);
+          }
+          group_any(group, false);
+          const int d = kHeads == 2 ? own - 64 * half : own;      // of two heads, a thread's element may be the other one's
+          if (d >= 0 && d < kDim) {
+#pragma unroll
+            for (int r = 0; r < kMine; ++r) {
+              const int kind = sm.kind[parity][row0 + r];
+              float acc = o[r] * sm.factor[0][row0 + r];
+              if (others) acc = fmaf(sm.sums[parity][row0 + r][own], sm.factor[1][row0 + r], acc);
+              const int64_t to = sm.to[parity][row0 + r] + d;
+              if (kind == kPartial) a.partials[to] = acc;
+              else if (kind != kNowhere) static_cast<T*>(a.out)[to] = Elem<T>::from_float(acc);
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.q_empty[parity]));
+        pass(x);
       }
     }
   }
   // a wait that gave up left NaN; copies still in flight land before the shared memory is given back
-  if (failed && warp < kConsumers)
+  if (failed && warp == kCopyWarp)
     for (int i = 0; i < kSlots; ++i)
-      if (!mbar_wait(full + 8 * i, 0) && !mbar_wait(full + 8 * i, 1)) break;
+      if (!wait_for(&sm.full[i], 0) && !wait_for(&sm.full[i], 1)) break;
+  tcgen05_before_sync();
+  __syncthreads();
+  if (warp == kScoreWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns) : "memory");
 }
 
 // ---- host ---------------------------------------------------------------------------------------
-// One cache as [pages][kv_heads][block][dim] bytes in boxes of 16 tokens of one head; with `distance` both caches, that far apart, as one tensor
-// whose boxes hold a tile of each.
-int make_tile_map(CUtensorMap* map, const void* base, const QuantizedCache& c, uint64_t distance) {
+// A cache as [pages][tokens][bytes of all heads], in boxes of 128 bytes and `box` tokens, swizzled; heads behind the last read as zeros.
+int make_code_map(CUtensorMap* map, const void* base, const QuantizedCache& c, int box) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (fn == nullptr) return RLT_ERR_UNSUPPORTED;
-  cuuint64_t dims[5], strides[4];
-  cuuint32_t box[5], element[5] = {1, 1, 1, 1, 1};
-  int rank = 0;
-  auto add = [&](uint64_t size, uint64_t stride, uint32_t in_box) {
-    dims[rank] = size;
-    box[rank] = in_box;
-    if (rank > 0) strides[rank - 1] = stride;
-    ++rank;
-  };
-  add(c.dim, 1, c.dim);
-  add(c.block, c.token_stride, 16);
-  add(c.kv_heads, c.dim, 1);
-  if (distance != 0) add(2, distance, 2);
-  add(c.num_pages, c.block_stride, 1);
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, element, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        c.dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(c.kv_heads) * c.dim, static_cast<cuuint64_t>(c.block), static_cast<cuuint64_t>(c.num_pages)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(c.token_stride), static_cast<cuuint64_t>(c.block_stride)};
+  const cuuint32_t in_box[3] = {128, static_cast<cuuint32_t>(box), 1}, element[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, in_box, element, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? RLT_OK : RLT_ERR_UNSUPPORTED;
 }
 
-template <typename T, int kD, int kRowTiles>
+template <typename T, int kDim, int kRows>
 int launch(const QuantizedAttentionArgs& a, cudaStream_t stream) {
   const QuantizedCache& c = a.cache;
   DeviceInfo info;
   int status = current_device_info(&info);
   if (status != RLT_OK) return status;
-  const uintptr_t k = reinterpret_cast<uintptr_t>(c.key), v = reinterpret_cast<uintptr_t>(c.value);
-  const bool key_first = k < v;
-  const uint64_t distance = key_first ? v - k : k - v;
+  int box = 16;                                     // tokens of a copy: as many as a page and a tile share
+  while (box < kTile && c.block % (2 * box) == 0) box *= 2;
   CUtensorMap key_map, value_map;
-  const bool joint = distance != 0 && distance % 16 == 0 && distance < (1ull << 40) &&
-                     make_tile_map(&key_map, key_first ? c.key : c.value, c, distance) == RLT_OK;
-  if (joint) {
-    value_map = key_map;
-  } else if (make_tile_map(&key_map, c.key, c, 0) != RLT_OK || make_tile_map(&value_map, c.value, c, 0) != RLT_OK) {
-    return RLT_ERR_UNSUPPORTED;
-  }
-  const size_t smem = sizeof(Shared<kD, kRowTiles>) + 1024;
-  auto kernel = joint ? quantized_tiles_kernel<T, kD, kRowTiles, true> : quantized_tiles_kernel<T, kD, kRowTiles, false>;
+  if (make_code_map(&key_map, c.key, c, box) != RLT_OK || make_code_map(&value_map, c.value, c, box) != RLT_OK) return RLT_ERR_UNSUPPORTED;
+  const size_t smem = sizeof(Shared<kRows>) + 1024;
+  auto kernel = quantized_tiles_kernel<T, kDim, kRows>;
   RLT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
   return launch_dependent("quantized_tiles_kernel", kernel, dim3(static_cast<unsigned>(info.sm_count)), dim3(kThreads), smem, stream, key_map, value_map, a,
-                          static_cast<float>(1.4426950408889634 * a.scale), joint && !key_first ? 0 : 1);
+                          static_cast<float>(1.4426950408889634 * a.scale), box);
 }
 
 template <typename T>
 int launch_for(const QuantizedAttentionArgs& a, int max_new, cudaStream_t stream) {
-  // up to eight rows an item: half the registers and products
-  const bool few = static_cast<int64_t>(max_new) * (a.q_heads / a.cache.kv_heads) <= 8;
-  if (a.cache.dim == 128) return few ? launch<T, 128, 1>(a, stream) : launch<T, 128, 2>(a, stream);
-  return few ? launch<T, 64, 1>(a, stream) : launch<T, 64, 2>(a, stream);
+  // Rows of an item: half the columns where a portion's rows fit (two heads of 64 share an item's rows).
+  const int64_t pairs = static_cast<int64_t>(max_new) * (a.q_heads / a.cache.kv_heads) * (128 / a.cache.dim);
+  if (a.cache.dim == 128) return pairs <= 8 ? launch<T, 128, 8>(a, stream) : launch<T, 128, 16>(a, stream);
+  return pairs <= 8 ? launch<T, 64, 8>(a, stream) : launch<T, 64, 16>(a, stream);
 }
 
 }  // namespace
@@ -667,8 +923,8 @@ bool quantized_tiles_supported(const QuantizedAttentionArgs& a) {
   const QuantizedCache& c = a.cache;
   if (a.dtype == RLT_F32 || (c.dim != 64 && c.dim != 128) || c.block % 16 != 0 || c.num_pages < 1 || c.num_pages > 0x7fffffff) return false;
   if (c.token_stride % 16 != 0 || c.block_stride % 16 != 0 || !aligned16(c.key) || !aligned16(c.value)) return false;
-  if (a.q_stride % 8 != 0 || !aligned16(a.q) || a.out_stride % 2 != 0 || (reinterpret_cast<uintptr_t>(a.out) & 3u) != 0) return false;
-  const int64_t group = a.q_heads / c.kv_heads, tiles = (static_cast<int64_t>(a.step.rows) * group + 7) / 8 + a.step.sequences;
+  if (a.q_stride % 4 != 0 || (reinterpret_cast<uintptr_t>(a.q) & 7u) != 0) return false;
+  const int64_t group = a.q_heads / c.kv_heads, tiles = (static_cast<int64_t>(a.step.rows) * group + 3) / 4 + a.step.sequences;
   return tiles * c.kv_heads * a.parts <= 0x7fffffff && static_cast<int64_t>(a.step.rows) * group <= 0x7fffffff;     // items are counted in 32 bits
 }
 
