@@ -34,8 +34,11 @@ namespace {
 constexpr int kGroups = 2;
 constexpr int kGroupThreads = 256;      // two threads per token, each with half of the rows
 constexpr int kGroupWarps = kGroupThreads / 32;
-constexpr int kThreads = kGroups * kGroupThreads + 128;       // and copies, S^T, O^T, queries
-constexpr int kCopyWarp = 16, kScoreWarp = 17, kValueWarp = 18, kQueryWarp = 19;
+constexpr int kCopyWarps = 4;           // each copies the same quarter of every tile
+constexpr int kCopyWarp = 16, kScoreWarp = 20, kValueWarp = 21, kQueryWarp = 22;
+constexpr int kThreads = 768;           // two groups; four warps that copy, those of S^T, O^T and the queries, and one that is none
+constexpr int kSoftmaxRegisters = 96, kControlRegisters = 48;
+static_assert(kGroups * kGroupThreads * kSoftmaxRegisters + 256 * kControlRegisters <= kThreads * 80, "what a block of this size is launched with");
 constexpr int kTile = 128;              // tokens
 constexpr int kTileBytes = kTile * 128; // of keys, or of values
 constexpr int kSlots = 10;              // tiles of keys or of values in the ring, in turn
@@ -80,8 +83,9 @@ struct __align__(1024) Shared {
   int kind[2][kRows];                                 // kNowhere, kOutput, kZero, kPartial
   Item item[2];
   uint32_t nan_value[kGroups][kRows][4];              // elements that a row gets NaN in
+  int marked[kGroups];                                // there are some
   float4 scales[kScaleSlots][2][kTile / 16];          // by head and 16 tokens: key scale, log2 of the value scale, its inverse
-  int wide[kScaleSlots];                              // a value scale of the tile beyond 2^+-kWide
+  int4 wide[kScaleSlots];                             // a value scale of the tile beyond 2^+-kWide; from each copy warp
   unsigned long long full[kSlots], empty[kSlots], q_full[2], q_empty[2], s_ready[kGroups], s_free[kGroups], p_ready[kGroups], o_done[kGroups];
   uint32_t tmem_base;
   // the work of a batch of sequences: cells (part, row tile) of whole parts in front of a sequence; then the last parts, largest first
@@ -95,10 +99,16 @@ struct __align__(1024) Shared {
 // instruction caches (with unrolled polls at every wait they did not, and every phase took three to ten times as long).
 __device__ __forceinline__ bool wait_for(const unsigned long long* barrier, uint32_t parity) {
   const uint32_t bar = smem_u32(barrier);
-  if (mbar_try_wait(bar, parity)) return true;
+  const auto poll = [&]() {              // suspended for up to 10 us at a time, so that waiting warps leave the issue slots to the others
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(10000u) : "memory");
+    return ok != 0;
+  };
+  if (poll()) return true;
   const long long begin = clock64();
 #pragma unroll 1
-  while (!mbar_try_wait(bar, parity))
+  while (!poll())
     if (clock64() - begin > kWaitCycles) return false;
   return true;
 }
@@ -231,7 +241,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kSlots; ++i) { mbar_init(smem_u32(&sm.full[i]), 1); mbar_init(smem_u32(&sm.empty[i]), 1); }
+    for (int i = 0; i < kSlots; ++i) { mbar_init(smem_u32(&sm.full[i]), kCopyWarps); mbar_init(smem_u32(&sm.empty[i]), 1); }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&sm.q_full[i]), 1);
       mbar_init(smem_u32(&sm.q_empty[i]), 1 + kGroups * kGroupWarps);             // the products' completion, and each softmax warp
@@ -244,6 +254,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   }
 #pragma unroll 1
   for (int i = threadIdx.x; i < kGroups * kRows * 4; i += kThreads) (&sm.nan_value[0][0][0])[i] = 0u;
+  if (threadIdx.x < kGroups) sm.marked[threadIdx.x] = 0;
   grid_dependency_wait();
   grid_dependency_release();
   tcgen05_before_sync();
@@ -371,35 +382,22 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     done_of[1] += tiles_of(x, 1);
   };
 
+  // (a loop for each: what runs with a kind's registers stays apart from the other's)
+  if (warp >= kCopyWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegisters));
 #pragma unroll 1
-  for (int batch = 0; batch < a.step.sequences; batch += kBatch) {
+    for (int batch = 0; batch < a.step.sequences; batch += kBatch) {
     const int total = lay_out(batch);
-    if (warp == kCopyWarp) {
+    if (warp >= kCopyWarp && warp < kCopyWarp + kCopyWarps) {
       static_assert(2 * kScaleSlots >= kSlots + 2, "tile n + kScaleSlots is copied after the values of tile n are done with");
-      // ---- copies: lane l has the pages of boxes l and l + 32 of an item (a part has up to 64 of 16 tokens), and the scales of its 16 tokens ----
+      // ---- copies: warp w has pieces 2w and 2w + 1 (16 tokens each) of every tile, lane 2j + i pages and scales of piece 2w + i of tile j of an item ----
+      // What a copy costs is its issue: one warp alone, at four or five cycles for each of its instructions, took 2600 cycles a tile.
       const uint64_t policy = policy_evict_first();
-      int page[2], next_page[2];
-      float2 scales[kHeads][2], next_scales[kHeads][2];
-      auto load_pages = [&](const Item& x, int (&to)[2]) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int token = x.begin + 16 * (lane + 32 * k);
-          to[k] = x.tiles > 0 && token < x.end && token + 16 > x.from ? a.step.tables[static_cast<int64_t>(x.s) * a.step.width + token / c.block] : -1;
-        }
-      };
-      // a page outside the cache reads as zeros, which is what the copies of it bring too
-      auto load_scales = [&](const Item& x, const int (&of)[2], float2 (&to)[kHeads][2]) {
-#pragma unroll
-        for (int h = 0; h < kHeads; ++h) {
-          const int head = min(x.unit * kHeads + h, c.kv_heads - 1);
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const bool there = of[k] >= 0 && of[k] < c.num_pages;
-            to[h][k].x = there ? c.key_scale[of[k] * c.scale_stride + head] : 0.0f;
-            to[h][k].y = there ? c.value_scale[of[k] * c.scale_stride + head] : 0.0f;
-          }
-        }
-      };
+      constexpr int kUnseen = static_cast<int>(0x80000000);               // a piece of a box that no row sees
+      const int quarter = warp - kCopyWarp;
+      const bool leads0 = ((32 * quarter) & (box - 1)) == 0, leads1 = box == 16;      // the pieces that a box starts with
+      int page, place, next_page = kUnseen, next_place = 0;
+      float4 scales[kHeads];                                              // as the softmax takes them; w: beyond 2^+-kWide
       Item x, next;
       x.tiles = 0;
 #pragma unroll 1
@@ -407,58 +405,63 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         const bool more = i_next < total;
         if (more) {
           next = item_at(batch, i_next);
-          load_pages(next, next_page);
+          const int token = next.begin + (lane >> 1) * kTile + 32 * quarter + 16 * (lane & 1), entry = token / c.block;
+          const bool seen = lane < 2 * next.tiles && (token & -box) < next.end && (token | (box - 1)) >= next.from;      // (a box lies in one page)
+          next_place = token - entry * c.block;
+          next_page = seen ? a.step.tables[static_cast<int64_t>(next.s) * a.step.width + entry] : kUnseen;
         }
 #pragma unroll 1
         for (int j = 0; j < x.tiles && !failed; ++j) {
           const unsigned n = done_tiles + j, scale_slot = n % kScaleSlots;
-          const int set = j >> 2, place = lane & 7;                        // tile j's 16-token pieces are 8j .. 8j + 7: lanes 8 (j & 3) .. of set j / 4
-          const int token = x.begin + j * kTile + 16 * place;
-          const bool holder = lane >> 3 == (j & 3);
-          const int id = set ? page[1] : page[0];
-          const bool copies = holder && token % box == 0 && token < x.end && token + box > x.from;
-          // the box's page is that of its first 16 tokens inside the visible range, which another lane may hold
-          const int skipped = token < x.from ? (x.from - token) / 16 : 0;
-          const int its_page = __shfl_sync(0xffffffffu, id, (lane & 24) + min(place + skipped, 7));
-          const uint32_t bytes = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, copies))) * box * 128;
-#pragma unroll
+          const int page0 = __shfl_sync(0xffffffffu, page, 2 * j), page1 = __shfl_sync(0xffffffffu, page, 2 * j + 1);
+          const int place0 = __shfl_sync(0xffffffffu, place, 2 * j), place1 = place0 + 16;
+          const bool copy0 = leads0 && page0 != kUnseen, copy1 = leads1 && page1 != kUnseen;
+          // (in a page of 16 tokens the second piece starts the next page)
+          const int in_page1 = place1 == c.block ? 0 : place1;
+          const uint32_t bytes = static_cast<uint32_t>((copy0 ? 1 : 0) + (copy1 ? 1 : 0)) * box * 128;
+#pragma unroll 1
           for (int values = 0; values < 2; ++values) {
             const unsigned h = 2 * n + values, slot = h % kSlots;
             if (h >= kSlots && !wait_for(&sm.empty[slot], (h / kSlots - 1) & 1)) { failed = true; break; }
             if (values == 0) {
               // The slots of the tile kScaleSlots before are free: its values gave theirs back before this tile's keys could be copied.
               bool wide = false;
-              if (holder) {
+              if ((lane >> 1) == j) {
 #pragma unroll
                 for (int k = 0; k < kHeads; ++k) {
-                  const float2 mine = set ? scales[k][1] : scales[k][0];
-                  // a scale that is no positive number within 2^-100 .. 2^100 is brought there: codes of a page of scale 0 then add nothing
-                  const float v = fminf(fmaxf(mine.y, 7.8886090522101181e-31f), 1.2676506002282294e30f);
-                  const int e = (__float_as_int(v) >> 23) - 127;
-                  const float significand = __int_as_float((__float_as_int(v) & 0x007fffff) | 0x3f800000);      // 1 for powers of two: exact then
-                  const float exponent = static_cast<float>(e) + __log2f(significand);
-                  wide |= fabsf(exponent) > kWide && token < x.end && token + 16 > x.from;
-                  sm.scales[scale_slot][k][place] = make_float4(mine.x, exponent, power_of_two(-e) * __frcp_rn(significand), 0.0f);
+                  wide |= scales[k].w != 0.0f;
+                  sm.scales[scale_slot][k][2 * quarter + (lane & 1)] = scales[k];
                 }
               }
               wide = __any_sync(0xffffffffu, wide);
-              if (lane == 0) sm.wide[scale_slot] = wide;
+              if (lane == 0) reinterpret_cast<int*>(&sm.wide[scale_slot])[quarter] = wide;
+              __syncwarp();                                                // the scales are written
             }
-            __syncwarp();                                                  // the scales are written
-            const uint32_t bar = smem_u32(&sm.full[slot]);
-            if (lane == 0) mbar_expect_tx(bar, bytes);
+            if (lane == 0) {
+              const uint32_t bar = smem_u32(&sm.full[slot]), dst = smem_u32(sm.ring[slot]) + quarter * 4096;
+              const CUtensorMap* map = values ? &value_map : &key_map;
+              mbar_expect_tx(bar, bytes);
+              if (copy0) tma_box(dst, map, x.unit * 128, place0, page0, bar, policy);
+              if (copy1) tma_box(dst + 2048, map, x.unit * 128, in_page1, page1, bar, policy);
+            }
             __syncwarp();
-            if (copies) tma_box(smem_u32(sm.ring[slot]) + place * 16 * 128, values ? &value_map : &key_map, x.unit * 128, token % c.block, its_page, bar, policy);
           }
-          __syncwarp();
         }
         if (more) {
-          load_scales(next, next_page, next_scales);
+          page = next_page;
+          place = next_place;
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            page[k] = next_page[k];
-#pragma unroll
-            for (int h = 0; h < kHeads; ++h) scales[h][k] = next_scales[h][k];
+          for (int h = 0; h < kHeads; ++h) {
+            const int head = min(next.unit * kHeads + h, c.kv_heads - 1);
+            // a page outside the cache reads as zeros, which is what the copies of it bring too
+            const bool there = next_page >= 0 && next_page < c.num_pages;
+            const float key = there ? c.key_scale[next_page * c.scale_stride + head] : 0.0f, value = there ? c.value_scale[next_page * c.scale_stride + head] : 1.0f;
+            // a scale that is no positive number within 2^-100 .. 2^100 is brought there: codes of a page of scale 0 then add nothing
+            const float v = fminf(fmaxf(value, 7.8886090522101181e-31f), 1.2676506002282294e30f);
+            const int e = (__float_as_int(v) >> 23) - 127;
+            const float significand = __int_as_float((__float_as_int(v) & 0x007fffff) | 0x3f800000);      // 1 for powers of two: exact then
+            const float exponent = static_cast<float>(e) + __log2f(significand);
+            scales[h] = make_float4(key, exponent, power_of_two(-e) * __frcp_rn(significand), fabsf(exponent) > kWide ? 1.0f : 0.0f);
           }
         }
         done_tiles += x.tiles;
@@ -604,7 +607,13 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         if (lane == 0) mbar_arrive(smem_u32(&sm.q_full[parity]));
         pass(x);
       }
-    } else {
+    }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
+#pragma unroll 1
+    for (int batch = 0; batch < a.step.sequences; batch += kBatch) {
+      const int total = lay_out(batch);
       // ---- softmax: a thread has a token and half of the rows (of two heads: one head's); in the end an element of the values and the same rows ----
       constexpr int kMine = kRows / 2;
       const int group = warp >> 3, half = (warp >> 2) & 1, own = threadIdx.x & (kTile - 1), row0 = half * kMine;
@@ -618,7 +627,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
 #pragma unroll 1
       for (int i = blockIdx.x; i < total; i += gridDim.x) {
         const unsigned parity = done_items & 1;
-        failed = group_any(group, failed || !wait_for(&sm.q_full[parity], (done_items >> 1) & 1));
+        failed = group_any(group, failed || ((warp & 7) == 0 && !wait_for(&sm.q_full[parity], (done_items >> 1) & 1)));
         const Item x = sm.item[parity];
         const int mine = tiles_of(x, group);
         const unsigned before = group ? done_of[1] : done_of[0];
@@ -627,7 +636,6 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         for (int r = 0; r < kMine; ++r) { ref[r] = 0.0f; l[r] = 0.0f; }
         uint32_t fresh = (1u << kMine) - 1;          // rows without a reference yet
         if (own == 0) { sm.fresh[group][half] = fresh; sm.moved[group][half] = 0xffffffffu; }      // (read behind barriers)
-        bool marked = false;                         // nan_value has something of this item
         bool wide = false;                           // so has a tile had a scale beyond 2^+-kWide
 #pragma unroll 1
         for (int k = 0; k < mine; ++k) {
@@ -636,15 +644,20 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           const int token0 = x.begin + j * kTile, token = token0 + own;
           // The tile's scales are there with its keys and its values.  Only the values can be waited for: they keep their place until this group's
           // weights have met them, while that of the keys may have been filled again (and its barrier be a whole turn on).
-          if (!failed && !(wait_for(&sm.s_ready[group], turn & 1) && wait_for(&sm.full[h % kSlots], (h / kSlots) & 1))) failed = true;
-          __syncwarp();
+          // One warp waits, for the product before as well (it has read the weights that this tile's replace, and its result is at rest then); the
+          // others wait for it at the group's barrier, which costs no issue slots.
+          bool ok = true;
+          if ((warp & 7) == 0 && !failed)
+            ok = wait_for(&sm.s_ready[group], turn & 1) && wait_for(&sm.full[h % kSlots], (h / kSlots) & 1) && (turn == 0 || wait_for(&sm.o_done[group], (turn - 1) & 1));
+          if (group_any(group, !ok)) failed = true;
           tcgen05_after_sync();
           float s[kMine], m[kMine], rest[kMine];
           load_columns<kMine>(scores_at, s);
           load_columns<kMine>(scores_at + kRows, m);
           load_columns<kMine>(scores_at + 2 * kRows, rest);
           const float4 scale = load_shared16f(smem_u32(&sm.scales[scale_slot][head_slot][own >> 4]));
-          wide |= sm.wide[scale_slot] != 0;
+          const int4 any_wide = sm.wide[scale_slot];
+          wide |= (any_wide.x | any_wide.y | any_wide.z | any_wide.w) != 0;
           tmem_load_wait();
           tcgen05_before_sync();
           __syncwarp();
@@ -702,10 +715,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
               l[r] = l[r] * root * root;           // in two steps: where a page of far larger values moved the reference, the whole factor may be 0 in fp32 and l not
             }
             const bool moves = sm.moved[group][half] == turn;
-            if (moves && k > 0) {                  // the same for the warps of a half; the output is at rest once the product before is complete
-              if (!failed && !wait_for(&sm.o_done[group], (turn - 1) & 1)) failed = true;
-              __syncwarp();
-              tcgen05_after_sync();
+            if (moves && k > 0) {                  // the same for the warps of a half
 #pragma unroll
               for (int part = 0; part < 3; ++part) {
                 float o[kMine];
@@ -739,10 +749,6 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             }
             three_parts(p.x, p.y, codes[r / 2]);
           }
-          if (turn > 0) {                          // the product before has read the weights (it is long done)
-            if (!failed && !wait_for(&sm.o_done[group], (turn - 1) & 1)) failed = true;
-            __syncwarp();
-          }
 #pragma unroll
           for (int r = 0; r < kMine; r += 2) {
             const uint32_t at0 = weights + (piece ^ (r << 4)), at1 = weights + (piece ^ ((r + 1) << 4));
@@ -764,7 +770,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
               if (!seen) {
                 *at = make_uint4(0u, 0u, 0u, 0u);
               } else if (nan_codes(w.x) | nan_codes(w.y) | nan_codes(w.z) | nan_codes(w.w)) {
-                marked = true;
+                sm.marked[group] = 1;
                 uint32_t* words = reinterpret_cast<uint32_t*>(at);
 #pragma unroll 1
                 for (int k4 = 0; k4 < 4; ++k4) {
@@ -792,9 +798,9 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         if (mine > 0) {
           const float total = fold_rows<kMine, false>(l, lane);
           if (folds) sm.folded[group][warp & 3][folded_row] = total;
-          if (!failed && !wait_for(&sm.o_done[group], (before + mine - 1) & 1)) failed = true;
-          marked = group_any(group, marked);
-          __syncwarp();
+          bool ok = true;
+          if ((warp & 7) == 0 && !failed) ok = wait_for(&sm.o_done[group], (before + mine - 1) & 1);
+          if (group_any(group, !ok)) failed = true;
           tcgen05_after_sync();
           float m[kMine], rest[kMine];
           load_columns<kMine>(outputs_at, o);
@@ -803,27 +809,35 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           tmem_load_wait();
           tcgen05_before_sync();
 #pragma unroll
-          for (int r = 0; r < kMine; ++r) {
-            o[r] = fmaf(fmaf(rest[r], 0.03125f, m[r]), 0.03125f, o[r]);
-            if (marked && (sm.nan_value[group][row0 + r][own >> 5] >> (own & 31)) & 1) o[r] = NAN;
-            l[r] = (sm.folded[group][0][row0 + r] + sm.folded[group][1][row0 + r]) + (sm.folded[group][2][row0 + r] + sm.folded[group][3][row0 + r]);
-            if (failed) { o[r] = NAN; l[r] = NAN; }
-          }
-          group_any(group, false);                 // folded and nan_value have been read
-          if (marked && own < kMine) {
+          for (int r = 0; r < kMine; ++r) o[r] = fmaf(fmaf(rest[r], 0.03125f, m[r]), 0.03125f, o[r]);
+          if (sm.marked[group]) {                  // set behind barriers, the same for all
 #pragma unroll
-            for (int b = 0; b < 4; ++b) sm.nan_value[group][row0 + own][b] = 0u;
+            for (int r = 0; r < kMine; ++r)
+              if ((sm.nan_value[group][row0 + r][own >> 5] >> (own & 31)) & 1) o[r] = NAN;
+            group_any(group, false);               // nan_value has been read
+            if (own < kMine) {
+#pragma unroll
+              for (int b = 0; b < 4; ++b) sm.nan_value[group][row0 + own][b] = 0u;
+            }
+            if (own == 0) sm.marked[group] = 0;
           }
+        }
+        // a row's reference and sum, by a thread each
+        float own_ref = -INFINITY, own_l = 0.0f;
+        if (mine > 0 && own < kMine) {
+          own_l = (sm.folded[group][0][row0 + own] + sm.folded[group][1][row0 + own]) + (sm.folded[group][2][row0 + own] + sm.folded[group][3][row0 + own]);
+#pragma unroll
+          for (int r = 0; r < kMine; ++r)
+            if (own == r && !((fresh >> r) & 1)) own_ref = ref[r];
+          if (failed) own_l = NAN;
         }
         if (group == 1) {
           if (mine > 0) {
 #pragma unroll
-            for (int r = 0; r < kMine; ++r) {
-              sm.sums[parity][row0 + r][own] = o[r];
-              if (own == 0) {
-                sm.other_ref[parity][row0 + r] = (fresh >> r) & 1 ? -INFINITY : ref[r];
-                sm.other_l[parity][row0 + r] = l[r];
-              }
+            for (int r = 0; r < kMine; ++r) sm.sums[parity][row0 + r][own] = o[r];
+            if (own < kMine) {
+              sm.other_ref[parity][row0 + own] = own_ref;
+              sm.other_l[parity][row0 + own] = own_l;
             }
           }
           sums_ready(parity);
@@ -833,18 +847,10 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           const bool others = tiles_of(x, 1) > 0;
           if (own < kMine) {
             const int row = row0 + own, kind = sm.kind[parity][row];
-            float mine_ref = -INFINITY, mine_l = 0.0f;
-#pragma unroll
-            for (int r = 0; r < kMine; ++r) {
-              if (own == r) {
-                mine_ref = (fresh >> r) & 1 ? -INFINITY : ref[r];
-                mine_l = l[r];
-              }
-            }
             const float other_ref = others ? sm.other_ref[parity][row] : -INFINITY, other_l = others ? sm.other_l[parity][row] : 0.0f;
-            const float big = fmaxf(mine_ref, other_ref), zero = big == -INFINITY ? 0.0f : big;
-            const float root0 = fast_exp2(0.5f * (mine_ref - zero)), root1 = fast_exp2(0.5f * (other_ref - zero));
-            const float sum = mine_l * root0 * root0 + other_l * root1 * root1;
+            const float big = fmaxf(own_ref, other_ref), zero = big == -INFINITY ? 0.0f : big;
+            const float root0 = fast_exp2(0.5f * (own_ref - zero)), root1 = fast_exp2(0.5f * (other_ref - zero));
+            const float sum = own_l * root0 * root0 + other_l * root1 * root1;
             const float scale = kind == kPartial ? 1.0f : (kind == kOutput ? __frcp_rn(sum) : 0.0f);
             sm.factor[0][row] = root0 * root0 * scale;
             sm.factor[1][row] = root1 * root1 * scale;
@@ -871,7 +877,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     }
   }
   // a wait that gave up left NaN; copies still in flight land before the shared memory is given back
-  if (failed && warp == kCopyWarp)
+  if (failed && warp >= kCopyWarp && warp < kCopyWarp + kCopyWarps)
     for (int i = 0; i < kSlots; ++i)
       if (!wait_for(&sm.full[i], 0) && !wait_for(&sm.full[i], 1)) break;
   tcgen05_before_sync();
