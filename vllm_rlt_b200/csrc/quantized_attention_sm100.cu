@@ -19,8 +19,8 @@
 //
 // Roles.  Two groups of eight warps take tiles of 128 tokens in turn, each with scores, weights, references and sums of its own; one warp issues
 // S^T products, one O^T products, one the copies (a ring of tiles that runs on across items; keys give their place back before their values),
-// one prepares the queries of the next item.  The second group's sums are joined with the first's.  Which group a tile belongs to goes by its
-// position, so a row's bits do not depend on the batch or on the other rows of its item.
+// two prepare the queries of the next items.  Which group a tile belongs to goes by its
+// position, so a row's bits do not depend on the batch or on the other rows of its item.  Four warps write the results; three items are under way.
 //
 // Bound by the bytes of keys and values.
 #include <cuda.h>
@@ -35,10 +35,12 @@ constexpr int kGroups = 2;
 constexpr int kGroupThreads = 256;      // two threads per token, each with half of the rows
 constexpr int kGroupWarps = kGroupThreads / 32;
 constexpr int kCopyWarps = 4;           // each copies the same quarter of every tile
-constexpr int kCopyWarp = 16, kScoreWarp = 20, kValueWarp = 21, kQueryWarp = 22;
-constexpr int kThreads = 768;           // two groups; four warps that copy, those of S^T, O^T and the queries, and one that is none
-constexpr int kSoftmaxRegisters = 96, kControlRegisters = 48;
-static_assert(kGroups * kGroupThreads * kSoftmaxRegisters + 256 * kControlRegisters <= kThreads * 80, "what a block of this size is launched with");
+constexpr int kQueryWarps = 2;          // half of the rows each
+constexpr int kCopyWarp = 16, kScoreWarp = 20, kValueWarp = 21, kQueryWarp = 22, kResultWarp = 24;
+constexpr int kThreads = 896;           // the groups, and warps that copy, issue S^T, issue O^T, prepare queries, and join and write results (four)
+constexpr int kSoftmaxRegisters = 88, kControlRegisters = 48;
+static_assert(kGroups * kGroupThreads * kSoftmaxRegisters + 384 * kControlRegisters <= kThreads * 72, "what a block of this size is launched with");
+constexpr int kDeep = 3;                // items between their queries and their results
 constexpr int kTile = 128;              // tokens
 constexpr int kTileBytes = kTile * 128; // of keys, or of values
 constexpr int kSlots = 10;              // tiles of keys or of values in the ring, in turn
@@ -63,54 +65,56 @@ struct Item {
 
 enum { kNowhere, kOutput, kZero, kPartial };
 
-template <int kRows>
-struct __align__(1024) Shared {
-  static constexpr int kN = kRows == 16 ? 48 : 32;    // three parts of every row, in whole sixteens
-  unsigned char ring[kSlots][kTileBytes];             // [token][128 bytes], swizzled by the copy: keys of a tile, its values, the next tile's keys ..
-  unsigned char q[2][kN * 128];                       // [item parity][part of a row][128 elements]
-  unsigned char p[kGroups][kN * 128];                 // [part of a row][128 tokens]
-  float sums[2][kRows][128];                          // [item parity]: O of the second group
-  float other_ref[2][kRows], other_l[2][kRows];       // its references and sums
-  float folded[kGroups][4][kRows];
-  uint32_t fresh[kGroups][2];                         // rows of a half without a reference yet
-  unsigned moved[kGroups][2];                         // the turn of a half's last move of a reference that had been there
-  float by[kGroups][kRows], root[kGroups][kRows];     // of a move of references: added to them; the root of what O and l are multiplied by
-  float factor[2][kRows];                             // of the joined result: the groups' O times these
-  uint32_t raw_q[kRows][64];                          // the next item's queries as they are
-  float row_scale[2][kRows];                          // of the scores, by item parity
-  int keys[2][kRows], low[2][kRows];                  // what a row sees
-  int64_t to[2][kRows];                               // where its result of the item goes: elements into the output, or floats into the partials
-  int kind[2][kRows];                                 // kNowhere, kOutput, kZero, kPartial
-  Item item[2];
-  uint32_t nan_value[kGroups][kRows][4];              // elements that a row gets NaN in
-  int marked[kGroups];                                // there are some
-  float4 scales[kScaleSlots][2][kTile / 16];          // by head and 16 tokens: key scale, log2 of the value scale, its inverse
-  int4 wide[kScaleSlots];                             // a value scale of the tile beyond 2^+-kWide; from each copy warp
-  unsigned long long full[kSlots], empty[kSlots], q_full[2], q_empty[2], s_ready[kGroups], s_free[kGroups], p_ready[kGroups], o_done[kGroups];
-  uint32_t tmem_base;
-  // the work of a batch of sequences: cells (part, row tile) of whole parts in front of a sequence; then the last parts, largest first
+// The work of a batch of sequences: cells (part, row tile) of whole parts in front of a sequence; then the last parts, largest first.
+struct Work {
   int whole_before[kBatch + 1], last_before[kBatch + 1], order[kBatch];
   int in_class[kClasses];
   unsigned char size_class[kBatch];
   int first[kBatch], count[kBatch], base[kBatch];     // a sequence's rows, and the keys its first row sees (below 1: none)
 };
 
-// Bounded wait for a phase of a barrier: false after about two seconds.  Few instructions: the roles' loops together have to stay within the
-// instruction caches (with unrolled polls at every wait they did not, and every phase took three to ten times as long).
-__device__ __forceinline__ bool wait_for(const unsigned long long* barrier, uint32_t parity) {
-  const uint32_t bar = smem_u32(barrier);
-  const auto poll = [&]() {              // suspended for up to 10 us at a time, so that waiting warps leave the issue slots to the others
+template <int kRows>
+struct __align__(1024) Shared {
+  static constexpr int kN = kRows == 16 ? 48 : 32;    // three parts of every row, in whole sixteens
+  unsigned char ring[kSlots][kTileBytes];             // [token][128 bytes], swizzled by the copy: keys of a tile, its values, the next tile's keys ..
+  unsigned char q[kDeep][kN * 128];                   // [item][part of a row][128 elements]
+  unsigned char p[kGroups][2][kN * 128];              // of a group's tiles in turn: [part of a row][128 tokens]
+  uint32_t raw_q[kRows][64];                          // the next item's queries as they are
+  float4 scales[kScaleSlots][2][kTile / 16];          // by head and 16 tokens: key scale, log2 of the value scale, its inverse
+  int4 wide[kScaleSlots];                             // a value scale of the tile beyond 2^+-kWide; from each copy warp
+  // of an item
+  Item item[kDeep];
+  alignas(16) float row_scale[kDeep][kRows];          // of the scores
+  int keys[kDeep][kRows], low[kDeep][kRows];          // what a row sees of the part
+  int64_t to[kDeep][kRows];                           // where its result goes: elements into the output, or floats into the partials
+  int kind[kDeep][kRows];                             // kNowhere, kOutput, kZero, kPartial
+  float ref[kDeep][kGroups][kRows], l[kDeep][kGroups][4][kRows];        // of each group; l of each quarter of its tokens
+  alignas(16) uint32_t nan_value[kDeep][kGroups][kRows][4];      // elements that a row gets NaN in
+  int marked[kDeep][kGroups];                         // there are some
+  // of a group's tile
+  float folded[kGroups][4][kRows];
+  float by[kGroups][kRows], root[kGroups][kRows];     // of a move of references: added to them; the root of what O and l are multiplied by
+  uint32_t fresh[kGroups][2];                         // rows of a half without a reference yet
+  unsigned moved[kGroups][2];                         // the turn of a half's last move of a reference that had been there
+  float4 result[4][kRows];                            // of each result warp: the groups' factors and where a row goes
+  // A waiter may be a phase of a barrier behind, never two (a phase and the one after the next look alike): what has two buffers has two barriers.
+  unsigned long long full[kSlots], empty[kSlots], q_full[kDeep], q_empty[kDeep], done[kDeep], s_ready[kGroups], s_free[kGroups], p_ready[kGroups][2], o_done[kGroups][2];
+  uint32_t tmem_base;
+  Work work;
+};
+
+// Bounded wait for a phase of a barrier: false after two million polls (a poll is suspended for up to a microsecond, which leaves the issue slots to
+// other warps).  Few instructions: the roles' loops together have to stay within the instruction caches.  With unrolled polls at every wait they did
+// not, and every phase took three to ten times as long.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+  for (int polls = 0; polls < 2000000; ++polls) {
     uint32_t ok;
     asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}\n"
-                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(10000u) : "memory");
-    return ok != 0;
-  };
-  if (poll()) return true;
-  const long long begin = clock64();
-#pragma unroll 1
-  while (!poll())
-    if (clock64() - begin > kWaitCycles) return false;
-  return true;
+                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000u) : "memory");
+    if (ok != 0) return true;
+  }
+  return false;
 }
 
 __device__ __forceinline__ int clamp_keys(int keys, int capacity) { return max(min(keys, capacity), 0); }
@@ -125,6 +129,50 @@ __device__ __forceinline__ Spread spread_of(int each, int count, int base, int g
   x.first_part = low / kPartTokens;
   x.parts = top > 0 ? (top - 1) / kPartTokens - x.first_part + 1 : 1;
   x.tiles = (count * group + each - 1) / each;
+  return x;
+}
+
+// The last i < n with before[i] <= x, 32 candidates at a time.
+__device__ __forceinline__ int find(const int* before, int n, int x) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = n;
+#pragma unroll 1
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+    const unsigned below = __ballot_sync(0xffffffffu, at < hi && before[at] <= x);
+    lo += (31 - __clz(below)) * step;
+    hi = min(lo + step, hi);
+  }
+  return lo;
+}
+
+// Item i of a batch, by a whole warp.
+__device__ __noinline__ Item find_item(const Work* work, int batch, int sequences, int whole, int i, int units, int each, int group, int window, int capacity) {
+  const int cell = i / units;
+  int lo, local;
+  if (cell < whole) {
+    lo = find(work->whole_before, sequences, cell);
+    local = cell - work->whole_before[lo];
+  } else {
+    const int k = find(work->last_before, sequences, cell - whole);
+    lo = work->order[k];
+    local = cell - whole - work->last_before[k];
+  }
+  Item x;
+  x.s = batch + lo; x.first = work->first[lo]; x.count = work->count[lo]; x.base = work->base[lo];
+  const Spread spread = spread_of(each, x.count, x.base, group, window, capacity);
+  const int chunk = cell < whole ? local / spread.tiles : spread.parts - 1;
+  x.unit = i - cell * units;
+  x.part = spread.first_part + chunk;
+  x.pair0 = (cell < whole ? local - chunk * spread.tiles : local) * each;
+  x.pairs = min(x.count * group - x.pair0, each);
+  const int least = clamp_keys(x.base + x.pair0 / group, capacity), top = clamp_keys(x.base + (x.pair0 + x.pairs - 1) / group, capacity);
+  x.from = max(window > 0 ? max(least - window, 0) : 0, x.part * kPartTokens);
+  x.end = min(top, (x.part + 1) * kPartTokens);
+  x.all_from = max(window > 0 ? max(top - window, 0) : 0, x.from);
+  x.all_end = min(least, x.end);
+  x.begin = x.from / kTile * kTile;
+  x.tiles = x.end > x.from ? (x.end - x.begin + kTile - 1) / kTile : 0;
   return x;
 }
 
@@ -168,9 +216,6 @@ __device__ __forceinline__ bool group_any(int group, bool mine) {
                : "=r"(any) : "r"(mine ? 1u : 0u), "r"(1 + group), "n"(kGroupThreads) : "memory");
   return any != 0;
 }
-// The second group's sums of an item are there: it goes on (at most an item, the queries see to that), the first one waits.
-__device__ __forceinline__ void sums_ready(unsigned parity) { asm volatile("bar.arrive %0, %1;" ::"r"(5 + parity), "n"(kGroups * kGroupThreads) : "memory"); }
-__device__ __forceinline__ void sums_wait(unsigned parity) { asm volatile("bar.sync %0, %1;" ::"r"(5 + parity), "n"(kGroups * kGroupThreads) : "memory"); }
 __device__ __forceinline__ void block_sync() { asm volatile("bar.sync 4, %0;" ::"n"(kThreads) : "memory"); }
 
 // Two numbers as packed codes of their three parts, x = h + m / 32 + l / 1024 for |x| <= 256: x in half precision (2^-11 of it, or 2^-25), then
@@ -229,7 +274,9 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
                        int box) {
   using Sm = Shared<kRows>;
   constexpr int kHeads = 128 / kDim, kEach = kRows / kHeads, kN = Sm::kN;
-  constexpr uint32_t kScores = 0, kOutputs = kGroups * 64, kColumns = 256;      // tensor memory: 64 columns per group for each
+  // tensor memory: 64 columns for the scores of each group, then for its outputs of the items under way
+  constexpr uint32_t kScores = 0, kOutputs = kGroups * 64, kColumns = 512;
+  static_assert(kOutputs + kGroups * kDeep * 64 <= kColumns, "tensor memory");
   extern __shared__ unsigned char smem_raw[];
   Sm& sm = *reinterpret_cast<Sm*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
@@ -242,19 +289,24 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSlots; ++i) { mbar_init(smem_u32(&sm.full[i]), kCopyWarps); mbar_init(smem_u32(&sm.empty[i]), 1); }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&sm.q_full[i]), 1);
-      mbar_init(smem_u32(&sm.q_empty[i]), 1 + kGroups * kGroupWarps);             // the products' completion, and each softmax warp
+    for (int i = 0; i < kDeep; ++i) {
+      mbar_init(smem_u32(&sm.q_full[i]), kQueryWarps);
+      mbar_init(smem_u32(&sm.q_empty[i]), 4);                              // the result warps
+      mbar_init(smem_u32(&sm.done[i]), 1 + kGroups * kGroupWarps);        // the last product's completion, and each softmax warp
+    }
+    for (int i = 0; i < kGroups; ++i) {
       mbar_init(smem_u32(&sm.s_ready[i]), 1);
       mbar_init(smem_u32(&sm.s_free[i]), kGroupWarps);
-      mbar_init(smem_u32(&sm.p_ready[i]), kGroupWarps);
-      mbar_init(smem_u32(&sm.o_done[i]), 1);
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(smem_u32(&sm.p_ready[i][k]), kGroupWarps);
+        mbar_init(smem_u32(&sm.o_done[i][k]), 1);
+      }
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
 #pragma unroll 1
-  for (int i = threadIdx.x; i < kGroups * kRows * 4; i += kThreads) (&sm.nan_value[0][0][0])[i] = 0u;
-  if (threadIdx.x < kGroups) sm.marked[threadIdx.x] = 0;
+  for (int i = threadIdx.x; i < kDeep * kGroups * kRows * 4; i += kThreads) (&sm.nan_value[0][0][0][0])[i] = 0u;
+  if (threadIdx.x < kDeep * kGroups) (&sm.marked[0][0])[threadIdx.x] = 0;
   grid_dependency_wait();
   grid_dependency_release();
   tcgen05_before_sync();
@@ -283,7 +335,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     }
     if (lane == 0) out[n] = before;
   };
-  auto row_tiles = [&](int i) { return (sm.count[i] * group_heads + kEach - 1) / kEach; };
+  auto row_tiles = [&](int i) { return (sm.work.count[i] * group_heads + kEach - 1) / kEach; };
 
   // The items of sequences batch .., by all threads; their number.  Cells of whole parts come first, then every sequence's last part, those with the
   // most tiles first: dealt in this order, one CTA has about as many tiles as another.  The heads of a cell go to neighbouring CTAs at a time.
@@ -295,86 +347,49 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       int first, count;
       rows_of(a.step, batch + i, &first, &count);
       const int64_t base = static_cast<int64_t>(a.step.lengths[batch + i]) - count + 1;
-      sm.first[i] = first;
-      sm.count[i] = count;
-      sm.base[i] = static_cast<int>(base < -0x20000000 ? -0x20000000 : (base > 0x20000000 ? 0x20000000 : base));
-      const Spread x = spread_of(kEach, count, sm.base[i], group_heads, a.window, capacity);
-      sm.whole_before[i] = count > 0 ? (x.parts - 1) * x.tiles : 0;
-      const int top = clamp_keys(sm.base[i] + count - 1, capacity);
-      sm.size_class[i] = static_cast<unsigned char>(top > 0 ? (top - 1) % kPartTokens / kTile + 1 : 0);
+      sm.work.first[i] = first;
+      sm.work.count[i] = count;
+      sm.work.base[i] = static_cast<int>(base < -0x20000000 ? -0x20000000 : (base > 0x20000000 ? 0x20000000 : base));
+      const Spread x = spread_of(kEach, count, sm.work.base[i], group_heads, a.window, capacity);
+      sm.work.whole_before[i] = count > 0 ? (x.parts - 1) * x.tiles : 0;
+      const int top = clamp_keys(sm.work.base[i] + count - 1, capacity);
+      sm.work.size_class[i] = static_cast<unsigned char>(top > 0 ? (top - 1) % kPartTokens / kTile + 1 : 0);
     }
     block_sync();
     if (warp < kClasses) {
       int n = 0;
 #pragma unroll 1
-      for (int i0 = 0; i0 < sequences; i0 += 32) n += __popc(__ballot_sync(0xffffffffu, i0 + lane < sequences && sm.size_class[i0 + lane] == warp));
-      if (lane == 0) sm.in_class[warp] = n;
+      for (int i0 = 0; i0 < sequences; i0 += 32) n += __popc(__ballot_sync(0xffffffffu, i0 + lane < sequences && sm.work.size_class[i0 + lane] == warp));
+      if (lane == 0) sm.work.in_class[warp] = n;
     } else if (warp == kClasses) {
-      scan(sequences, sm.whole_before, [&](int i) { return sm.whole_before[i]; });
+      scan(sequences, sm.work.whole_before, [&](int i) { return sm.work.whole_before[i]; });
     }
     block_sync();
     if (warp < kClasses) {
       int at = 0;
 #pragma unroll 1
-      for (int k = kClasses - 1; k > warp; --k) at += sm.in_class[k];
+      for (int k = kClasses - 1; k > warp; --k) at += sm.work.in_class[k];
 #pragma unroll 1
       for (int i0 = 0; i0 < sequences; i0 += 32) {
-        const unsigned mine = __ballot_sync(0xffffffffu, i0 + lane < sequences && sm.size_class[i0 + lane] == warp);
-        if ((mine >> lane) & 1) sm.order[at + __popc(mine & ((1u << lane) - 1))] = i0 + lane;
+        const unsigned mine = __ballot_sync(0xffffffffu, i0 + lane < sequences && sm.work.size_class[i0 + lane] == warp);
+        if ((mine >> lane) & 1) sm.work.order[at + __popc(mine & ((1u << lane) - 1))] = i0 + lane;
         at += __popc(mine);
       }
     }
     block_sync();
-    if (warp == 0) scan(sequences, sm.last_before, [&](int k) { return row_tiles(sm.order[k]); });
+    if (warp == 0) scan(sequences, sm.work.last_before, [&](int k) { return row_tiles(sm.work.order[k]); });
     block_sync();
-    whole = sm.whole_before[sequences];
-    return (whole + sm.last_before[sequences]) * units;
-  };
-
-  // The last i < n with before[i] <= x, 32 candidates at a time.
-  auto find = [&](const int* before, int n, int x) {
-    int lo = 0, hi = n;
-#pragma unroll 1
-    while (hi - lo > 1) {
-      const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-      const unsigned below = __ballot_sync(0xffffffffu, at < hi && before[at] <= x);
-      lo += (31 - __clz(below)) * step;
-      hi = min(lo + step, hi);
-    }
-    return lo;
+    whole = sm.work.whole_before[sequences];
+    return (whole + sm.work.last_before[sequences]) * units;
   };
 
   auto item_at = [&](int batch, int i) {
-    const int cell = i / units, unit = i - cell * units;
-    int lo, local;
-    if (cell < whole) {
-      lo = find(sm.whole_before, sequences, cell);
-      local = cell - sm.whole_before[lo];
-    } else {
-      const int k = find(sm.last_before, sequences, cell - whole);
-      lo = sm.order[k];
-      local = cell - whole - sm.last_before[k];
-    }
-    Item x;
-    x.s = batch + lo; x.first = sm.first[lo]; x.count = sm.count[lo]; x.base = sm.base[lo];
-    const Spread spread = spread_of(kEach, x.count, x.base, group_heads, a.window, capacity);
-    const int chunk = cell < whole ? local / spread.tiles : spread.parts - 1;
-    x.unit = unit;
-    x.part = spread.first_part + chunk;
-    x.pair0 = (cell < whole ? local - chunk * spread.tiles : local) * kEach;
-    x.pairs = min(x.count * group_heads - x.pair0, kEach);
-    const int top = clamp_keys(x.base + (x.pair0 + x.pairs - 1) / group_heads, capacity);
-    const int low = a.window > 0 ? max(clamp_keys(x.base + x.pair0 / group_heads, capacity) - a.window, 0) : 0;
-    x.from = max(low, x.part * kPartTokens);
-    x.end = min(top, (x.part + 1) * kPartTokens);
-    x.all_from = max(a.window > 0 ? max(top - a.window, 0) : 0, x.from);
-    x.all_end = min(clamp_keys(x.base + x.pair0 / group_heads, capacity), x.end);
-    x.begin = x.from / kTile * kTile;
-    x.tiles = x.end > x.from ? (x.end - x.begin + kTile - 1) / kTile : 0;
-    return x;
+    return find_item(&sm.work, batch, sequences, whole, i, units, kEach, group_heads, a.window, capacity);
   };
   auto group_of = [&](const Item& x, int j) { return (x.begin / kTile + j) & 1; };
   auto tiles_of = [&](const Item& x, int group) { return (x.tiles + (group_of(x, 0) == group ? 1 : 0)) / 2; };
+  auto buffer = [&]() { return done_items % kDeep; };
+  auto phase = [&]() { return (done_items / kDeep) & 1; };
   auto pass = [&](const Item& x) {
     ++done_items;
     done_tiles += x.tiles;
@@ -422,7 +437,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
 #pragma unroll 1
           for (int values = 0; values < 2; ++values) {
             const unsigned h = 2 * n + values, slot = h % kSlots;
-            if (h >= kSlots && !wait_for(&sm.empty[slot], (h / kSlots - 1) & 1)) { failed = true; break; }
+            if (h >= kSlots && !wait_for(smem_u32(&sm.empty[slot]), (h / kSlots - 1) & 1)) { failed = true; break; }
             if (values == 0) {
               // The slots of the tile kScaleSlots before are free: its values gave theirs back before this tile's keys could be copied.
               bool wide = false;
@@ -473,18 +488,18 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       constexpr uint32_t kIdesc = (1u << 4) | (static_cast<uint32_t>(kN >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
 #pragma unroll 1
       for (int i = blockIdx.x; i < total && !failed; i += gridDim.x) {
-        const unsigned parity = done_items & 1;
-        bool ok = wait_for(&sm.q_full[parity], (done_items >> 1) & 1);
-        const Item x = sm.item[parity];
+        const unsigned at = buffer();
+        bool ok = wait_for(smem_u32(&sm.q_full[at]), phase());
+        const Item x = sm.item[at];
         {
-          const uint64_t q_desc = umma_desc(smem_u32(sm.q[parity]), 16, 1024);
+          const uint64_t q_desc = umma_desc(smem_u32(sm.q[at]), 16, 1024);
           unsigned of[kGroups] = {done_of[0], done_of[1]};
 #pragma unroll 1
           for (int j = 0; j < x.tiles; ++j) {
             const int group = group_of(x, j);
             const unsigned h = 2 * (done_tiles + j), slot = h % kSlots, mine = group ? of[1] : of[0];
-            ok = ok && (mine == 0 || wait_for(&sm.s_free[group], (mine - 1) & 1));
-            ok = ok && wait_for(&sm.full[slot], (h / kSlots) & 1);
+            ok = ok && (mine == 0 || wait_for(smem_u32(&sm.s_free[group]), (mine - 1) & 1));
+            ok = ok && wait_for(smem_u32(&sm.full[slot]), (h / kSlots) & 1);
             if (!__all_sync(0xffffffffu, ok)) { failed = true; break; }
             tcgen05_after_sync();
             const uint64_t k_desc = umma_desc(smem_u32(sm.ring[slot]), 16, 1024);
@@ -500,8 +515,6 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           }
         }
         if (!__all_sync(0xffffffffu, ok)) failed = true;
-        if (elect_one()) umma_commit(smem_u32(&sm.q_empty[parity]));
-        __syncwarp();
         pass(x);
       }
     } else if (warp == kValueWarp) {
@@ -509,35 +522,38 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       constexpr uint32_t kIdesc = (1u << 4) | (1u << 15) | (static_cast<uint32_t>(kN >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
 #pragma unroll 1
       for (int i = blockIdx.x; i < total && !failed; i += gridDim.x) {
-        const unsigned parity = done_items & 1;
-        if (!__all_sync(0xffffffffu, wait_for(&sm.q_full[parity], (done_items >> 1) & 1))) { failed = true; break; }
-        const Item x = sm.item[parity];        // (held until the groups are done with the item, which needs these products)
+        const unsigned at = buffer();
+        if (!__all_sync(0xffffffffu, wait_for(smem_u32(&sm.q_full[at]), phase()))) { failed = true; break; }
+        const Item x = sm.item[at];
 #pragma unroll 1
         for (int j = 0; j < x.tiles; ++j) {
           const int group = group_of(x, j);
           const unsigned h = 2 * (done_tiles + j) + 1, slot = h % kSlots, mine = (group ? done_of[1] : done_of[0]) + j / 2;
-          if (!__all_sync(0xffffffffu, wait_for(&sm.full[slot], (h / kSlots) & 1) && wait_for(&sm.p_ready[group], mine & 1))) { failed = true; break; }
+          if (!__all_sync(0xffffffffu, wait_for(smem_u32(&sm.full[slot]), (h / kSlots) & 1) && wait_for(smem_u32(&sm.p_ready[group][mine & 1]), (mine >> 1) & 1))) { failed = true; break; }
           tcgen05_after_sync();
-          const uint64_t v_desc = umma_desc(smem_u32(sm.ring[slot]), kTileBytes, 1024), p_desc = umma_desc(smem_u32(sm.p[group]), 16, 1024);
+          const uint64_t v_desc = umma_desc(smem_u32(sm.ring[slot]), kTileBytes, 1024), p_desc = umma_desc(smem_u32(sm.p[group][mine & 1]), 16, 1024);
           if (elect_one()) {
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
-              code_product(tmem + kOutputs + group * 64, v_desc + static_cast<uint64_t>(ks * 4096 >> 4), p_desc + static_cast<uint64_t>(ks * 2), kIdesc,
+              code_product(tmem + kOutputs + (at * kGroups + group) * 64, v_desc + static_cast<uint64_t>(ks * 4096 >> 4), p_desc + static_cast<uint64_t>(ks * 2), kIdesc,
                            (j >= 2 || ks > 0) ? 1u : 0u);
-            umma_commit(smem_u32(&sm.o_done[group]));
+            umma_commit(smem_u32(&sm.o_done[group][mine & 1]));
             umma_commit(smem_u32(&sm.empty[slot]));
           }
           __syncwarp();
         }
+        if (elect_one()) umma_commit(smem_u32(&sm.done[at]));
+        __syncwarp();
         pass(x);
       }
-    } else if (warp == kQueryWarp) {
-      // ---- the queries of an item in three parts, and what its rows see ----
+    } else if (warp >= kQueryWarp && warp < kQueryWarp + kQueryWarps) {
+      // ---- the queries of an item in three parts, half of the rows each; what its rows see ----
+      const int first_row = (warp - kQueryWarp) * (kRows / kQueryWarps);
 #pragma unroll 1
       for (int i = blockIdx.x; i < total && !failed; i += gridDim.x) {
         const Item x = item_at(batch, i);
-        const unsigned parity = done_items & 1;
-        if (done_items >= 2 && !__all_sync(0xffffffffu, wait_for(&sm.q_empty[parity], ((done_items >> 1) - 1) & 1))) { failed = true; break; }
+        const unsigned buf = buffer();
+        if (done_items >= kDeep && !__all_sync(0xffffffffu, wait_for(smem_u32(&sm.q_empty[buf]), phase() ^ 1))) { failed = true; break; }
         constexpr int kMine = kDim / 32;            // elements of a lane
         // lane r has row r's place in the item
         const int my_head = x.unit * kHeads + lane % kRows / kEach, my_pair = x.pair0 + lane % kEach, my_row = my_pair / group_heads;
@@ -546,7 +562,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         const int64_t my_source = my_live ? at_row * a.q_stride + head * kDim : -1;
         // all rows on their way at once, a lane's kMine elements of each
 #pragma unroll 1
-        for (int r = 0; r < kRows; ++r) {
+        for (int r = first_row; r < first_row + kRows / kQueryWarps; ++r) {
           const int64_t source = __shfl_sync(0xffffffffu, my_source, r);
           const T* src = static_cast<const T*>(a.q) + (source < 0 ? 0 : source) + lane * kMine;
           asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(smem_u32(&sm.raw_q[r][lane * (kMine / 2)])), "l"(src), "n"(kMine * 2), "r"(source < 0 ? 0 : kMine * 2) : "memory");
@@ -554,7 +570,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
         __syncwarp();
 #pragma unroll 1
-        for (int r = 0; r < kRows; ++r) {
+        for (int r = first_row; r < first_row + kRows / kQueryWarps; ++r) {
           {
             uint32_t raw[kMine / 2];
 #pragma unroll
@@ -572,12 +588,12 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             odd = __any_sync(0xffffffffu, odd);
             const int e = largest > 0.0f && !odd ? max((__float_as_int(largest) >> 23) - 127 - 7, -126) : 0;
             const float up = odd ? 0.0f : power_of_two(-e);
-            if (lane == 0) sm.row_scale[parity][r] = odd ? NAN : scale_log2 * power_of_two(e);
+            if (lane == 0) sm.row_scale[buf][r] = odd ? NAN : scale_log2 * power_of_two(e);
             uint32_t codes[kMine / 2][3];
 #pragma unroll
             for (int w = 0; w < kMine / 2; ++w) three_parts(odd ? 0.0f : v[2 * w] * up, odd ? 0.0f : v[2 * w + 1] * up, codes[w]);
             // element lane * kMine of a 128-byte line whose 16-byte pieces are swizzled by the row; of two heads, the other's half of the line is zero
-            const uint32_t line = smem_u32(sm.q[parity]) + r * 128;
+            const uint32_t line = smem_u32(sm.q[buf]) + r * 128;
             const int byte = (kHeads == 2 ? (r / kEach) * 64 : 0) + lane * kMine;
             const uint32_t at = line + (byte ^ ((r & 7) << 4));
 #pragma unroll
@@ -591,20 +607,86 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             }
           }
         }
-        if (lane < kRows) {
+        if (first_row == 0 && lane < kRows) {
           const int sees = clamp_keys(x.base + my_row, capacity), low = a.window > 0 ? max(sees - a.window, 0) : 0;
           const int first_part = low / kPartTokens, last_part = sees > 0 ? (sees - 1) / kPartTokens : first_part;
-          sm.keys[parity][lane] = my_live ? min(sees, x.end) : x.end;          // of the part; rows that are none see all of it, and nothing is masked for them
-          sm.low[parity][lane] = my_live ? max(low, x.from) : x.from;
+          sm.keys[buf][lane] = my_live ? min(sees, x.end) : x.end;          // of the part; rows that are none see all of it, and nothing is masked for them
+          sm.low[buf][lane] = my_live ? max(low, x.from) : x.from;
           int kind = kNowhere;
           if (my_live && x.part >= first_part && x.part <= last_part) kind = first_part < last_part ? kPartial : (sees > low ? kOutput : kZero);
-          sm.kind[parity][lane] = kind;
-          sm.to[parity][lane] = kind == kPartial ? ((at_row * a.q_heads + head) * a.parts + x.part - first_part) * partial_stride(kDim) : at_row * a.out_stride + head * kDim;
+          sm.kind[buf][lane] = kind;
+          sm.to[buf][lane] = kind == kPartial ? ((at_row * a.q_heads + head) * a.parts + x.part - first_part) * partial_stride(kDim) : at_row * a.out_stride + head * kDim;
         }
-        if (lane == 0) sm.item[parity] = x;
+        if (first_row == 0 && lane == 0) sm.item[buf] = x;
         fence_async_proxy();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sm.q_full[parity]));
+        if (lane == 0) mbar_arrive(smem_u32(&sm.q_full[buf]));
+        pass(x);
+      }
+    } else if (warp >= kResultWarp) {
+      // ---- results: an element of the values per thread; both groups' parts added up ----
+      const int own = threadIdx.x & (kTile - 1), row = lane % kRows;
+      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+#pragma unroll 1
+      for (int i = blockIdx.x; i < total; i += gridDim.x) {
+        const unsigned buf = buffer();
+        if (!failed && !wait_for(smem_u32(&sm.done[buf]), phase())) failed = true;
+        failed = __any_sync(0xffffffffu, failed);
+        tcgen05_after_sync();
+        const Item x = sm.item[buf];
+        const bool has0 = tiles_of(x, 0) > 0, has1 = tiles_of(x, 1) > 0;
+        // a lane has a row's factors: 2^(R - max R) of each group, over the joined sum where this is the row's only part
+        const int kind = sm.kind[buf][row];
+        const int64_t to = sm.to[buf][row];
+        {
+          const float ref0 = has0 ? sm.ref[buf][0][row] : -INFINITY, ref1 = has1 ? sm.ref[buf][1][row] : -INFINITY;
+          const float big = fmaxf(ref0, ref1), zero = big == -INFINITY ? 0.0f : big;
+          const float root0 = fast_exp2(0.5f * (ref0 - zero)), root1 = fast_exp2(0.5f * (ref1 - zero));
+          float sum = 0.0f;
+          if (has0) sum = ((sm.l[buf][0][0][row] + sm.l[buf][0][1][row]) + (sm.l[buf][0][2][row] + sm.l[buf][0][3][row])) * root0 * root0;
+          if (has1) sum += ((sm.l[buf][1][0][row] + sm.l[buf][1][1][row]) + (sm.l[buf][1][2][row] + sm.l[buf][1][3][row])) * root1 * root1;
+          const float scale = failed ? NAN : (kind == kPartial ? 1.0f : (kind == kOutput ? __frcp_rn(sum) : 0.0f));
+          if (lane < kRows) sm.result[warp & 3][row] = make_float4(root0 * root0 * scale, root1 * root1 * scale, __int_as_float(static_cast<int>(to)), __int_as_float(static_cast<int>(to >> 32)));
+          if (kind == kPartial && lane < kRows && (warp & 3) == 0) *reinterpret_cast<float2*>(a.partials + to + kDim) = make_float2(big, sum);
+        }
+        const uint32_t partial = __ballot_sync(0xffffffffu, kind == kPartial), nowhere = __ballot_sync(0xffffffffu, kind == kNowhere);
+        const bool marked = (sm.marked[buf][0] | sm.marked[buf][1]) != 0;
+        __syncwarp();
+        const uint32_t outputs0 = tmem + lanes + kOutputs + (buf * kGroups) * 64, outputs1 = outputs0 + 64;
+#pragma unroll 1
+        for (int r0 = 0; r0 < kRows; r0 += 4) {
+          const int d = kHeads == 2 ? own - 64 * (r0 / kEach) : own;      // of two heads, a thread's element may be the other one's
+          float acc0[4], m0[4], rest0[4], acc1[4], m1[4], rest1[4];
+          load_columns<4>(outputs0 + r0, acc0);
+          load_columns<4>(outputs0 + kRows + r0, m0);
+          load_columns<4>(outputs0 + 2 * kRows + r0, rest0);
+          load_columns<4>(outputs1 + r0, acc1);
+          load_columns<4>(outputs1 + kRows + r0, m1);
+          load_columns<4>(outputs1 + 2 * kRows + r0, rest1);
+          tmem_load_wait();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int r = r0 + k;
+            const float4 of = sm.result[warp & 3][r];
+            float o0 = fmaf(fmaf(rest0[k], 0.03125f, m0[k]), 0.03125f, acc0[k]), o1 = fmaf(fmaf(rest1[k], 0.03125f, m1[k]), 0.03125f, acc1[k]);
+            float value = has0 ? o0 * of.x : 0.0f;                         // (a group without tiles has left nothing there)
+            if (has1) value = fmaf(o1, of.y, value);
+            if (marked && ((sm.nan_value[buf][0][r][own >> 5] | sm.nan_value[buf][1][r][own >> 5]) >> (own & 31)) & 1) value = NAN;
+            if (((nowhere >> r) & 1) || d < 0 || d >= kDim) continue;
+            const int64_t at = static_cast<int64_t>(static_cast<uint32_t>(__float_as_int(of.z)) | static_cast<uint64_t>(static_cast<uint32_t>(__float_as_int(of.w))) << 32) + d;
+            if ((partial >> r) & 1) a.partials[at] = value;
+            else static_cast<T*>(a.out)[at] = Elem<T>::from_float(value);
+          }
+        }
+        tcgen05_before_sync();
+        if (marked) {
+          asm volatile("bar.sync 3, 128;" ::: "memory");                   // the four warps have read them
+          if (own < kGroups * kRows)
+            *reinterpret_cast<uint4*>(&sm.nan_value[buf][own / kRows][own % kRows][0]) = make_uint4(0u, 0u, 0u, 0u);
+          if (own < kGroups) sm.marked[buf][own] = 0;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.q_empty[buf]));
         pass(x);
       }
     }
@@ -618,17 +700,18 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       constexpr int kMine = kRows / 2;
       const int group = warp >> 3, half = (warp >> 2) & 1, own = threadIdx.x & (kTile - 1), row0 = half * kMine;
       const int head_slot = kHeads == 2 ? half : 0;
-      const uint32_t lanes = (static_cast<uint32_t>((warp & 3) * 32) << 16) + group * 64 + row0;
-      const uint32_t scores_at = tmem + lanes + kScores, outputs_at = tmem + lanes + kOutputs;
+      const uint32_t lanes = (static_cast<uint32_t>((warp & 3) * 32) << 16) + group * 64 + row0;      // and columns
+      const uint32_t scores_at = tmem + lanes + kScores;
       // where this thread's weights go: rows of 128 tokens, 16-byte pieces swizzled by the row (a half's first row is a multiple of its rows)
-      const uint32_t weights = smem_u32(sm.p[group]) + row0 * 128 + (own & 15), piece = static_cast<uint32_t>((own >> 4) ^ (row0 & 7)) << 4;
+      const uint32_t first_weights = smem_u32(sm.p[group][0]) + row0 * 128 + (own & 15), piece = static_cast<uint32_t>((own >> 4) ^ (row0 & 7)) << 4;
       const int folded_row = row0 + row_after_fold<kMine>(lane);
       const bool folds = lane % (32 / kMine) == 0;
 #pragma unroll 1
       for (int i = blockIdx.x; i < total; i += gridDim.x) {
-        const unsigned parity = done_items & 1;
-        failed = group_any(group, failed || ((warp & 7) == 0 && !wait_for(&sm.q_full[parity], (done_items >> 1) & 1)));
-        const Item x = sm.item[parity];
+        const unsigned buf = buffer();
+        failed = group_any(group, failed || ((warp & 7) == 0 && !wait_for(smem_u32(&sm.q_full[buf]), phase())));
+        const Item x = sm.item[buf];
+        const uint32_t outputs_at = tmem + lanes + kOutputs + buf * kGroups * 64;
         const int mine = tiles_of(x, group);
         const unsigned before = group ? done_of[1] : done_of[0];
         float ref[kMine], l[kMine];
@@ -644,11 +727,12 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           const int token0 = x.begin + j * kTile, token = token0 + own;
           // The tile's scales are there with its keys and its values.  Only the values can be waited for: they keep their place until this group's
           // weights have met them, while that of the keys may have been filled again (and its barrier be a whole turn on).
-          // One warp waits, for the product before as well (it has read the weights that this tile's replace, and its result is at rest then); the
-          // others wait for it at the group's barrier, which costs no issue slots.
+          // One warp waits, for the product of the tile before the last as well (it has read the weights that this tile's replace); the others wait for
+          // it at the group's barrier, which costs no issue slots.
           bool ok = true;
           if ((warp & 7) == 0 && !failed)
-            ok = wait_for(&sm.s_ready[group], turn & 1) && wait_for(&sm.full[h % kSlots], (h / kSlots) & 1) && (turn == 0 || wait_for(&sm.o_done[group], (turn - 1) & 1));
+            ok = wait_for(smem_u32(&sm.s_ready[group]), turn & 1) && wait_for(smem_u32(&sm.full[h % kSlots]), (h / kSlots) & 1) &&
+                 (turn < 2 || wait_for(smem_u32(&sm.o_done[group][turn & 1]), ((turn >> 1) - 1) & 1));
           if (group_any(group, !ok)) failed = true;
           tcgen05_after_sync();
           float s[kMine], m[kMine], rest[kMine];
@@ -664,7 +748,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           if (lane == 0) mbar_arrive(smem_u32(&sm.s_free[group]));
 #pragma unroll
           for (int r = 0; r < kMine; r += 4) {
-            const float4 row_scale = load_shared16f(smem_u32(&sm.row_scale[parity][row0 + r]));
+            const float4 row_scale = load_shared16f(smem_u32(&sm.row_scale[buf][row0 + r]));
             const float2 part = make_float2(0.03125f, 0.03125f), keys_scale = make_float2(scale.x, scale.x), exponent = make_float2(scale.y, scale.y);
 #pragma unroll
             for (int i2 = 0; i2 < 4; i2 += 2) {
@@ -680,7 +764,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           if (ragged) {
 #pragma unroll
             for (int r = 0; r < kMine; ++r)
-              if (token >= sm.keys[parity][row0 + r] || token < sm.low[parity][row0 + r]) s[r] = -INFINITY;
+              if (token >= sm.keys[buf][row0 + r] || token < sm.low[buf][row0 + r]) s[r] = -INFINITY;
           }
           float top = fmaxf(s[0], s[1]);
 #pragma unroll
@@ -715,8 +799,11 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
               l[r] = l[r] * root * root;           // in two steps: where a page of far larger values moved the reference, the whole factor may be 0 in fp32 and l not
             }
             const bool moves = sm.moved[group][half] == turn;
-            if (moves && k > 0) {                  // the same for the warps of a half
-#pragma unroll
+            if (moves && k > 0) {                  // the same for the warps of a half; the output is at rest once the product before is complete
+              if (!failed && !wait_for(smem_u32(&sm.o_done[group][(turn - 1) & 1]), ((turn - 1) >> 1) & 1)) failed = true;
+              __syncwarp();
+              tcgen05_after_sync();
+#pragma unroll 1
               for (int part = 0; part < 3; ++part) {
                 float o[kMine];
                 load_columns<kMine>(outputs_at + part * kRows, o);
@@ -729,6 +816,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
               tcgen05_before_sync();
             }
           }
+          const uint32_t weights = first_weights + (turn & 1) * (kN * 128);
           uint32_t codes[kMine / 2][3];
 #pragma unroll
           for (int r = 0; r < kMine; r += 2) {
@@ -770,7 +858,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
               if (!seen) {
                 *at = make_uint4(0u, 0u, 0u, 0u);
               } else if (nan_codes(w.x) | nan_codes(w.y) | nan_codes(w.z) | nan_codes(w.w)) {
-                sm.marked[group] = 1;
+                sm.marked[buf][group] = 1;
                 uint32_t* words = reinterpret_cast<uint32_t*>(at);
 #pragma unroll 1
                 for (int k4 = 0; k4 < 4; ++k4) {
@@ -778,8 +866,8 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
                   const uint32_t bits = (marks & 1) | ((marks >> 7) & 2) | ((marks >> 14) & 4) | ((marks >> 21) & 8);
 #pragma unroll 1
                   for (int r = 0; r < kRows; ++r)
-                    if ((kHeads == 1 || r / kEach == b / 4) && token < sm.keys[parity][r] && token >= sm.low[parity][r])
-                      atomicOr(&sm.nan_value[group][r][b >> 1], bits << (16 * (b & 1) + 4 * k4));
+                    if ((kHeads == 1 || r / kEach == b / 4) && token < sm.keys[buf][r] && token >= sm.low[buf][r])
+                      atomicOr(&sm.nan_value[buf][group][r][b >> 1], bits << (16 * (b & 1) + 4 * k4));
                   words[k4] &= ~(marks * 0xffu);
                 }
               }
@@ -788,98 +876,31 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           fence_async_proxy();
           tcgen05_before_sync();
           __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&sm.p_ready[group]));
+          if (lane == 0) mbar_arrive(smem_u32(&sm.p_ready[group][turn & 1]));
         }
 
-        // the group's sums: the second one leaves them in shared memory, the first joins them with its own
-        float o[kMine];
-#pragma unroll
-        for (int r = 0; r < kMine; ++r) o[r] = 0.0f;
+        // what the result warps need
         if (mine > 0) {
           const float total = fold_rows<kMine, false>(l, lane);
-          if (folds) sm.folded[group][warp & 3][folded_row] = total;
-          bool ok = true;
-          if ((warp & 7) == 0 && !failed) ok = wait_for(&sm.o_done[group], (before + mine - 1) & 1);
-          if (group_any(group, !ok)) failed = true;
-          tcgen05_after_sync();
-          float m[kMine], rest[kMine];
-          load_columns<kMine>(outputs_at, o);
-          load_columns<kMine>(outputs_at + kRows, m);
-          load_columns<kMine>(outputs_at + 2 * kRows, rest);
-          tmem_load_wait();
-          tcgen05_before_sync();
-#pragma unroll
-          for (int r = 0; r < kMine; ++r) o[r] = fmaf(fmaf(rest[r], 0.03125f, m[r]), 0.03125f, o[r]);
-          if (sm.marked[group]) {                  // set behind barriers, the same for all
+          if (folds) sm.l[buf][group][warp & 3][folded_row] = failed ? NAN : total;
+          if (own < kMine) {
+            float own_ref = -INFINITY;
 #pragma unroll
             for (int r = 0; r < kMine; ++r)
-              if ((sm.nan_value[group][row0 + r][own >> 5] >> (own & 31)) & 1) o[r] = NAN;
-            group_any(group, false);               // nan_value has been read
-            if (own < kMine) {
-#pragma unroll
-              for (int b = 0; b < 4; ++b) sm.nan_value[group][row0 + own][b] = 0u;
-            }
-            if (own == 0) sm.marked[group] = 0;
-          }
-        }
-        // a row's reference and sum, by a thread each
-        float own_ref = -INFINITY, own_l = 0.0f;
-        if (mine > 0 && own < kMine) {
-          own_l = (sm.folded[group][0][row0 + own] + sm.folded[group][1][row0 + own]) + (sm.folded[group][2][row0 + own] + sm.folded[group][3][row0 + own]);
-#pragma unroll
-          for (int r = 0; r < kMine; ++r)
-            if (own == r && !((fresh >> r) & 1)) own_ref = ref[r];
-          if (failed) own_l = NAN;
-        }
-        if (group == 1) {
-          if (mine > 0) {
-#pragma unroll
-            for (int r = 0; r < kMine; ++r) sm.sums[parity][row0 + r][own] = o[r];
-            if (own < kMine) {
-              sm.other_ref[parity][row0 + own] = own_ref;
-              sm.other_l[parity][row0 + own] = own_l;
-            }
-          }
-          sums_ready(parity);
-        } else {
-          sums_wait(parity);
-          // a row's factors by one thread: 2^(R - max R) of each group, over the joined sum where this is the row's only part
-          const bool others = tiles_of(x, 1) > 0;
-          if (own < kMine) {
-            const int row = row0 + own, kind = sm.kind[parity][row];
-            const float other_ref = others ? sm.other_ref[parity][row] : -INFINITY, other_l = others ? sm.other_l[parity][row] : 0.0f;
-            const float big = fmaxf(own_ref, other_ref), zero = big == -INFINITY ? 0.0f : big;
-            const float root0 = fast_exp2(0.5f * (own_ref - zero)), root1 = fast_exp2(0.5f * (other_ref - zero));
-            const float sum = own_l * root0 * root0 + other_l * root1 * root1;
-            const float scale = kind == kPartial ? 1.0f : (kind == kOutput ? __frcp_rn(sum) : 0.0f);
-            sm.factor[0][row] = root0 * root0 * scale;
-            sm.factor[1][row] = root1 * root1 * scale;
-            if (kind == kPartial) *reinterpret_cast<float2*>(a.partials + sm.to[parity][row] + kDim) = make_float2(big, sum);
-          }
-          group_any(group, false);
-          const int d = kHeads == 2 ? own - 64 * half : own;      // of two heads, a thread's element may be the other one's
-          if (d >= 0 && d < kDim) {
-#pragma unroll
-            for (int r = 0; r < kMine; ++r) {
-              const int kind = sm.kind[parity][row0 + r];
-              float acc = o[r] * sm.factor[0][row0 + r];
-              if (others) acc = fmaf(sm.sums[parity][row0 + r][own], sm.factor[1][row0 + r], acc);
-              const int64_t to = sm.to[parity][row0 + r] + d;
-              if (kind == kPartial) a.partials[to] = acc;
-              else if (kind != kNowhere) static_cast<T*>(a.out)[to] = Elem<T>::from_float(acc);
-            }
+              if (own == r && !((fresh >> r) & 1)) own_ref = ref[r];
+            sm.ref[buf][group][row0 + own] = own_ref;
           }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sm.q_empty[parity]));
+        if (lane == 0) mbar_arrive(smem_u32(&sm.done[buf]));
         pass(x);
       }
     }
   }
-  // a wait that gave up left NaN; copies still in flight land before the shared memory is given back
+  // a wait that gave up left NaN (a result warp's own, at the latest); copies still in flight land before the shared memory is given back
   if (failed && warp >= kCopyWarp && warp < kCopyWarp + kCopyWarps)
     for (int i = 0; i < kSlots; ++i)
-      if (!wait_for(&sm.full[i], 0) && !wait_for(&sm.full[i], 1)) break;
+      if (!wait_for(smem_u32(&sm.full[i]), 0) && !wait_for(smem_u32(&sm.full[i]), 1)) break;
   tcgen05_before_sync();
   __syncthreads();
   if (warp == kScoreWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns) : "memory");
@@ -908,7 +929,8 @@ int launch(const QuantizedAttentionArgs& a, cudaStream_t stream) {
   while (box < kTile && c.block % (2 * box) == 0) box *= 2;
   CUtensorMap key_map, value_map;
   if (make_code_map(&key_map, c.key, c, box) != RLT_OK || make_code_map(&value_map, c.value, c, box) != RLT_OK) return RLT_ERR_UNSUPPORTED;
-  const size_t smem = sizeof(Shared<kRows>) + 1024;
+  constexpr size_t smem = sizeof(Shared<kRows>) + 1024;
+  static_assert(smem <= 227 * 1024, "shared memory of a block");
   auto kernel = quantized_tiles_kernel<T, kDim, kRows>;
   RLT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
   return launch_dependent("quantized_tiles_kernel", kernel, dim3(static_cast<unsigned>(info.sm_count)), dim3(kThreads), smem, stream, key_map, value_map, a,
