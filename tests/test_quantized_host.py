@@ -124,7 +124,7 @@ def test_the_c_entries_refuse_without_a_launch():
                 dict(dtype=7), dict(rows=-1)):
         assert attend(**bad) == _capi.ERR_INVALID, bad
     need = lib.rlt_quantized_attention_workspace_bytes(1, 4, 64, 16, 1000, 0)
-    assert need == 4 * 16 * 4 * (64 + 4)                              # 16 parts of 1024 tokens
+    assert need == 4 * 10 * 4 * (64 + 4)                              # four parts of 1024 tokens and six of 2048
     assert lib.rlt_quantized_attention_workspace_bytes(1, 4, 64, 16, 64, 0) == 0
     assert lib.rlt_quantized_attention_workspace_bytes(1, 4, 64, 16, 1000, 1) == 0
     assert lib.rlt_quantized_attention_workspace_bytes(1, 4, 64, 16, 1000, 2) == 4 * 2 * 4 * (64 + 4)

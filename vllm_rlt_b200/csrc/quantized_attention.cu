@@ -3,7 +3,7 @@
 //
 //   s_t = scale * q . (key_scale[page] * key_code[t]),   p = softmax over the keys a row sees,   out = sum_t p_t * value_scale[page] * value_code[t]
 //
-// Contexts are split at fixed positions (kPartTokens).  A part leaves O = sum 2^(s_t - M) v_t, M and l = sum 2^(s_t - M) in fp32 (s in log2
+// Contexts are split at fixed positions.  A part leaves O = sum 2^(s_t - M) v_t, M and l = sum 2^(s_t - M) in fp32 (s in log2
 // units); rows whose keys lie in one part are finished by the kernel that scored them, the others by the merge.
 #include "attention.cuh"
 #include "quantized_kv.cuh"
@@ -34,9 +34,9 @@ quantized_rows_kernel(QuantizedAttentionArgs a) {
   rows_of(a.step, s, &first, &count);
   if (row < first || row >= first + count) return;                    // in no sequence: left as it was
   keys_of(a.step, c.block, a.window, s, first, count, row, &low, &keys);
-  const int first_part = low / kPartTokens, last_part = keys > 0 ? (keys - 1) / kPartTokens : first_part;
+  const int first_part = part_of(low), last_part = keys > 0 ? part_of(keys - 1) : first_part;
   if (first_part + part > last_part) return;
-  const int begin = max(low, (first_part + part) * kPartTokens), end = min(keys, (first_part + part + 1) * kPartTokens);
+  const int begin = max(low, part_begin(first_part + part)), end = min(keys, part_begin(first_part + part + 1));
 
   const T* q = static_cast<const T*>(a.q) + row * a.q_stride + static_cast<int64_t>(head) * c.dim;
   for (int d = threadIdx.x; d < kDims * 32; d += kWarps * 32) s_q[d] = d < c.dim ? Elem<T>::to_float(q[d]) * (a.scale * kToLog2) : 0.0f;
@@ -125,7 +125,7 @@ quantized_merge_kernel(QuantizedAttentionArgs a) {
   rows_of(a.step, s, &first, &count);
   if (row < first || row >= first + count) return;
   keys_of(a.step, c.block, a.window, s, first, count, row, &low, &keys);
-  const int parts = keys > 0 ? (keys - 1) / kPartTokens - low / kPartTokens + 1 : 1;
+  const int parts = keys > 0 ? part_of(keys - 1) - part_of(low) + 1 : 1;
   if (parts < 2) return;
   const int stride = partial_stride(c.dim), quads = (stride - 4) / 4;
   const float* part = a.partials + pair * a.parts * stride;

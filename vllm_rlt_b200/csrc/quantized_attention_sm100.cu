@@ -3,7 +3,7 @@
 // them to half precision took 77 % of the conversion pipe's time at 28 % of the memory's rate).
 //
 // Work.  An item is up to kRows query rows — (row, query head of the group) pairs of one sequence — of 128 bytes of heads (one 128-wide key/value
-// head or two 64-wide ones) over one part of the context (kPartTokens at fixed positions).  Items are dealt to one CTA per SM in an order that every
+// head or two 64-wide ones) over one part of the context (at fixed positions).  Items are dealt to one CTA per SM in an order that every
 // CTA derives from the lengths: no work list, no atomics, no launch before the first byte is read.
 //
 // Products.  Keys and values are the M operands, so a handful of rows is the N and nothing is padded to a tensor tile:
@@ -32,21 +32,27 @@ namespace rlt {
 namespace {
 
 constexpr int kGroups = 2;
-constexpr int kGroupThreads = 256;      // two threads per token, each with half of the rows
-constexpr int kGroupWarps = kGroupThreads / 32;
 constexpr int kCopyWarps = 4;           // each copies the same quarter of every tile
 constexpr int kQueryWarps = 2;          // half of the rows each
-constexpr int kCopyWarp = 16, kScoreWarp = 20, kValueWarp = 21, kQueryWarp = 22, kResultWarp = 24;
-constexpr int kThreads = 896;           // the groups, and warps that copy, issue S^T, issue O^T, prepare queries, and join and write results (four)
-constexpr int kSoftmaxRegisters = 88, kControlRegisters = 48;
-static_assert(kGroups * kGroupThreads * kSoftmaxRegisters + 384 * kControlRegisters <= kThreads * 72, "what a block of this size is launched with");
+// The warps of a block for items of so many rows: a softmax thread has a token and up to eight rows.  Behind the groups come the warps that copy, issue
+// S^T, issue O^T, prepare queries, and join and write results (four, from a multiple of four on).
+template <int kRows>
+struct Roles {
+  static constexpr int kMine = kRows < 8 ? kRows : 8, kHalves = kRows / kMine;
+  static constexpr int kGroupWarps = 4 * kHalves, kGroupThreads = 32 * kGroupWarps;
+  static constexpr int kCopy = kGroups * kGroupWarps, kScore = kCopy + kCopyWarps, kValue = kScore + 1, kQuery = kScore + 2, kResult = kCopy + 8;
+  static constexpr int kThreads = 32 * (kResult + 4);
+  static constexpr int kLaunched = 65536 / kThreads / 8 * 8;                               // registers of a thread
+  static constexpr int kControlRegisters = 48;
+  static constexpr int kSoftmaxRegisters = (kThreads * kLaunched - 384 * kControlRegisters) / (kGroups * kGroupThreads) / 8 * 8;
+};
 constexpr int kDeep = 3;                // items between their queries and their results
 constexpr int kTile = 128;              // tokens
 constexpr int kTileBytes = kTile * 128; // of keys, or of values
 constexpr int kSlots = 10;              // tiles of keys or of values in the ring, in turn
 constexpr int kScaleSlots = 8;          // tiles' scales; see the copies
 constexpr int kBatch = 256;             // sequences whose items are laid out at a time
-constexpr int kClasses = kPartTokens / kTile + 1;
+constexpr int kClasses = kLongPart / kTile + 1;
 constexpr float kHighest = 8.0f, kFresh = 6.0f;
 constexpr float kFaint = -100.0f;       // log2 of a weight whose product with 1 / scale_v may leave fp32
 constexpr float kWide = 30.0f;          // log2 of a value scale that makes that possible
@@ -75,7 +81,7 @@ struct Work {
 
 template <int kRows>
 struct __align__(1024) Shared {
-  static constexpr int kN = kRows == 16 ? 48 : 32;    // three parts of every row, in whole sixteens
+  static constexpr int kN = (3 * kRows + 15) / 16 * 16;         // three parts of every row, in whole sixteens
   unsigned char ring[kSlots][kTileBytes];             // [token][128 bytes], swizzled by the copy: keys of a tile, its values, the next tile's keys ..
   unsigned char q[kDeep][kN * 128];                   // [item][part of a row][128 elements]
   unsigned char p[kGroups][2][kN * 128];              // of a group's tiles in turn: [part of a row][128 tokens]
@@ -92,8 +98,9 @@ struct __align__(1024) Shared {
   alignas(16) uint32_t nan_value[kDeep][kGroups][kRows][4];      // elements that a row gets NaN in
   int marked[kDeep][kGroups];                         // there are some
   // of a group's tile
-  float folded[kGroups][4][kRows];
-  float by[kGroups][kRows], root[kGroups][kRows];     // of a move of references: added to them; the root of what O and l are multiplied by
+  alignas(16) float folded[kGroups][4][kRows];
+  alignas(16) float by[kGroups][kRows];
+  alignas(16) float root[kGroups][kRows];       // of a move of references: added to them (by); the root of what O and l are multiplied by
   uint32_t fresh[kGroups][2];                         // rows of a half without a reference yet
   unsigned moved[kGroups][2];                         // the turn of a half's last move of a reference that had been there
   float4 result[4][kRows];                            // of each result warp: the groups' factors and where a row goes
@@ -126,8 +133,8 @@ struct Spread {
 __device__ __forceinline__ Spread spread_of(int each, int count, int base, int group, int window, int capacity) {
   Spread x;
   const int top = clamp_keys(base + count - 1, capacity), low = window > 0 ? max(clamp_keys(base, capacity) - window, 0) : 0;
-  x.first_part = low / kPartTokens;
-  x.parts = top > 0 ? (top - 1) / kPartTokens - x.first_part + 1 : 1;
+  x.first_part = part_of(low);
+  x.parts = top > 0 ? part_of(top - 1) - x.first_part + 1 : 1;
   x.tiles = (count * group + each - 1) / each;
   return x;
 }
@@ -167,8 +174,8 @@ __device__ __noinline__ Item find_item(const Work* work, int batch, int sequence
   x.pair0 = (cell < whole ? local - chunk * spread.tiles : local) * each;
   x.pairs = min(x.count * group - x.pair0, each);
   const int least = clamp_keys(x.base + x.pair0 / group, capacity), top = clamp_keys(x.base + (x.pair0 + x.pairs - 1) / group, capacity);
-  x.from = max(window > 0 ? max(least - window, 0) : 0, x.part * kPartTokens);
-  x.end = min(top, (x.part + 1) * kPartTokens);
+  x.from = max(window > 0 ? max(least - window, 0) : 0, part_begin(x.part));
+  x.end = min(top, part_begin(x.part + 1));
   x.all_from = max(window > 0 ? max(top - window, 0) : 0, x.from);
   x.all_end = min(least, x.end);
   x.begin = x.from / kTile * kTile;
@@ -210,13 +217,13 @@ __device__ __forceinline__ void store_columns(uint32_t at, const float (&x)[kCou
   }
 }
 // A group's barrier, with the OR of a predicate.
-__device__ __forceinline__ bool group_any(int group, bool mine) {
+template <int kGroupThreads>
+__device__ __forceinline__ bool any_of_group(int group, bool mine) {
   uint32_t any;
   asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbarrier.cta.red.or.pred q, %2, %3, p;\nselp.u32 %0, 1, 0, q;\n}\n"
                : "=r"(any) : "r"(mine ? 1u : 0u), "r"(1 + group), "n"(kGroupThreads) : "memory");
   return any != 0;
 }
-__device__ __forceinline__ void block_sync() { asm volatile("bar.sync 4, %0;" ::"n"(kThreads) : "memory"); }
 
 // Two numbers as packed codes of their three parts, x = h + m / 32 + l / 1024 for |x| <= 256: x in half precision (2^-11 of it, or 2^-25), then
 // h and m rounded by the conversion to a code; what each leaves, times 32, is exact in half precision.
@@ -243,11 +250,10 @@ __device__ __forceinline__ float4 load_shared16f(uint32_t at) {
   return v;
 }
 
-// Folds kCount values over the lanes of a warp, all of them at once: at every step a lane gives half of its values away and takes the other half's
+// Adds kCount values up over the lanes of a warp, all of them at once: at every step a lane gives half of its values away and takes the other half's
 // partners.  Returns value row_after_fold(lane) of them, complete, in every lane.
-template <int kCount, bool kMax>
+template <int kCount>
 __device__ __forceinline__ float fold_rows(float (&v)[kCount], int lane) {
-  auto op = [](float a, float b) { return kMax ? fmaxf(a, b) : a + b; };
   int bit = 16;
 #pragma unroll
   for (int half = kCount / 2; half > 0; half /= 2, bit /= 2) {
@@ -255,12 +261,17 @@ __device__ __forceinline__ float fold_rows(float (&v)[kCount], int lane) {
 #pragma unroll
     for (int i = 0; i < half; ++i) {
       const float give = upper ? v[i] : v[i + half], stay = upper ? v[i + half] : v[i];
-      v[i] = op(stay, __shfl_xor_sync(0xffffffffu, give, bit));
+      v[i] = stay + __shfl_xor_sync(0xffffffffu, give, bit);
     }
   }
   float x = v[0];
-  for (; bit > 0; bit /= 2) x = op(x, __shfl_xor_sync(0xffffffffu, x, bit));
+  for (; bit > 0; bit /= 2) x += __shfl_xor_sync(0xffffffffu, x, bit);
   return x;
+}
+__device__ __forceinline__ float warp_max(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
 }
 template <int kCount>
 __device__ __forceinline__ int row_after_fold(int lane) { return lane / (32 / kCount); }
@@ -269,10 +280,15 @@ __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7
 
 // kDim: 128, or 64 with two heads side by side, whose pairs are rows 0 .. kRows / 2 - 1 and kRows / 2 .. of an item.
 template <typename T, int kDim, int kRows>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Roles<kRows>::kThreads, 1)
 quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map, QuantizedAttentionArgs a, float scale_log2,
                        int box) {
   using Sm = Shared<kRows>;
+  using Role = Roles<kRows>;
+  constexpr int kThreads = Role::kThreads, kGroupWarps = Role::kGroupWarps, kHalves = Role::kHalves;
+  constexpr int kCopyWarp = Role::kCopy, kScoreWarp = Role::kScore, kValueWarp = Role::kValue, kQueryWarp = Role::kQuery, kResultWarp = Role::kResult;
+  const auto block_sync = [] { asm volatile("bar.sync 4, %0;" ::"n"(kThreads) : "memory"); };
+  const auto group_any = [](int group, bool mine) { return any_of_group<Role::kGroupThreads>(group, mine); };
   constexpr int kHeads = 128 / kDim, kEach = kRows / kHeads, kN = Sm::kN;
   // tensor memory: 64 columns for the scores of each group, then for its outputs of the items under way
   constexpr uint32_t kScores = 0, kOutputs = kGroups * 64, kColumns = 512;
@@ -353,7 +369,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       const Spread x = spread_of(kEach, count, sm.work.base[i], group_heads, a.window, capacity);
       sm.work.whole_before[i] = count > 0 ? (x.parts - 1) * x.tiles : 0;
       const int top = clamp_keys(sm.work.base[i] + count - 1, capacity);
-      sm.work.size_class[i] = static_cast<unsigned char>(top > 0 ? (top - 1) % kPartTokens / kTile + 1 : 0);
+      sm.work.size_class[i] = static_cast<unsigned char>(top > 0 ? (top - 1 - part_begin(part_of(top - 1))) / kTile + 1 : 0);
     }
     block_sync();
     if (warp < kClasses) {
@@ -399,13 +415,13 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
 
   // (a loop for each: what runs with a kind's registers stays apart from the other's)
   if (warp >= kCopyWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegisters));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Role::kControlRegisters));
 #pragma unroll 1
     for (int batch = 0; batch < a.step.sequences; batch += kBatch) {
     const int total = lay_out(batch);
     if (warp >= kCopyWarp && warp < kCopyWarp + kCopyWarps) {
       static_assert(2 * kScaleSlots >= kSlots + 2, "tile n + kScaleSlots is copied after the values of tile n are done with");
-      // ---- copies: warp w has pieces 2w and 2w + 1 (16 tokens each) of every tile, lane 2j + i pages and scales of piece 2w + i of tile j of an item ----
+      // ---- copies: warp w has pieces 2w and 2w + 1 (16 tokens each) of every tile, lane 2j + i pages and scales of piece 2w + i of tile j of an item (a part has up to sixteen) ----
       // What a copy costs is its issue: one warp alone, at four or five cycles for each of its instructions, took 2600 cycles a tile.
       const uint64_t policy = policy_evict_first();
       constexpr int kUnseen = static_cast<int>(0x80000000);               // a piece of a box that no row sees
@@ -595,9 +611,9 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             // element lane * kMine of a 128-byte line whose 16-byte pieces are swizzled by the row; of two heads, the other's half of the line is zero
             const uint32_t line = smem_u32(sm.q[buf]) + r * 128;
             const int byte = (kHeads == 2 ? (r / kEach) * 64 : 0) + lane * kMine;
-            const uint32_t at = line + (byte ^ ((r & 7) << 4));
 #pragma unroll
             for (int part = 0; part < 3; ++part) {
+              const uint32_t at = line + (byte ^ (((part * kRows + r) & 7) << 4));
               if constexpr (kDim == 128) {
                 asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + part * kRows * 128), "r"(codes[0][part] | codes[kMine / 2 - 1][part] << 16) : "memory");
               } else {
@@ -609,7 +625,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         }
         if (first_row == 0 && lane < kRows) {
           const int sees = clamp_keys(x.base + my_row, capacity), low = a.window > 0 ? max(sees - a.window, 0) : 0;
-          const int first_part = low / kPartTokens, last_part = sees > 0 ? (sees - 1) / kPartTokens : first_part;
+          const int first_part = part_of(low), last_part = sees > 0 ? part_of(sees - 1) : first_part;
           sm.keys[buf][lane] = my_live ? min(sees, x.end) : x.end;          // of the part; rows that are none see all of it, and nothing is masked for them
           sm.low[buf][lane] = my_live ? max(low, x.from) : x.from;
           int kind = kNowhere;
@@ -692,14 +708,14 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Role::kSoftmaxRegisters));
 #pragma unroll 1
     for (int batch = 0; batch < a.step.sequences; batch += kBatch) {
       const int total = lay_out(batch);
-      // ---- softmax: a thread has a token and half of the rows (of two heads: one head's); in the end an element of the values and the same rows ----
-      constexpr int kMine = kRows / 2;
-      const int group = warp >> 3, half = (warp >> 2) & 1, own = threadIdx.x & (kTile - 1), row0 = half * kMine;
-      const int head_slot = kHeads == 2 ? half : 0;
+      // ---- softmax: a thread has a token and all or half of the rows (of two heads then: one head's) ----
+      constexpr int kMine = Role::kMine, kOfHead = kHeads == 2 && kHalves == 1 ? kEach : kMine;       // rows of a thread that share a head's scales
+      const int group = warp / kGroupWarps, half = kHalves == 2 ? (warp >> 2) & 1 : 0, own = threadIdx.x & (kTile - 1), row0 = half * kMine;
+      const bool leads = warp % kGroupWarps == 0;
       const uint32_t lanes = (static_cast<uint32_t>((warp & 3) * 32) << 16) + group * 64 + row0;      // and columns
       const uint32_t scores_at = tmem + lanes + kScores;
       // where this thread's weights go: rows of 128 tokens, 16-byte pieces swizzled by the row (a half's first row is a multiple of its rows)
@@ -709,7 +725,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
 #pragma unroll 1
       for (int i = blockIdx.x; i < total; i += gridDim.x) {
         const unsigned buf = buffer();
-        failed = group_any(group, failed || ((warp & 7) == 0 && !wait_for(smem_u32(&sm.q_full[buf]), phase())));
+        failed = group_any(group, failed || (leads && !wait_for(smem_u32(&sm.q_full[buf]), phase())));
         const Item x = sm.item[buf];
         const uint32_t outputs_at = tmem + lanes + kOutputs + buf * kGroups * 64;
         const int mine = tiles_of(x, group);
@@ -730,7 +746,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           // One warp waits, for the product of the tile before the last as well (it has read the weights that this tile's replace); the others wait for
           // it at the group's barrier, which costs no issue slots.
           bool ok = true;
-          if ((warp & 7) == 0 && !failed)
+          if (leads && !failed)
             ok = wait_for(smem_u32(&sm.s_ready[group]), turn & 1) && wait_for(smem_u32(&sm.full[h % kSlots]), (h / kSlots) & 1) &&
                  (turn < 2 || wait_for(smem_u32(&sm.o_done[group][turn & 1]), ((turn >> 1) - 1) & 1));
           if (group_any(group, !ok)) failed = true;
@@ -739,7 +755,9 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           load_columns<kMine>(scores_at, s);
           load_columns<kMine>(scores_at + kRows, m);
           load_columns<kMine>(scores_at + 2 * kRows, rest);
-          const float4 scale = load_shared16f(smem_u32(&sm.scales[scale_slot][head_slot][own >> 4]));
+          float4 scale_of[kMine / kOfHead];
+#pragma unroll
+          for (int h = 0; h < kMine / kOfHead; ++h) scale_of[h] = load_shared16f(smem_u32(&sm.scales[scale_slot][kHeads == 2 && kHalves == 2 ? half : h][own >> 4]));
           const int4 any_wide = sm.wide[scale_slot];
           wide |= (any_wide.x | any_wide.y | any_wide.z | any_wide.w) != 0;
           tmem_load_wait();
@@ -749,9 +767,11 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
 #pragma unroll
           for (int r = 0; r < kMine; r += 4) {
             const float4 row_scale = load_shared16f(smem_u32(&sm.row_scale[buf][row0 + r]));
-            const float2 part = make_float2(0.03125f, 0.03125f), keys_scale = make_float2(scale.x, scale.x), exponent = make_float2(scale.y, scale.y);
+            const float2 part = make_float2(0.03125f, 0.03125f);
 #pragma unroll
             for (int i2 = 0; i2 < 4; i2 += 2) {
+              const float4& scale = scale_of[(r + i2) / kOfHead];
+              const float2 keys_scale = make_float2(scale.x, scale.x), exponent = make_float2(scale.y, scale.y);
               float2 raw = fma_pair(make_float2(rest[r + i2], rest[r + i2 + 1]), part, make_float2(m[r + i2], m[r + i2 + 1]));
               raw = fma_pair(raw, part, make_float2(s[r + i2], s[r + i2 + 1]));
               const float2 factor = mul_pair(i2 ? make_float2(row_scale.z, row_scale.w) : make_float2(row_scale.x, row_scale.y), keys_scale);
@@ -771,12 +791,10 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           for (int r = 2; r < kMine; r += 2) top = max3(top, s[r], s[r + 1]);
           // (the first tile, and rows that have not seen a key: always; the other half's rows need it as well)
           if (group_any(group, top > kHighest || fresh != 0)) {
-            {
-              float most[kMine];
 #pragma unroll
-              for (int r = 0; r < kMine; ++r) most[r] = s[r];
-              const float folded = fold_rows<kMine, true>(most, lane);
-              if (folds) sm.folded[group][warp & 3][folded_row] = folded;
+            for (int r = 0; r < kMine; r += 4) {
+              const float4 most = make_float4(warp_max(s[r]), warp_max(s[r + 1]), warp_max(s[r + 2]), warp_max(s[r + 3]));
+              if (lane == 0) *reinterpret_cast<float4*>(&sm.folded[group][warp & 3][row0 + r]) = most;
             }
             group_any(group, false);
             if (own < kMine) {                     // a row each
@@ -792,11 +810,12 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             group_any(group, false);
             fresh = sm.fresh[group][half];
 #pragma unroll
-            for (int r = 0; r < kMine; ++r) {
-              const float by = sm.by[group][row0 + r], root = sm.root[group][row0 + r];
-              ref[r] += by;
-              s[r] -= by;
-              l[r] = l[r] * root * root;           // in two steps: where a page of far larger values moved the reference, the whole factor may be 0 in fp32 and l not
+            for (int r = 0; r < kMine; r += 4) {
+              const float4 by = load_shared16f(smem_u32(&sm.by[group][row0 + r])), root = load_shared16f(smem_u32(&sm.root[group][row0 + r]));
+              ref[r] += by.x; ref[r + 1] += by.y; ref[r + 2] += by.z; ref[r + 3] += by.w;
+              s[r] -= by.x; s[r + 1] -= by.y; s[r + 2] -= by.z; s[r + 3] -= by.w;
+              // in two steps: where a page of far larger values moved the reference, the whole factor may be 0 in fp32 and l not
+              l[r] = l[r] * root.x * root.x; l[r + 1] = l[r + 1] * root.y * root.y; l[r + 2] = l[r + 2] * root.z * root.z; l[r + 3] = l[r + 3] * root.w * root.w;
             }
             const bool moves = sm.moved[group][half] == turn;
             if (moves && k > 0) {                  // the same for the warps of a half; the output is at rest once the product before is complete
@@ -820,6 +839,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           uint32_t codes[kMine / 2][3];
 #pragma unroll
           for (int r = 0; r < kMine; r += 2) {
+            const float4& scale = scale_of[r / kOfHead];
             float2 p;
             if (!wide) {
               p = make_float2(fast_exp2(s[r]), fast_exp2(s[r + 1]));
@@ -842,17 +862,18 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             const uint32_t at0 = weights + (piece ^ (r << 4)), at1 = weights + (piece ^ ((r + 1) << 4));
 #pragma unroll
             for (int k3 = 0; k3 < 3; ++k3) {
-              store_shared1(at0 + (k3 * kRows + r) * 128, codes[r / 2][k3]);
-              store_shared1(at1 + (k3 * kRows + r + 1) * 128, codes[r / 2][k3] >> 8);
+              constexpr uint32_t kTurn[3] = {0u, (kRows & 7) << 4, (2 * kRows & 7) << 4};      // of the swizzle: parts of four rows start inside eight
+              store_shared1((at0 ^ kTurn[k3]) + (k3 * kRows + r) * 128, codes[r / 2][k3]);
+              store_shared1((at1 ^ kTurn[k3]) + (k3 * kRows + r + 1) * 128, codes[r / 2][k3] >> 8);
             }
           }
           if (ragged) {
             // Slots that no row of the item sees may hold anything, and a weight of zero times NaN is NaN: they are cleared.  NaN in a token that some
-            // rows see and others do not is cleared too, and kept for those that do.  The two threads of a token take 64 bytes each.
+            // rows see and others do not is cleared too, and kept for those that do.  (Of two threads of a token, each takes 64 bytes.)
             unsigned char* value = sm.ring[h % kSlots] + own * 128;
             const bool seen = token >= x.from && token < x.end;
 #pragma unroll 1
-            for (int b = 4 * half; b < 4 * half + 4; ++b) {
+            for (int b = 8 / kHalves * half; b < 8 / kHalves * (half + 1); ++b) {
               uint4* at = reinterpret_cast<uint4*>(value + ((b ^ (own & 7)) << 4));
               const uint4 w = *at;
               if (!seen) {
@@ -881,14 +902,11 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
 
         // what the result warps need
         if (mine > 0) {
-          const float total = fold_rows<kMine, false>(l, lane);
+          const float total = fold_rows<kMine>(l, lane);
           if (folds) sm.l[buf][group][warp & 3][folded_row] = failed ? NAN : total;
-          if (own < kMine) {
-            float own_ref = -INFINITY;
+          if (own == 0) {
 #pragma unroll
-            for (int r = 0; r < kMine; ++r)
-              if (own == r && !((fresh >> r) & 1)) own_ref = ref[r];
-            sm.ref[buf][group][row0 + own] = own_ref;
+            for (int r = 0; r < kMine; ++r) sm.ref[buf][group][row0 + r] = (fresh >> r) & 1 ? -INFINITY : ref[r];
           }
         }
         __syncwarp();
@@ -933,15 +951,15 @@ int launch(const QuantizedAttentionArgs& a, cudaStream_t stream) {
   static_assert(smem <= 227 * 1024, "shared memory of a block");
   auto kernel = quantized_tiles_kernel<T, kDim, kRows>;
   RLT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  return launch_dependent("quantized_tiles_kernel", kernel, dim3(static_cast<unsigned>(info.sm_count)), dim3(kThreads), smem, stream, key_map, value_map, a,
+  return launch_dependent("quantized_tiles_kernel", kernel, dim3(static_cast<unsigned>(info.sm_count)), dim3(Roles<kRows>::kThreads), smem, stream, key_map, value_map, a,
                           static_cast<float>(1.4426950408889634 * a.scale), box);
 }
 
 template <typename T>
 int launch_for(const QuantizedAttentionArgs& a, int max_new, cudaStream_t stream) {
-  // Rows of an item: half the columns where a portion's rows fit (two heads of 64 share an item's rows).
+  // Rows of an item: the fewest that a portion's fit in (two heads of 64 share an item's rows).
   const int64_t pairs = static_cast<int64_t>(max_new) * (a.q_heads / a.cache.kv_heads) * (128 / a.cache.dim);
-  if (a.cache.dim == 128) return pairs <= 8 ? launch<T, 128, 8>(a, stream) : launch<T, 128, 16>(a, stream);
+  if (a.cache.dim == 128) return pairs <= 4 ? launch<T, 128, 4>(a, stream) : (pairs <= 8 ? launch<T, 128, 8>(a, stream) : launch<T, 128, 16>(a, stream));
   return pairs <= 8 ? launch<T, 64, 8>(a, stream) : launch<T, 64, 16>(a, stream);
 }
 

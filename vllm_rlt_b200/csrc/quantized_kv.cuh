@@ -14,7 +14,15 @@ namespace rlt {
 
 constexpr int kMinScaleExponent = -100, kMaxScaleExponent = 100;
 constexpr float kLargestCode = 448.0f;
-constexpr int kPartTokens = 1024;       // a context is split at multiples of this, whatever the batch: a row's bits are its own
+// A context is split at fixed positions, whatever the batch: a row's bits are its own.  1024 tokens at first, so that a few ordinary contexts make
+// enough parts for all SMs; 2048 from 4096 on, where a part's costs (references found anew, its sums written and joined) weigh more.
+constexpr int kShortPart = 1024, kShortParts = 4, kLongPart = 2048;
+__host__ __device__ __forceinline__ int part_of(int token) {
+  return token < kShortParts * kShortPart ? token / kShortPart : kShortParts + (token - kShortParts * kShortPart) / kLongPart;
+}
+__host__ __device__ __forceinline__ int part_begin(int part) {
+  return part <= kShortParts ? part * kShortPart : kShortParts * kShortPart + (part - kShortParts) * kLongPart;
+}
 
 struct QuantizedCache {
   uint8_t* key;
@@ -58,10 +66,10 @@ struct QuantizedAttentionArgs {
 // Floats of one partial: O (dim, rounded up to whole float4), M, l, two unused.
 __host__ __device__ inline int partial_stride(int dim) { return (dim + 3) / 4 * 4 + 4; }
 
-// Parts that a row's keys can span in a table of so many tokens, behind a window: w keys lie in at most ceil((w - 1) / part) + 1 of them.
+// Parts that a row's keys can span in a table of so many tokens, behind a window: w keys lie in at most ceil((w - 1) / part) + 1 parts of one size.
 inline int parts_of(int64_t capacity, int window) {
-  const int64_t all = (capacity + kPartTokens - 1) / kPartTokens;
-  const int64_t seen = window > 0 ? (static_cast<int64_t>(window) + 2 * kPartTokens - 2) / kPartTokens : all;
+  const int all = part_of(static_cast<int>(capacity) - 1) + 1;
+  const int64_t seen = window > 0 ? (static_cast<int64_t>(window) + 2 * kShortPart - 2) / kShortPart : all;
   return static_cast<int>(seen < all ? seen : all);
 }
 
