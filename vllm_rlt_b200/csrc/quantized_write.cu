@@ -9,12 +9,15 @@
 //
 // A run is what one sequence writes to one page in a call; a warp takes a run of one head, so the maximum is one shuffle reduction and
 // nothing is shared between warps.  Runs are found by their first rows: a CTA looks at kWindow rows.
+#include <type_traits>
+
 #include "quantized_kv.cuh"
 
 namespace rlt {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kHeld = 8;                // pieces of a run that a lane keeps in registers
 constexpr int kStaged = 2048;           // sequence bounds kept in shared memory
 
 struct Run {
@@ -24,23 +27,55 @@ struct Run {
   int64_t page;
 };
 
+// kVec elements as they are stored.
 template <typename T, int kVec>
-struct Vec {
-  float x[kVec];
+struct Piece {
+  static constexpr int kWords = kVec == 1 ? 1 : kVec * static_cast<int>(sizeof(T)) / 4;
+  static constexpr bool kPairs = sizeof(T) == 2;
+  // |x| as an unsigned number grows with |x|; from here on it is infinite or NaN
+  static constexpr uint32_t kNotFinite = sizeof(T) == 4 ? 0x7f800000u : (std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u);
+  uint32_t w[kWords];
+
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (kVec == 1) {
-      x[0] = Elem<T>::to_float(*p);
-    } else if constexpr (sizeof(T) == 4) {
-      const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+      if constexpr (kPairs) w[0] = *reinterpret_cast<const uint16_t*>(p);
+      else w[0] = *reinterpret_cast<const uint32_t*>(p);
     } else {
-      const uint4 raw = *reinterpret_cast<const uint4*>(p);
-      const T* t = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) x[i] = Elem<T>::to_float(t[i]);
+      for (int i = 0; i < kWords / 4; ++i) {
+        const uint4 a = reinterpret_cast<const uint4*>(p)[i];
+        w[4 * i] = a.x; w[4 * i + 1] = a.y; w[4 * i + 2] = a.z; w[4 * i + 3] = a.w;
+      }
     }
   }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+  }
+  // the largest of `top` and the |x|, for 16-bit types in two halves
+  __device__ __forceinline__ uint32_t fold(uint32_t top) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) top = kPairs ? __vmaxu2(top, w[i] & 0x7fff7fffu) : max(top, w[i] & 0x7fffffffu);
+    return top;
+  }
+  __device__ __forceinline__ float at(int i) const {
+    T x;
+    if constexpr (kPairs) {
+      const uint16_t half = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+      x = *reinterpret_cast<const T*>(&half);
+    } else {
+      x = *reinterpret_cast<const T*>(&w[i]);
+    }
+    return Elem<T>::to_float(x);
+  }
 };
+
+template <typename T>
+__device__ __forceinline__ float of_bits(uint32_t bits) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(bits);
+  const uint16_t half = static_cast<uint16_t>(bits);
+  return Elem<T>::to_float(*reinterpret_cast<const T*>(&half));
+}
 
 template <int kVec>
 __device__ __forceinline__ void store_codes(uint8_t* p, const float (&x)[kVec]) {
@@ -112,18 +147,50 @@ quantized_write_kernel(QuantizedCache c, PackedRows step, const T* __restrict__ 
     uint8_t* page = (value ? c.value : c.key) + run.page * c.block_stride + static_cast<int64_t>(head) * c.dim;
     float* scale_at = (value ? c.value_scale : c.key_scale) + run.page * c.scale_stride + head;
     const float old = run.offset == 0 ? 0.0f : *scale_at;
-    float largest = 0.0f;
-    for (int i = lane; i < run.count * per_row; i += 32) {
-      Vec<T, kVec> x;
-      x.load(src + (i / per_row) * src_stride + (i % per_row) * kVec);
+    // The run in chunks of kHeld pieces a lane, all of a chunk's loads in flight together; the last chunk (of sixteen tokens with 128
+    // elements there is one) stays in registers for the second pass.
+    using P = Piece<T, kVec>;
+    const int items = run.count * per_row, chunks = (items + 32 * kHeld - 1) / (32 * kHeld), step_rows = 32 / per_row, step_at = 32 % per_row;
+    P x[kHeld];
+    auto each = [&](int chunk, auto&& what) {              // what(j, token of the run, piece of the row) for the lane's pieces of a chunk
+      int i = chunk * 32 * kHeld + lane, t = i / per_row, at = i - t * per_row;
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        const float m = fabsf(x.x[j]);
-        if (m < INFINITY) largest = fmaxf(largest, m);
+      for (int j = 0; j < kHeld; ++j) {
+        if (i < items) what(j, t, at);
+        i += 32; t += step_rows; at += step_at;
+        if (at >= per_row) { at -= per_row; ++t; }
       }
-    }
+    };
+    auto load = [&](int chunk) {
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, x));
+      for (int j = 0; j < kHeld; ++j) x[j].clear();
+      each(chunk, [&](int j, int t, int at) { x[j].load(src + t * src_stride + at * kVec); });
+    };
+    uint32_t top = 0;
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+      load(chunk);
+#pragma unroll
+      for (int j = 0; j < kHeld; ++j) top = x[j].fold(top);
+    }
+    if (P::kPairs) top = max(top & 0xffffu, top >> 16);
+    top = __reduce_max_sync(0xffffffffu, top);
+    const bool finite = top < P::kNotFinite;
+    float largest = of_bits<T>(top);
+    if (!finite) {                                         // rare: once more, for the finite ones
+      largest = 0.0f;
+      for (int chunk = 0; chunk < chunks; ++chunk) {
+        load(chunk);
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+#pragma unroll
+          for (int k = 0; k < kVec; ++k) {
+            const float m = fabsf(x[j].at(k));
+            if (m < INFINITY) largest = fmaxf(largest, m);
+          }
+        }
+      }
+      largest = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(largest)));
+    }
     int e = scale_exponent(largest);
     if (run.offset != 0) e = max(e, exponent_above(old));
     const float scale = power_of_two(e), inverse = power_of_two(-e);
@@ -132,12 +199,19 @@ quantized_write_kernel(QuantizedCache c, PackedRows step, const T* __restrict__ 
       for (int i = lane; i < run.offset * per_row; i += 32) rescale_codes<kVec>(page + (i / per_row) * c.token_stride + (i % per_row) * kVec, ratio);
     }
     if (lane == 0 && (run.offset == 0 || scale != old)) *scale_at = scale;
-    for (int i = lane; i < run.count * per_row; i += 32) {
-      Vec<T, kVec> x;
-      x.load(src + (i / per_row) * src_stride + (i % per_row) * kVec);
+    uint8_t* to = page + run.offset * c.token_stride;
+    for (int chunk = chunks - 1; chunk >= 0; --chunk) {
+      if (chunk < chunks - 1) load(chunk);
+      each(chunk, [&](int j, int t, int at) {
+        float y[kVec];
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) x.x[j] = fabsf(x.x[j]) < INFINITY ? x.x[j] * inverse : NAN;
-      store_codes<kVec>(page + (run.offset + i / per_row) * c.token_stride + (i % per_row) * kVec, x.x);
+        for (int k = 0; k < kVec; ++k) y[k] = x[j].at(k) * inverse;
+        if (!finite) {
+#pragma unroll
+          for (int k = 0; k < kVec; ++k) y[k] = fabsf(x[j].at(k)) < INFINITY ? y[k] : NAN;
+        }
+        store_codes<kVec>(to + t * c.token_stride + at * kVec, y);
+      });
     }
   }
 }
