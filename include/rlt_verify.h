@@ -801,27 +801,21 @@ RLT_API int rlt_return_pages(const int32_t* lengths, int requests, const int32_t
  * rlt_quantized_attention: out[r, h] = sum_t softmax_t(scale * q[r, h] . K[t, h / g]) V[t, h / g], row i of the n_s of a sequence over
  * t < lengths[s] - n_s + i + 1, with window > 0 the last `window` of those; a row that sees no key gives zeros, rows behind
  * cu_rows[sequences] are left alone.  A length beyond table_width * block_size (at most 2^26) is cut to it; a page outside the cache reads as zeros.  q, out:
- * [rows][q_heads][head_dim] with row strides.  max_new: the longest portion (it chooses the kernel, and nothing depends on its being
- * exact).  A row's bits depend on its own query, keys and values only.  workspace: rlt_quantized_attention_workspace_bytes(...) bytes, 16-byte
- * aligned, private to the call until its work on `stream` completes.
- *
- * rlt_quantized_kv_expand: the tokens of every sequence in `dtype` as 16-token pages, [sequences * pages_width][16][kv_heads][head_dim], page p
- * of sequence s at s * pages_width + p, which page_tables (int32 [sequences][pages_width]) then names; slots and entries behind a length
- * are not written.  pages_width * 16 >= table_width * block_size. */
+ * [rows][q_heads][head_dim] with row strides.  max_new: the longest portion.  It, the numbers of rows and sequences and the shape choose the
+ * kernels; among calls that they choose the same ones for, a row's bits depend on its own query, keys and values only.  bf16 portions of
+ * more than 16 rows, long enough on average, are scored over an expansion of the pages in the workspace.  workspace:
+ * rlt_quantized_attention_workspace_bytes(...) bytes, 256-byte aligned, private to the call until its work on `stream` completes. */
 RLT_API int rlt_quantized_kv_write(void* key_cache, void* value_cache, float* key_scale, float* value_scale, int64_t block_stride,
                            int64_t token_stride, int64_t scale_stride, int64_t num_blocks, int block_size, int kv_heads, int head_dim,
                            const void* k, int64_t k_stride, const void* v, int64_t v_stride, int dtype, const int32_t* block_tables,
                            const int32_t* lengths, const int32_t* cu_rows, int sequences, int table_width, int rows, rlt_stream_t stream);
-RLT_API size_t rlt_quantized_attention_workspace_bytes(int rows, int q_heads, int head_dim, int block_size, int table_width, int window);
+RLT_API size_t rlt_quantized_attention_workspace_bytes(int rows, int sequences, int max_new, int q_heads, int kv_heads, int head_dim, int block_size,
+                                              int table_width, int window, int dtype);
 RLT_API int rlt_quantized_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const void* key_cache, const void* value_cache,
                             const float* key_scale, const float* value_scale, int64_t block_stride, int64_t token_stride,
                             int64_t scale_stride, int64_t num_blocks, int block_size, int q_heads, int kv_heads, int head_dim, int dtype,
                             const int32_t* block_tables, const int32_t* lengths, const int32_t* cu_rows, int sequences, int table_width,
                             int rows, int max_new, float scale, int window, void* workspace, size_t workspace_bytes, rlt_stream_t stream);
-RLT_API int rlt_quantized_kv_expand(const void* key_cache, const void* value_cache, const float* key_scale, const float* value_scale,
-                            int64_t block_stride, int64_t token_stride, int64_t scale_stride, int64_t num_blocks, int block_size,
-                            int kv_heads, int head_dim, const int32_t* block_tables, const int32_t* lengths, int sequences, int table_width,
-                            void* key_pages, void* value_pages, int32_t* page_tables, int pages_width, int dtype, rlt_stream_t stream);
 
 #ifdef __cplusplus
 }

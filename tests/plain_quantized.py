@@ -165,7 +165,7 @@ def attention(q, codes, scales, tables, lengths, cu, *, scale=None, window=0, ou
     return result, (spread, size, tiny, count)
 
 
-def allowed(result, parts, dtype, dim, tiles):
+def allowed(result, parts, dtype, dim, tiles, expanded=False):
     """How far a kernel's output may be from `result`, element by element.
 
     Half a step of the output's type, eps / 2 * |result|, and the weights' errors, each of which moves the output by at most its relative
@@ -178,12 +178,14 @@ def allowed(result, parts, dtype, dim, tiles):
       tiles:  weights are rounded to half precision, 2^-11, and held as three parts of four significant bits, of which eleven bits need no more
               (a part leaves at most 2^-4 of what it took: 2^-4, 2^-8, then three bits for the last); the parts' smallest steps are those of
               the codes, 2^-9 / 1024, half of it 2^-20, at a largest p * value scale of at least 2^6: 2^-26 of it, per key, times
-              the largest code 448."""
+              the largest code 448
+      expanded (long portions in bfloat16, over pages expanded into bfloat16 without a rounding): weights are rounded to bfloat16, half a step
+              of 2^-7, before they meet the values, not in their sum; q is taken as it is."""
     spread, size, tiny, count = parts
     eps = torch.finfo(torch.float32).eps
     weight = 2 * (dim * eps * size + eps * size) + 2 * (4 * 2.0 ** -22 + count * eps / 2)
     if tiles:
-        weight = weight + 2.0 ** -11
+        weight = weight + (2.0 ** -8 if expanded else 2.0 ** -11)
     total = spread * weight + torch.finfo(dtype).eps / 2 * result.abs() + torch.finfo(torch.float32).tiny
     if dtype == torch.float16:
         total = total + 2.0 ** -25                                   # half a step of its smallest numbers

@@ -244,13 +244,22 @@ def attention_case(heads, kv_heads, dim, block, lengths, counts, dtype, *, windo
     return call, dict(window=window, scale=scale), want, parts
 
 
+def is_expanded(call, options):
+    """Whether a step's portions are long enough for pages expanded into bfloat16."""
+    q, cache, tables, _, _, most = call
+    block, kv_heads, dim = cache.key.shape[1:]
+    rows, n, heads = q.shape[0], tables.shape[0], q.shape[1]
+    pays = rows * (heads // kv_heads) // 16 >= 8 * n and rows >= 64 * n and (rows // 256 + n) * heads >= 64
+    return q.dtype == torch.bfloat16 and most > 16 and not options.get("window") and dim in (64, 128) and block % 16 == 0 and pays
+
+
 def check_attention(*args, **kw):
     dtype, dim, block = args[6], args[2], args[3]
     call, options, want, parts = attention_case(*args, **kw)
     out = torch.full(call[0].shape, 7.0, dtype=dtype, device="cuda")
     got = rlt.quantized_attention(*call, out=out, **options)
     assert got is out
-    tol = plain.allowed(want, parts, dtype, dim, tiles=dtype != torch.float32)
+    tol = plain.allowed(want, parts, dtype, dim, tiles=dtype != torch.float32, expanded=is_expanded(call, options))
     err = (got.cpu().double() - want).abs()
     assert bool((err <= tol).all()), (float((err / tol).max()), int((err > tol).sum()))
     return call, options, got
@@ -380,6 +389,80 @@ def test_pages_of_unlike_scales_and_scales_that_are_no_powers_of_two(dtype, dim)
         assert bool((err[fits] <= tol[fits]).all()), (kind, float((err[fits] / tol[fits]).max()))
 
 
+LONG = [
+    (32, 32, 128, 16, [300, 700], [300, 129], {}),
+    (32, 8, 128, 32, [513, 100, 1, 65], [257, 100, 1, 17], {}),
+    (14, 2, 64, 64, [4100, 90, 0, 2050], [60, 33, 40, 200], {}),                  # a sequence of padding rows in between
+    (16, 1, 64, 16, [1000], [1000], dict(strided=True)),
+    (32, 16, 128, 48, [200, 31], [128, 64], dict(scale=0.3, spare=0)),            # rows at negative positions
+    (32, 8, 128, 16, [64, 17], [64, 64], dict(width=100)),
+]
+
+
+@pytest.mark.parametrize("heads, kv_heads, dim, block, lengths, counts, more", LONG)
+def test_long_portions(heads, kv_heads, dim, block, lengths, counts, more):
+    args = (heads, kv_heads, dim, block, lengths, counts, torch.bfloat16)
+    call, options, got = check_attention(*args, **more)
+    assert is_expanded(call, options)
+    few = rlt.quantized_attention(*call[:5], 16, out=torch.full(call[0].shape, 7.0, dtype=torch.bfloat16, device="cuda"), **options)
+    assert not torch.equal(few, got)                              # another kernel's roundings
+    for dtype in (torch.float16, torch.float32):
+        check_attention(*args[:-1], dtype, **more)
+
+
+@pytest.mark.parametrize("dim", [128, 64])
+def test_long_portions_that_an_expansion_cannot_hold(dim):
+    """A sequence with a NaN value, one with a page scale that is no power of two, one beyond its table: each as from short portions' kernel, and
+    the others beside them as they were.  Pages outside the cache are zeros."""
+    lengths, counts = [200, 160, 230, 90, 111], [100, 160, 80, 64, 64]
+    call, options, _, _ = attention_case(16, 4, dim, 16, lengths, counts, torch.bfloat16, spare=0, width=20)
+    q, cache, tables, on, cu, most = call
+    assert is_expanded(call, options)
+    clean = rlt.quantized_attention(*call)
+    starts = plain.starts_of(counts)
+
+    def check(marked, lengths=on):
+        long, short = (rlt.quantized_attention(q, cache, tables, lengths, cu, m) for m in (most, 16))
+        for s in range(5):
+            rows = slice(starts[s], starts[s + 1])
+            same = short if s in marked else clean
+            assert torch.equal(long[rows].nan_to_num(99.0), same[rows].nan_to_num(99.0)), (marked, s)
+        return long
+
+    check([])
+    codes = cache.value.view(torch.uint8)
+    at = (int(tables[1, 7]), 3, 2, 5)                               # token 115 of sequence 1
+    saved = codes[at].clone()
+    codes[at] = 0xff
+    got = check([1])
+    assert got[starts[1] + 115:starts[2], 8:12, 5].isnan().all() and got[starts[1]:starts[1] + 115].isfinite().all()
+    for scale in (cache.key_scale, cache.value_scale):
+        page = int(tables[2, 3])
+        keep = scale[page, 1].clone()
+        for odd in (keep * 1.5, keep * 0, keep * 2.0 ** 120):
+            scale[page, 1] = odd
+            check([1, 2])
+        scale[page, 1] = keep
+    codes[at] = saved
+    far = on.clone()
+    far[4] = 20 * 16 + 7                                            # (its table's other entries name pages of other sequences, or none)
+    tables[4, 7:] = tables[4, :1]
+    check([4], far)
+    keys = cache.key.view(torch.uint8)
+    keys[int(tables[3, 1])] = 0x7f                                  # keys that are NaN need no marks: who sees them is NaN
+    got = rlt.quantized_attention(*call)
+    assert got[starts[3]:starts[4]].isnan().all() and torch.equal(got[:starts[3]], clean[:starts[3]])
+    tables[0, 2], tables[0, 5] = -1, 1 << 20
+    raw = [torch.nan_to_num(t.cpu().double()) for t in (cache.key, cache.value, cache.key_scale, cache.value_scale)]
+    raw = [torch.cat((t, torch.zeros_like(t[:1]))) for t in raw]    # a page of zeros behind the others
+    named = tables.cpu()[:1].clone()
+    named[0, 2] = named[0, 5] = raw[0].shape[0] - 1
+    want, parts = plain.attention(q.cpu()[:100], raw[:2], raw[2:], named, [200], [0, 100])
+    got = rlt.quantized_attention(*call)[:100]
+    tol = plain.allowed(want, parts, torch.bfloat16, dim, tiles=True, expanded=True)
+    assert bool(((got.cpu().double() - want).abs() <= tol).all())
+
+
 def test_rows_of_extreme_size():
     """Queries near the largest and smallest numbers of their type, beside ordinary ones."""
     for dtype, sizes in ((torch.bfloat16, [1e30, 1e-30, 0.0, 1.0]), (torch.float16, [60000.0, 1e-6, 0.0, 1.0]), (torch.float32, [1e30, 1e-38, 0.0, 1.0])):
@@ -438,7 +521,8 @@ def test_offsets_beyond_32_bits():
             n = q[rows].shape[0]
             want, parts = plain.attention(q[rows], codes, scales, plain.words([[0, 1, 2]]), lengths, [0, n])
             got = rlt.quantized_attention(q[rows].cuda(), cache, tables.cuda(), plain.words(lengths).cuda(), plain.words([0, n]).cuda(), most)
-            err, tol = (got.cpu().double() - want).abs(), plain.allowed(want, parts, dtype, dim, tiles=dtype != torch.float32)
+            tol = plain.allowed(want, parts, dtype, dim, tiles=dtype != torch.float32)
+            err = (got.cpu().double() - want).abs()
             assert bool((err <= tol).all())
 
 

@@ -123,11 +123,23 @@ def test_the_c_entries_refuse_without_a_launch():
     for bad in (dict(heads=3), dict(heads=0), dict(dim=257), dict(width=0), dict(width=(1 << 22) + 1), dict(window=-1), dict(max_new=-1), dict(stride=255),
                 dict(dtype=7), dict(rows=-1)):
         assert attend(**bad) == _capi.ERR_INVALID, bad
-    need = lib.rlt_quantized_attention_workspace_bytes(1, 4, 64, 16, 1000, 0)
+    def bytes_of(rows=1, sequences=1, max_new=1, heads=4, kv=2, dim=64, block=16, width=1000, window=0, dtype=2):
+        return lib.rlt_quantized_attention_workspace_bytes(rows, sequences, max_new, heads, kv, dim, block, width, window, dtype)
+
+    need = bytes_of()
     assert need == 4 * 10 * 4 * (64 + 4)                              # four parts of 1024 tokens and six of 2048
-    assert lib.rlt_quantized_attention_workspace_bytes(1, 4, 64, 16, 64, 0) == 0
-    assert lib.rlt_quantized_attention_workspace_bytes(1, 4, 64, 16, 1000, 1) == 0
-    assert lib.rlt_quantized_attention_workspace_bytes(1, 4, 64, 16, 1000, 2) == 4 * 2 * 4 * (64 + 4)
+    assert bytes_of(width=64) == bytes_of(window=1) == bytes_of(rows=0) == bytes_of(sequences=0) == 0
+    assert bytes_of(window=2) == 4 * 2 * 4 * (64 + 4)
+    long = dict(rows=256, max_new=256, heads=32)
+    parts = 256 * 32 * 10 * 4 * (64 + 4)
+    assert bytes_of(**long) > 2 * 16000 * 2 * 64 * 2 + parts          # and 16000 expanded tokens
+    for short in (dict(max_new=16), dict(dtype=1), dict(dtype=0), dict(sequences=5), dict(sequences=65536), dict(dim=65 + 31), dict(block=8, width=2000),
+                  dict(heads=30), dict(heads=32, kv=32, rows=127)):
+        given = dict(long, **short)
+        assert bytes_of(**given) == 4 * given["rows"] * given["heads"] * 10 * (given.get("dim", 64) + 4), short
+    assert bytes_of(**long, window=5) == 4 * 256 * 32 * 2 * (64 + 4)
+    wide = dict(long, width=1 << 22, heads=64, kv=1, dim=128)         # 2^26 tokens are not expanded
+    assert bytes_of(**wide) == 4 * 256 * 64 * (4 + (1 << 15) - 2) * 132
     assert attend(width=1000, nbytes=need - 1) == _capi.ERR_WORKSPACE
     assert attend(width=1000, nbytes=need, ws=p + 4) == _capi.ERR_WORKSPACE
     assert attend(width=1000, nbytes=need, ws=null) == _capi.ERR_WORKSPACE
@@ -140,13 +152,6 @@ def test_the_c_entries_refuse_without_a_launch():
     for bad in (dict(n=8193), dict(block=0), dict(count=null)):
         given = dict(dict(n=1, block=16, count=p), **bad)
         assert lib.rlt_return_pages(p, given["n"], p, 2, given["block"], p, p, 4, given["count"], p, null) == _capi.ERR_INVALID, bad
-
-    def expand(sequences=1, pages_width=2, to=p):
-        return lib.rlt_quantized_kv_expand(p, p, p, p, 2048, 128, 2, 4, 16, 2, 64, p, p, sequences, 2, to, p, p, pages_width, 2, null)
-
-    for bad in (dict(pages_width=1), dict(to=null), dict(sequences=65536)):
-        assert expand(**bad) == _capi.ERR_INVALID, bad
-    assert expand(sequences=0) == _capi.OK
 
 
 def test_plain_codes_and_scales():

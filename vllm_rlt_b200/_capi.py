@@ -96,9 +96,8 @@ SIGNATURES = {
     "rlt_step_slots": (_I, [_P, _P, _I, _P, _I, _I, _P, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "rlt_return_pages": (_I, [_P, _I, _P, _I, _I, _P, _P, _I, _P, _P, _P]),
     "rlt_quantized_kv_write": (_I, [_P, _P, _P, _P, _L, _L, _L, _L, _I, _I, _I, _P, _L, _P, _L, _I, _P, _P, _P, _I, _I, _I, _P]),
-    "rlt_quantized_attention_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I]),
+    "rlt_quantized_attention_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I, _I, _I, _I, _I]),
     "rlt_quantized_attention": (_I, [_P, _L, _P, _L, _P, _P, _P, _P, _L, _L, _L, _L, _I, _I, _I, _I, _I, _P, _P, _P, _I, _I, _I, _I, _F, _I, _P, _Z, _P]),
-    "rlt_quantized_kv_expand": (_I, [_P, _P, _P, _P, _L, _L, _L, _L, _I, _I, _I, _P, _P, _I, _I, _P, _P, _P, _I, _I, _P]),
     "rlt_step_metadata": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _L, _L]),
 }
 

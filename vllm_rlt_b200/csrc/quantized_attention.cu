@@ -1,5 +1,4 @@
-// Attention over an 8-bit paged cache: the kernel for every shape, the joining of parts, and the expansion of pages that long portions
-// attend over with the 16-bit prompt kernels.
+// Attention over an 8-bit paged cache: the kernel for every shape, the joining of parts, and the expansion of pages for long portions.
 //
 //   s_t = scale * q . (key_scale[page] * key_code[t]),   p = softmax over the keys a row sees,   out = sum_t p_t * value_scale[page] * value_code[t]
 //
@@ -115,6 +114,7 @@ template <typename T>
 __global__ void __launch_bounds__(kWarps * 32)
 quantized_merge_kernel(QuantizedAttentionArgs a) {
   grid_dependency_wait();
+  if (a.step.only != nullptr && a.step.only[a.step.sequences] == 0) return;
   const QuantizedCache& c = a.cache;
   const int lane = threadIdx.x & 31;
   const int64_t pair = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
@@ -198,64 +198,146 @@ int launch_merge(const QuantizedAttentionArgs& a, cudaStream_t stream) {
                           stream, a);
 }
 
-// ---- expansion ---------------------------------------------------------------------------------------
-// The tokens of every sequence as 16-token pages of T, sequence s in pages s * width16 .., and the tables that say so.  Bound by its
-// traffic: a byte read, two (four) written.
-template <typename T, bool kWide>
+// ---- long portions -----------------------------------------------------------------------------------
+// Tiles of at most sixteen rows read and convert a context once for each of them; a portion of hundreds of rows is bound by that, not by its
+// products.  So its pages are expanded into bf16 once, which has room for every code times 2^-100 .. 2^100 without a rounding, and the
+// prompt kernel of 16-bit caches scores them in tiles of 256 rows.  What that kernel would get wrong is left to the tiles of this one: a
+// sequence with a value that is NaN (its weight of 0 in rows that do not see it would make them NaN), with a page scale that is no power of
+// two (its values would be rounded), or with a length beyond its table (rows are cut one by one here) is marked, and scored behind it.
+//
+// A CTA takes pages of 16 tokens of one sequence: sequence s in pages s * width16 .. of `key` and `value`, and the tables, lengths and row
+// bounds that say so.  Bound by its traffic: a byte read, two written.
+struct Expanded {
+  __nv_bfloat16* key;
+  __nv_bfloat16* value;
+  int32_t* tables;              // [sequences, width16]
+  int32_t* lengths;             // [sequences]
+  int32_t* cu;                  // [sequences + 1]
+  int32_t* marked;              // [sequences + 1], zero before; the last: some sequence is
+  int width16;
+};
+
+// Of four codes in a word: the top bit of each that is NaN (all seven bits under its sign are set).
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+__device__ __forceinline__ bool plain_scale(float scale) {
+  const uint32_t bits = __float_as_uint(scale);
+  return (bits & 0x807fffffu) == 0 && bits >= static_cast<uint32_t>(kMinScaleExponent + 127) << 23 && bits <= static_cast<uint32_t>(kMaxScaleExponent + 127) << 23;
+}
+
 __global__ void __launch_bounds__(256)
-quantized_expand_kernel(QuantizedCache c, PackedRows step, T* key, T* value, int32_t* tables, int width16) {
-  const int s = blockIdx.y;
-  const int64_t length = step.lengths[s];
-  const int tokens = static_cast<int>(length < 0 ? 0 : (length < table_tokens(step, c.block) ? length : table_tokens(step, c.block)));
+quantized_expand_kernel(QuantizedCache c, PackedRows step, Expanded x) {
+  const int s = blockIdx.y, capacity = table_tokens(step, c.block);
+  const int tokens = min(max(step.lengths[s], 0), capacity);
   const int32_t* table = step.tables + static_cast<int64_t>(s) * step.width;
-  constexpr int kVec = kWide ? 8 : 1;
-  const int row = c.kv_heads * c.dim, per_row = row / kVec;
+  bool marks = step.lengths[s] > capacity;
+  if (blockIdx.x == 0) {
+    // bounds inside the rows that never fall, whatever stands in cu: the prompt kernel's list of tiles has room for those
+    __shared__ int s_most[8];
+    int most = 0;
+    for (int i = threadIdx.x; i <= s; i += 256) most = max(most, min(step.cu[i], step.rows));
+    most = static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<unsigned>(max(most, 0))));
+    if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < 8; ++i) most = max(most, s_most[i]);
+      x.cu[s] = most;
+      x.lengths[s] = tokens;
+      if (s == step.sequences - 1) x.cu[s + 1] = max(most, min(step.cu[s + 1], step.rows));
+    }
+  }
+  const int row = c.kv_heads * c.dim, per_row = row / 16;
   for (int p = blockIdx.x; p * 16 < tokens; p += gridDim.x) {
-    const int64_t to = static_cast<int64_t>(s) * width16 + p;
-    if (threadIdx.x == 0) tables[to] = static_cast<int32_t>(to);
-    const int here = min(tokens - p * 16, 16);
+    const int64_t to = static_cast<int64_t>(s) * x.width16 + p;
+    const int entry = p * 16 / c.block, place = p * 16 - entry * c.block, here = min(tokens - p * 16, 16);      // (pages are whole sixteens)
+    const int64_t page = table[entry];
+    const bool there = page >= 0 && page < c.num_pages;
+    if (threadIdx.x == 0) x.tables[to] = static_cast<int32_t>(to);
     for (int i = threadIdx.x; i < here * per_row; i += 256) {
-      const int t = i / per_row, at = (i - t * per_row) * kVec, token = p * 16 + t, entry = token / c.block;
-      const int64_t page = table[entry];
-      const bool there = page >= 0 && page < c.num_pages;
-      const int64_t from = there ? page * c.block_stride + (token - entry * c.block) * c.token_stride + at : 0;
+      const int t = i / per_row, at = (i - t * per_row) * 16;
+      const int64_t from = there ? page * c.block_stride + (place + t) * c.token_stride + at : 0, dst = (to * 16 + t) * row + at;
       const int64_t scale_at = there ? page * c.scale_stride + at / c.dim : 0;
-      const float ks = there ? c.key_scale[scale_at] : 0.0f, vs = there ? c.value_scale[scale_at] : 0.0f;
-      const int64_t dst = (to * 16 + t) * row + at;
-      if constexpr (kWide) {
-        const uint2 kw = there ? *reinterpret_cast<const uint2*>(c.key + from) : make_uint2(0u, 0u);
-        const uint2 vw = there ? *reinterpret_cast<const uint2*>(c.value + from) : make_uint2(0u, 0u);
-        const uint32_t words[4] = {kw.x, kw.y, vw.x, vw.y};
+      const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+      const uint4 kw = there ? *reinterpret_cast<const uint4*>(c.key + from) : zero, vw = there ? *reinterpret_cast<const uint4*>(c.value + from) : zero;
+      const float ks = there ? c.key_scale[scale_at] : 1.0f, vs = there ? c.value_scale[scale_at] : 1.0f;
+      marks |= (nan_codes(vw.x) | nan_codes(vw.y) | nan_codes(vw.z) | nan_codes(vw.w)) != 0 || !plain_scale(ks) || !plain_scale(vs);
+      const uint32_t words[8] = {kw.x, kw.y, kw.z, kw.w, vw.x, vw.y, vw.z, vw.w};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          T x[8];
+      for (int h = 0; h < 2; ++h) {
+        const float scale = h ? vs : ks;
+        uint32_t out[8];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 pair = decode_pair(static_cast<uint16_t>(words[2 * h + (j >> 1)] >> (16 * (j & 1))));
-            x[2 * j] = Elem<T>::from_float(pair.x * (h ? vs : ks));
-            x[2 * j + 1] = Elem<T>::from_float(pair.y * (h ? vs : ks));
-          }
-          T* out = (h ? value : key) + dst;
-#pragma unroll
-          for (int j = 0; j < static_cast<int>(8 * sizeof(T) / 16); ++j) reinterpret_cast<uint4*>(out)[j] = reinterpret_cast<const uint4*>(x)[j];
+        for (int j = 0; j < 8; ++j) {
+          const float2 pair = decode_pair(static_cast<uint16_t>(words[4 * h + (j >> 1)] >> (16 * (j & 1))));
+          const __nv_bfloat162 two = __floats2bfloat162_rn(pair.x * scale, pair.y * scale);
+          out[j] = *reinterpret_cast<const uint32_t*>(&two);
         }
-      } else {
-        key[dst] = Elem<T>::from_float(there ? decode_one(c.key[from]) * ks : 0.0f);
-        value[dst] = Elem<T>::from_float(there ? decode_one(c.value[from]) * vs : 0.0f);
+        uint4* to16 = reinterpret_cast<uint4*>((h ? x.value : x.key) + dst);
+        to16[0] = make_uint4(out[0], out[1], out[2], out[3]);
+        to16[1] = make_uint4(out[4], out[5], out[6], out[7]);
       }
     }
   }
+  if (__syncthreads_or(marks) && threadIdx.x == 0) x.marked[s] = x.marked[step.sequences] = 1;
 }
 
-template <typename T>
-int launch_expand(const QuantizedCache& c, const PackedRows& step, void* key, void* value, int32_t* tables, int width16, int sm_count, cudaStream_t stream) {
-  const bool wide = c.dim % 8 == 0 && c.block_stride % 8 == 0 && c.token_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(c.key) & 7u) == 0 &&
-                    (reinterpret_cast<uintptr_t>(c.value) & 7u) == 0 && aligned16(key) && aligned16(value);
-  const int across = 8 * sm_count / step.sequences + 1;
-  const dim3 grid(static_cast<unsigned>(width16 < across ? width16 : across), static_cast<unsigned>(step.sequences));
-  if (wide) quantized_expand_kernel<T, true><<<grid, 256, 0, stream>>>(c, step, static_cast<T*>(key), static_cast<T*>(value), tables, width16);
-  else quantized_expand_kernel<T, false><<<grid, 256, 0, stream>>>(c, step, static_cast<T*>(key), static_cast<T*>(value), tables, width16);
-  return launch_status("quantized_expand_kernel");
+constexpr size_t kMostExpanded = size_t{4} << 30;      // bytes of expanded pages: tables are as wide as the longest context may become
+
+// Whether a step's portions are long enough, and what the expansion takes of the workspace.
+struct Expansion {
+  bool used;
+  int width16;
+  size_t key, value, tables, lengths, cu, marked, prompt, partials;      // offsets
+};
+size_t aligned_up(size_t n) { return (n + 255) / 256 * 256; }
+Expansion expansion_of(int rows, int sequences, int max_new, int q_heads, int kv_heads, int dim, int block, int width, int window, int dtype) {
+  Expansion e = {};
+  if (max_new <= 16 || window != 0 || dtype != RLT_BF16 || (dim != 64 && dim != 128) || block % 16 != 0 || kv_heads <= 0 || sequences <= 0 || sequences > 65535) return e;
+  // The tiles pass over a context once for sixteen pairs of a row and a head; the prompt kernel has a CTA for 256 rows of a head, however many
+  // of them there are, and walks the context alone.  us, tiles / expanded, heads of 128: 16 portions of 128 rows on 4096 tokens, 16 of 16
+  // heads 570 / 338, 4 such portions 153 / 128, 4 of 1021 rows on 5120 tokens 431 / 119; with fewer rows 16 of 64, 292 / 331, 16 of 32 in
+  // groups of four heads 291 / 359; with few CTAs 1 of 256 on 512 tokens 25 / 31, 1 of 64 in groups of four on 131072 tokens 911 / 1990.
+  const int64_t passes = static_cast<int64_t>(rows) * (q_heads / kv_heads) / 16;
+  const bool pays = passes >= 8ll * sequences && rows >= 64ll * sequences && (static_cast<int64_t>(rows) / 256 + sequences) * q_heads >= 64;
+  e.width16 = static_cast<int>(static_cast<int64_t>(width) * block / 16);
+  const size_t pages = static_cast<size_t>(sequences) * e.width16, bytes = pages * 16 * kv_heads * dim * 2;
+  if (!pays || 2 * bytes > kMostExpanded || pages > 0x7fffffff) return e;
+  e.used = true;
+  e.value = e.key + aligned_up(bytes);
+  e.tables = e.value + aligned_up(bytes);
+  e.lengths = e.tables + aligned_up(pages * 4);
+  e.cu = e.lengths + aligned_up(static_cast<size_t>(sequences) * 4);
+  e.marked = e.cu + aligned_up(static_cast<size_t>(sequences + 1) * 4);
+  e.prompt = e.marked + aligned_up(static_cast<size_t>(sequences + 1) * 4);
+  e.partials = e.prompt + aligned_up(prefill_sm100_workspace_bytes(rows, sequences));
+  return e;
+}
+
+// Scores a step over expanded pages; *scored: false where the prompt kernel does not take its tensors, and nothing was launched that counts.
+int launch_expanded(const QuantizedAttentionArgs& a, const Expansion& e, unsigned char* workspace, int sm_count, bool* scored, cudaStream_t stream) {
+  const QuantizedCache& c = a.cache;
+  *scored = false;
+  if (c.block_stride % 16 != 0 || c.token_stride % 16 != 0 || !aligned16(c.key) || !aligned16(c.value)) return RLT_OK;
+  Expanded x;
+  x.key = reinterpret_cast<__nv_bfloat16*>(workspace + e.key); x.value = reinterpret_cast<__nv_bfloat16*>(workspace + e.value);
+  x.tables = reinterpret_cast<int32_t*>(workspace + e.tables); x.lengths = reinterpret_cast<int32_t*>(workspace + e.lengths);
+  x.cu = reinterpret_cast<int32_t*>(workspace + e.cu); x.marked = reinterpret_cast<int32_t*>(workspace + e.marked); x.width16 = e.width16;
+  AttentionArgs p;
+  p.q = a.q; p.out = a.out; p.key_cache = x.key; p.value_cache = x.value;
+  p.token_stride = static_cast<int64_t>(c.kv_heads) * c.dim; p.block_stride = 16 * p.token_stride; p.num_blocks = static_cast<int64_t>(a.step.sequences) * e.width16;
+  p.block_size = 16; p.q_heads = a.q_heads; p.kv_heads = c.kv_heads; p.head_dim = c.dim; p.dtype = a.dtype; p.block_tables = x.tables;
+  p.table_rows = a.step.sequences; p.table_width = e.width16; p.context_lengths = x.lengths; p.cu_seqlens_q = x.cu; p.rows = a.step.rows;
+  p.value_dim = c.dim; p.v_block_stride = p.block_stride; p.v_token_stride = p.token_stride; p.q_stride = a.q_stride; p.out_stride = a.out_stride;
+  p.terms.scale = a.scale;
+  if (!(a.scale > 0.0f) || !prefill_sm100_supported(p)) return RLT_OK;      // (there a scale of 0 means the usual one, and the largest score is taken before it)
+  RLT_CUDA_TRY(cudaMemsetAsync(x.marked, 0, static_cast<size_t>(a.step.sequences + 1) * 4, stream));
+  const int across = 8 * sm_count / a.step.sequences + 1;
+  quantized_expand_kernel<<<dim3(static_cast<unsigned>(e.width16 < across ? e.width16 : across), static_cast<unsigned>(a.step.sequences)), 256, 0, stream>>>(
+      c, a.step, x);
+  int status = launch_status("quantized_expand_kernel");
+  if (status != RLT_OK) return status;
+  status = launch_prefill_sm100(p, workspace + e.prompt, e.partials - e.prompt, stream);
+  *scored = status == RLT_OK;
+  return status == RLT_ERR_UNSUPPORTED ? RLT_OK : status;
 }
 
 int read_args(QuantizedAttentionArgs& a, const void* key_cache, const void* value_cache, const float* key_scale, const float* value_scale,
@@ -279,11 +361,13 @@ int read_args(QuantizedAttentionArgs& a, const void* key_cache, const void* valu
 }  // namespace
 }  // namespace rlt
 
-extern "C" RLT_API size_t rlt_quantized_attention_workspace_bytes(int rows, int q_heads, int head_dim, int block_size, int table_width, int window) {
+extern "C" RLT_API size_t rlt_quantized_attention_workspace_bytes(int rows, int sequences, int max_new, int q_heads, int kv_heads, int head_dim,
+                                                                  int block_size, int table_width, int window, int dtype) {
   using namespace rlt;
-  if (rows <= 0 || q_heads <= 0 || head_dim <= 0 || block_size <= 0 || table_width <= 0) return 0;
+  if (rows <= 0 || sequences <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || block_size <= 0 || table_width <= 0) return 0;
   const int parts = parts_of(static_cast<int64_t>(table_width) * block_size, window);
-  return parts < 2 ? 0 : sizeof(float) * static_cast<size_t>(rows) * q_heads * parts * partial_stride(head_dim);
+  const Expansion e = expansion_of(rows, sequences, max_new, q_heads, kv_heads, head_dim, block_size, table_width, window, dtype);
+  return e.partials + (parts < 2 ? 0 : sizeof(float) * static_cast<size_t>(rows) * q_heads * parts * partial_stride(head_dim));
 }
 
 extern "C" RLT_API int rlt_quantized_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const void* key_cache,
@@ -305,36 +389,25 @@ extern "C" RLT_API int rlt_quantized_attention(const void* q, int64_t q_stride, 
   RLT_REQUIRE(q_stride >= width && out_stride >= width, "quantized_attention: row strides smaller than a row");
   a.q = q; a.q_stride = q_stride; a.out = out; a.out_stride = out_stride; a.q_heads = q_heads; a.scale = scale; a.window = window;
   a.parts = parts_of(static_cast<int64_t>(table_width) * block_size, window);
-  a.partials = static_cast<float*>(workspace);
-  if (workspace_bytes < rlt_quantized_attention_workspace_bytes(rows, q_heads, head_dim, block_size, table_width, window) ||
-      (a.parts > 1 && (workspace == nullptr || !aligned16(workspace)))) {
+  const Expansion e = expansion_of(rows, sequences, max_new, q_heads, kv_heads, head_dim, block_size, table_width, window, dtype);
+  a.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + e.partials);
+  const size_t needed = rlt_quantized_attention_workspace_bytes(rows, sequences, max_new, q_heads, kv_heads, head_dim, block_size, table_width, window, dtype);
+  if (workspace_bytes < needed || (needed > 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0))) {
     set_last_error_text("quantized_attention: workspace missing, misaligned or too small");
     return RLT_ERR_WORKSPACE;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (e.used) {
+    DeviceInfo info;
+    status = current_device_info(&info);
+    if (status != RLT_OK) return status;
+    bool scored = false;
+    status = launch_expanded(a, e, static_cast<unsigned char*>(workspace), info.sm_count, &scored, s);
+    if (status != RLT_OK) return status;
+    if (scored) a.step.only = reinterpret_cast<const int32_t*>(static_cast<unsigned char*>(workspace) + e.marked);
+  }
   status = quantized_tiles_supported(a) ? launch_quantized_tiles(a, max_new, s) : RLT_ERR_UNSUPPORTED;
   if (status == RLT_ERR_UNSUPPORTED) RLT_DISPATCH_DTYPE(dtype, T, status = launch_rows<T>(a, s));
   if (status != RLT_OK || a.parts < 2) return status;
   RLT_DISPATCH_DTYPE(dtype, T, return launch_merge<T>(a, s));
-}
-
-extern "C" RLT_API int rlt_quantized_kv_expand(const void* key_cache, const void* value_cache, const float* key_scale, const float* value_scale,
-                                               int64_t block_stride, int64_t token_stride, int64_t scale_stride, int64_t num_blocks, int block_size,
-                                               int kv_heads, int head_dim, const int32_t* block_tables, const int32_t* lengths, int sequences,
-                                               int table_width, void* key_pages, void* value_pages, int32_t* page_tables, int pages_width, int dtype,
-                                               rlt_stream_t stream) {
-  using namespace rlt;
-  QuantizedAttentionArgs a = {};
-  int status = read_args(a, key_cache, value_cache, key_scale, value_scale, block_stride, token_stride, scale_stride, num_blocks, block_size, kv_heads,
-                         head_dim, dtype, block_tables, lengths, lengths, sequences, table_width, 1);
-  if (status != RLT_OK || sequences == 0 || table_width == 0) return status;
-  RLT_REQUIRE(key_cache && value_cache && key_scale && value_scale && key_pages && value_pages && page_tables, "quantized_kv_expand: null pointer");
-  RLT_REQUIRE(static_cast<int64_t>(pages_width) * 16 >= static_cast<int64_t>(table_width) * block_size &&
-                  static_cast<int64_t>(pages_width) * sequences <= 0x7fffffff, "quantized_kv_expand: page tables too narrow, or too many pages");
-  RLT_REQUIRE(sequences <= 65535, "quantized_kv_expand: at most 65535 sequences");
-  DeviceInfo info;
-  status = current_device_info(&info);
-  if (status != RLT_OK) return status;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  RLT_DISPATCH_DTYPE(dtype, T, return launch_expand<T>(a.cache, a.step, key_pages, value_pages, page_tables, pages_width, info.sm_count, s));
 }

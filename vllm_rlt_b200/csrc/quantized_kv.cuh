@@ -46,6 +46,7 @@ struct PackedRows {
   int sequences;
   int width;
   int rows;
+  const int32_t* only = nullptr;        // [sequences + 1]: where 0 the sequence has no rows, the last one 0: none has; nullptr: all have theirs
 };
 
 struct QuantizedAttentionArgs {
@@ -77,7 +78,7 @@ inline int parts_of(int64_t capacity, int window) {
 __device__ __forceinline__ void rows_of(const PackedRows& p, int s, int* first, int* count) {
   const int begin = min(max(p.cu[s], 0), p.rows), end = min(max(p.cu[s + 1], begin), p.rows);
   *first = begin;
-  *count = end - begin;
+  *count = p.only == nullptr || p.only[s] != 0 ? end - begin : 0;
 }
 
 // The sequence of a row: the last one that starts at or before it (a row behind the last sequence is in none of them).

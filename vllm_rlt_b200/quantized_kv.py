@@ -43,14 +43,16 @@ class QuantizedKV:
 
     def check(self) -> None:
         key, value, ks, vs = self.key, self.value, self.key_scale, self.value_scale
-        if key.dim() != 4 or value.shape != key.shape or key.stride() != value.stride() or key.dtype != CODE_DTYPE or value.dtype != CODE_DTYPE:
+        shape, stride, scale_stride = key.shape, key.stride(), ks.stride()
+        if len(shape) != 4 or value.shape != shape or value.stride() != stride or key.dtype != CODE_DTYPE or value.dtype != CODE_DTYPE:
             raise ValueError("key and value must be float8_e4m3fn [pages, block, kv_heads, dim] of one layout")
-        if (key.shape[3] > 1 and key.stride(3) != 1) or (key.shape[2] > 1 and key.stride(2) != key.shape[3]):
+        pages, block, heads, dim = shape
+        if (dim > 1 and stride[3] != 1) or (heads > 1 and stride[2] != dim):
             raise ValueError("the [kv_heads, dim] tail of the cache must be contiguous")
-        if not 0 < key.shape[3] <= 256 or key.shape[1] == 0 or key.shape[2] == 0:
+        if not 0 < dim <= 256 or block == 0 or heads == 0:
             raise ValueError("a cache needs tokens, heads, and a dim of 1 .. 256")
-        if ks.dtype != torch.float32 or vs.dtype != torch.float32 or ks.shape != (key.shape[0], key.shape[2]) or vs.shape != ks.shape \
-                or ks.stride() != vs.stride() or (ks.shape[1] > 1 and ks.stride(1) != 1):
+        if ks.dtype != torch.float32 or vs.dtype != torch.float32 or ks.shape != (pages, heads) or vs.shape != ks.shape \
+                or vs.stride() != scale_stride or (heads > 1 and scale_stride[1] != 1):
             raise ValueError("scales must be float32 [pages, kv_heads] of one layout with unit inner stride")
 
 
@@ -72,6 +74,28 @@ def _check_words(n: int, **tensors) -> None:
     for name, t in tensors.items():
         if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous int32 [{n}]")
+
+
+# A decoding step makes these calls once a layer, and their kernels take less time than a call of Python's slower ways would: addresses go to
+# the library as integers, and the device is switched only where it is another.
+def _device_of(*tensors) -> int:
+    """The index of the device that all tensors are on."""
+    index = tensors[0].get_device()
+    if index < 0 or any(t.get_device() != index for t in tensors):
+        _capi.require_cuda(*tensors)                 # says what is wrong
+    return index
+
+
+def _run(what: str, index: int, *args) -> None:
+    entry = getattr(_capi.load(), "rlt_" + what)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch.cuda.current_device() == index:
+        code = entry(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            code = entry(*args, stream)
+    if code:
+        _capi.check(code, what)
 
 
 def _check_stack(tables, held, free_pages, free_count) -> None:
@@ -104,19 +128,20 @@ def step_slots(lengths, counts, tables, block: int, rows: int, *, held=None, fre
         _check_stack(tables, held, free_pages, free_count)
     if block < 1 or rows < 0:
         raise ValueError("block must be positive, rows not negative")
-    device = _capi.require_cuda(lengths, counts, tables, held, free_pages, free_count)
+    if held is None:
+        index, stack = _device_of(lengths, counts, tables), (None, None, 0, None)
+    else:
+        index = _device_of(lengths, counts, tables, held, free_pages, free_count)
+        stack = held.data_ptr(), free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr()
+    device = tables.device
     words = torch.empty(2 * n + 3 + 2 * rows, dtype=torch.int32, device=device)
-    cu, new_lengths, positions, row_seq, last = words.split((n + 1, n, rows, rows, 2))
-    write_blocks, write_offsets = torch.empty(2, rows, dtype=torch.int64, device=device).unbind()
-    active_rows, status = last.unbind()
-    with torch.cuda.device(device):
-        code = _capi.load().rlt_step_slots(
-            _capi.ptr(lengths), _capi.ptr(counts), n, _capi.ptr(tables), width, block, _capi.ptr(held), _capi.ptr(free_pages),
-            0 if free_pages is None else free_pages.numel(), _capi.ptr(free_count), rows, _capi.ptr(cu), _capi.ptr(new_lengths),
-            _capi.ptr(positions), _capi.ptr(row_seq), _capi.ptr(write_blocks), _capi.ptr(write_offsets), _capi.ptr(active_rows), _capi.ptr(status),
-            _capi.stream_of(words))
-    _capi.check(code, "step_slots")
-    return StepSlots(cu, new_lengths, positions, row_seq, write_blocks, write_offsets, active_rows, status)
+    cu, new_lengths, positions, row_seq, last = words.split_with_sizes((n + 1, n, rows, rows, 2))
+    places = torch.empty((2, rows), dtype=torch.int64, device=device)
+    at, place_at = words.data_ptr(), places.data_ptr()
+    end = at + 4 * (2 * n + 1 + 2 * rows)
+    _run("step_slots", index, lengths.data_ptr(), counts.data_ptr(), n, tables.data_ptr(), width, block, *stack, rows, at, at + 4 * (n + 1),
+         at + 4 * (2 * n + 1), at + 4 * (2 * n + 1 + rows), place_at, place_at + 8 * rows, end, end + 4)
+    return StepSlots(cu, new_lengths, positions, row_seq, places[0], places[1], last[0], last[1])
 
 
 def return_pages(lengths, tables, block: int, *, held, free_pages, free_count):
@@ -129,12 +154,10 @@ def return_pages(lengths, tables, block: int, *, held, free_pages, free_count):
     _check_stack(tables, held, free_pages, free_count)
     if block < 1:
         raise ValueError("block must be positive")
-    device = _capi.require_cuda(lengths, tables, held, free_pages, free_count)
-    status = torch.empty((), dtype=torch.int32, device=device)
-    with torch.cuda.device(device):
-        code = _capi.load().rlt_return_pages(_capi.ptr(lengths), n, _capi.ptr(tables), width, block, _capi.ptr(held), _capi.ptr(free_pages),
-                                             free_pages.numel(), _capi.ptr(free_count), _capi.ptr(status), _capi.stream_of(status))
-    _capi.check(code, "return_pages")
+    index = _device_of(lengths, tables, held, free_pages, free_count)
+    status = torch.empty((), dtype=torch.int32, device=tables.device)
+    _run("return_pages", index, lengths.data_ptr(), n, tables.data_ptr(), width, block, held.data_ptr(), free_pages.data_ptr(), free_pages.numel(),
+         free_count.data_ptr(), status.data_ptr())
     return status
 
 
@@ -147,18 +170,19 @@ def _check_step(tables, lengths, cu) -> None:
 
 def _row_stride(t) -> int:
     """Elements between the rows of a [rows, heads, dim] tensor with a contiguous tail, which may be a slice of wider rows."""
-    if (t.shape[2] > 1 and t.stride(2) != 1) or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+    (rows, heads, dim), (row, head, element) = t.shape, t.stride()
+    if (dim > 1 and element != 1) or (heads > 1 and head != dim):
         raise ValueError("the [heads, dim] tail of rows must be contiguous")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    return row if rows > 1 else heads * dim
 
 
 def _cache_args(cache: QuantizedKV) -> tuple:
     """Addresses, strides and pages of a cache; a dimension of one has the stride of a dense layout."""
     key, scale = cache.key, cache.key_scale
-    pages, block, kv_heads, dim = key.shape
-    token = key.stride(1) if block > 1 else kv_heads * dim
-    return (_capi.ptr(key), _capi.ptr(cache.value), _capi.ptr(scale), _capi.ptr(cache.value_scale), key.stride(0) if pages > 1 else block * token, token,
-            scale.stride(0) if pages > 1 else kv_heads, pages)
+    (pages, block, kv_heads, dim), (page_stride, token_stride, _, _) = key.shape, key.stride()
+    token = token_stride if block > 1 else kv_heads * dim
+    return (key.data_ptr(), cache.value.data_ptr(), scale.data_ptr(), cache.value_scale.data_ptr(), page_stride if pages > 1 else block * token, token,
+            scale.stride()[0] if pages > 1 else kv_heads, pages, block)
 
 
 def quantized_kv_write(cache: QuantizedKV, k, v, tables, lengths, cu) -> None:
@@ -178,14 +202,12 @@ def quantized_kv_write(cache: QuantizedKV, k, v, tables, lengths, cu) -> None:
         raise ValueError("k and v must be [rows, kv_heads, dim] of the cache's heads, in float32, float16 or bfloat16")
     rows = k.shape[0]
     k_stride, v_stride = _row_stride(k), _row_stride(v)
-    device = _capi.require_cuda(cache.key, cache.value, cache.key_scale, cache.value_scale, k, v, tables, lengths, cu)
+    index = _device_of(k, v, cache.key, cache.value, cache.key_scale, cache.value_scale, tables, lengths, cu)
     if rows == 0 or pages == 0:
         return
-    with torch.cuda.device(device):
-        code = _capi.load().rlt_quantized_kv_write(
-            *_cache_args(cache), block, kv_heads, dim, _capi.ptr(k), k_stride, _capi.ptr(v), v_stride, _capi.DTYPE_CODES[k.dtype], _capi.ptr(tables),
-            _capi.ptr(lengths), _capi.ptr(cu), tables.shape[0], tables.shape[1], rows, _capi.stream_of(k))
-    _capi.check(code, "quantized_kv_write")
+    sequences, width = tables.shape
+    _run("quantized_kv_write", index, *_cache_args(cache), kv_heads, dim, k.data_ptr(), k_stride, v.data_ptr(), v_stride, _capi.DTYPE_CODES[k.dtype],
+         tables.data_ptr(), lengths.data_ptr(), cu.data_ptr(), sequences, width, rows)
 
 
 def quantized_attention(q, cache: QuantizedKV, tables, lengths, cu, max_new: int, *, scale: float | None = None, window: int = 0, out=None):
@@ -203,11 +225,13 @@ def quantized_attention(q, cache: QuantizedKV, tables, lengths, cu, max_new: int
         raise ValueError("q must be [rows, heads, dim] in float32, float16 or bfloat16, with whole groups of heads over the cache's")
     if isinstance(window, bool) or not isinstance(window, int) or window < 0 or max_new < 0:
         raise ValueError("window and max_new must be integers that are not negative")
-    device = _capi.require_cuda(q, cache.key, cache.value, cache.key_scale, cache.value_scale, tables, lengths, cu, out)
+    index = _device_of(q, cache.key, cache.value, cache.key_scale, cache.value_scale, tables, lengths, cu)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype:
         raise ValueError("out must have q's shape and dtype")
+    else:
+        _device_of(q, out)
     rows, heads, _ = q.shape
     sequences, width = tables.shape
     q_stride, out_stride = _row_stride(q), _row_stride(out)
@@ -215,14 +239,10 @@ def quantized_attention(q, cache: QuantizedKV, tables, lengths, cu, max_new: int
         return out
     if width == 0:
         raise ValueError("tables need at least one page per sequence")
-    window = min(window, 2 ** 31 - 1)
-    lib = _capi.load()
-    with torch.cuda.device(device):
-        nbytes = lib.rlt_quantized_attention_workspace_bytes(rows, heads, dim, block, width, window)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None   # a call's own: graphs and streams share none
-        code = lib.rlt_quantized_attention(
-            _capi.ptr(q), q_stride, _capi.ptr(out), out_stride, *_cache_args(cache), block, heads, kv_heads, dim, _capi.DTYPE_CODES[q.dtype],
-            _capi.ptr(tables), _capi.ptr(lengths), _capi.ptr(cu), sequences, width, rows, int(max_new),
-            float(1.0 / math.sqrt(dim) if scale is None else scale), window, _capi.ptr(workspace), nbytes, _capi.stream_of(q))
-    _capi.check(code, "quantized_attention")
+    window, dtype, max_new = min(window, 2 ** 31 - 1), _capi.DTYPE_CODES[q.dtype], min(int(max_new), rows)
+    nbytes = _capi.load().rlt_quantized_attention_workspace_bytes(rows, sequences, max_new, heads, kv_heads, dim, block, width, window, dtype)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None   # a call's own: graphs and streams share none
+    _run("quantized_attention", index, q.data_ptr(), q_stride, out.data_ptr(), out_stride, *_cache_args(cache), heads, kv_heads, dim, dtype,
+         tables.data_ptr(), lengths.data_ptr(), cu.data_ptr(), sequences, width, rows, max_new,
+         float(1.0 / math.sqrt(dim) if scale is None else scale), window, None if workspace is None else workspace.data_ptr(), nbytes)
     return out
