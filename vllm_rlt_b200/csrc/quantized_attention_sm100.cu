@@ -32,7 +32,7 @@ namespace rlt {
 namespace {
 
 constexpr int kGroups = 2;
-constexpr int kCopyWarps = 4;           // each copies the same quarter of every tile
+constexpr int kPieces = 8;              // of 16 tokens, in a tile
 constexpr int kQueryWarps = 2;          // half of the rows each
 // The warps of a block for items of so many rows: a softmax thread has a token and up to eight rows.  Behind the groups come the warps that copy, issue
 // S^T, issue O^T, prepare queries, and join and write results (four, from a multiple of four on).
@@ -40,11 +40,13 @@ template <int kRows>
 struct Roles {
   static constexpr int kMine = kRows < 8 ? kRows : 8, kHalves = kRows / kMine;
   static constexpr int kGroupWarps = 4 * kHalves, kGroupThreads = 32 * kGroupWarps;
-  static constexpr int kCopy = kGroups * kGroupWarps, kScore = kCopy + kCopyWarps, kValue = kScore + 1, kQuery = kScore + 2, kResult = kCopy + 8;
+  static constexpr int kCopyWarps = kHalves == 2 ? 4 : 8;                                    // each copies the same pieces of every tile
+  static constexpr int kCopy = kGroups * kGroupWarps, kScore = kCopy + kCopyWarps, kValue = kScore + 1, kQuery = kScore + 2, kResult = kScore + 4;
+  static constexpr int kControl = kCopyWarps + 8;
   static constexpr int kThreads = 32 * (kResult + 4);
   static constexpr int kLaunched = 65536 / kThreads / 8 * 8;                               // registers of a thread
   static constexpr int kControlRegisters = 48;
-  static constexpr int kSoftmaxRegisters = (kThreads * kLaunched - 384 * kControlRegisters) / (kGroups * kGroupThreads) / 8 * 8;
+  static constexpr int kSoftmaxRegisters = (kThreads * kLaunched - 32 * kControl * kControlRegisters) / (kGroups * kGroupThreads) / 8 * 8;
 };
 constexpr int kDeep = 3;                // items between their queries and their results
 constexpr int kTile = 128;              // tokens
@@ -52,12 +54,13 @@ constexpr int kTileBytes = kTile * 128; // of keys, or of values
 constexpr int kSlots = 10;              // tiles of keys or of values in the ring, in turn
 constexpr int kScaleSlots = 8;          // tiles' scales; see the copies
 constexpr int kBatch = 256;             // sequences whose items are laid out at a time
+constexpr int kList = 48;               // items of this CTA that are looked up at a time
 constexpr int kClasses = kLongPart / kTile + 1;
 constexpr float kHighest = 8.0f, kFresh = 6.0f;
 constexpr float kFaint = -100.0f;       // log2 of a weight whose product with 1 / scale_v may leave fp32
 constexpr float kWide = 30.0f;          // log2 of a value scale that makes that possible
 
-struct Item {
+struct alignas(16) Item {
   int s, first, count, base;
   int unit;         // 128 bytes of heads
   int pair0;        // the first pair of the item; pairs of every head of the unit
@@ -86,10 +89,10 @@ struct __align__(1024) Shared {
   unsigned char q[kDeep][kN * 128];                   // [item][part of a row][128 elements]
   unsigned char p[kGroups][2][kN * 128];              // of a group's tiles in turn: [part of a row][128 tokens]
   uint32_t raw_q[kRows][64];                          // the next item's queries as they are
-  float4 scales[kScaleSlots][2][kTile / 16];          // by head and 16 tokens: key scale, log2 of the value scale, its inverse
-  int4 wide[kScaleSlots];                             // a value scale of the tile beyond 2^+-kWide; from each copy warp
+  float4 scales[kScaleSlots][2][kPieces];             // by head and 16 tokens: key scale, log2 of the value scale, its inverse
+  alignas(8) unsigned char wide[kScaleSlots][kPieces];      // a value scale of the piece is beyond 2^+-kWide
+  Item list[kList];
   // of an item
-  Item item[kDeep];
   alignas(16) float row_scale[kDeep][kRows];          // of the scores
   int keys[kDeep][kRows], low[kDeep][kRows];          // what a row sees of the part
   int64_t to[kDeep][kRows];                           // where its result goes: elements into the output, or floats into the partials
@@ -304,7 +307,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kSlots; ++i) { mbar_init(smem_u32(&sm.full[i]), kCopyWarps); mbar_init(smem_u32(&sm.empty[i]), 1); }
+    for (int i = 0; i < kSlots; ++i) { mbar_init(smem_u32(&sm.full[i]), Role::kCopyWarps); mbar_init(smem_u32(&sm.empty[i]), 1); }
     for (int i = 0; i < kDeep; ++i) {
       mbar_init(smem_u32(&sm.q_full[i]), kQueryWarps);
       mbar_init(smem_u32(&sm.q_empty[i]), 4);                              // the result warps
@@ -399,8 +402,17 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     return (whole + sm.work.last_before[sequences]) * units;
   };
 
-  auto item_at = [&](int batch, int i) {
-    return find_item(&sm.work, batch, sequences, whole, i, units, kEach, group_heads, a.window, capacity);
+  // Items of this CTA that are looked up together, from its item `base` of the batch on.  The control warps do it, an item each in turn, between two
+  // barriers of the block.
+  auto items_of = [&](int base, int total) {
+    return min((total - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x) - base, kList);
+  };
+  auto look_up = [&](int batch, int base, int items) {
+#pragma unroll 1
+    for (int k = warp - kCopyWarp; k < items; k += Role::kControl) {
+      const Item x = find_item(&sm.work, batch, sequences, whole, blockIdx.x + (base + k) * gridDim.x, units, kEach, group_heads, a.window, capacity);
+      if (lane == 0) sm.list[k] = x;
+    }
   };
   auto group_of = [&](const Item& x, int j) { return (x.begin / kTile + j) & 1; };
   auto tiles_of = [&](const Item& x, int group) { return (x.tiles + (group_of(x, 0) == group ? 1 : 0)) / 2; };
@@ -417,96 +429,109 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   if (warp >= kCopyWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Role::kControlRegisters));
 #pragma unroll 1
-    for (int batch = 0; batch < a.step.sequences; batch += kBatch) {
-    const int total = lay_out(batch);
-    if (warp >= kCopyWarp && warp < kCopyWarp + kCopyWarps) {
+    for (int batch = 0, base = 0, total = 0; batch < a.step.sequences; base += kList) {
+    if (base == 0) total = lay_out(batch);
+    else block_sync();          // the items before are done with
+    const int items = items_of(base, total);
+    look_up(batch, base, items);
+    block_sync();
+    if (items < kList) { batch += kBatch; base = -kList; }
+    if (warp >= kCopyWarp && warp < kScoreWarp) {
       static_assert(2 * kScaleSlots >= kSlots + 2, "tile n + kScaleSlots is copied after the values of tile n are done with");
-      // ---- copies: warp w has pieces 2w and 2w + 1 (16 tokens each) of every tile, lane 2j + i pages and scales of piece 2w + i of tile j of an item (a part has up to sixteen) ----
-      // What a copy costs is its issue: one warp alone, at four or five cycles for each of its instructions, took 2600 cycles a tile.
+      // ---- copies: a warp has one or two pieces of every tile, its lane for tile j of an item (a part has up to sixteen) and piece their pages
+      // and scales ----
+      // What a copy costs is its issue, at four or five cycles for each of a warp's instructions: one warp alone took 2600 cycles a tile, of 1440 that the
+      // memory gives it.  Nothing that waits for the memory stands between the copies of two items: a next item's pages are read when an item's copies
+      // begin, and its scales when a tile of them has gone out.
+      constexpr int kOwn = kPieces / Role::kCopyWarps;
       const uint64_t policy = policy_evict_first();
       constexpr int kUnseen = static_cast<int>(0x80000000);               // a piece of a box that no row sees
-      const int quarter = warp - kCopyWarp;
-      const bool leads0 = ((32 * quarter) & (box - 1)) == 0, leads1 = box == 16;      // the pieces that a box starts with
-      int page, place, next_page = kUnseen, next_place = 0;
-      float4 scales[kHeads];                                              // as the softmax takes them; w: beyond 2^+-kWide
-      Item x, next;
-      x.tiles = 0;
-#pragma unroll 1
-      for (int i_next = blockIdx.x;; i_next += gridDim.x) {                // an item ahead of the copies
-        const bool more = i_next < total;
-        if (more) {
-          next = item_at(batch, i_next);
-          const int token = next.begin + (lane >> 1) * kTile + 32 * quarter + 16 * (lane & 1), entry = token / c.block;
-          const bool seen = lane < 2 * next.tiles && (token & -box) < next.end && (token | (box - 1)) >= next.from;      // (a box lies in one page)
-          next_place = token - entry * c.block;
-          next_page = seen ? a.step.tables[static_cast<int64_t>(next.s) * a.step.width + entry] : kUnseen;
+      const int piece0 = kOwn * (warp - kCopyWarp), piece = piece0 + lane % kOwn;
+      const bool leads0 = ((16 * piece0) & (box - 1)) == 0, leads1 = kOwn == 2 && box == 16;      // the pieces that a box starts with
+      int next_page = kUnseen, next_place = 0;
+      float next_key[kHeads], next_value[kHeads];
+      auto look = [&](const Item& next) {
+        const int token = next.begin + lane / kOwn * kTile + 16 * piece, entry = token / c.block;
+        const bool seen = lane < kOwn * next.tiles && (token & -box) < next.end && (token | (box - 1)) >= next.from;      // (a box lies in one page)
+        next_place = token - entry * c.block;
+        next_page = seen ? a.step.tables[static_cast<int64_t>(next.s) * a.step.width + entry] : kUnseen;
+      };
+      auto load_scales = [&](const Item& next) {
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+          const int64_t at = next_page * c.scale_stride + min(next.unit * kHeads + h, c.kv_heads - 1);
+          // a page outside the cache reads as zeros, which is what the copies of it bring too
+          const bool there = next_page >= 0 && next_page < c.num_pages;
+          next_key[h] = there ? c.key_scale[at] : 0.0f;
+          next_value[h] = there ? c.value_scale[at] : 1.0f;
         }
+      };
+      unsigned slot = 2 * done_tiles % kSlots, turn = 2 * done_tiles / kSlots & 1, scale_slot = done_tiles % kScaleSlots;
+      if (items > 0) {
+        look(sm.list[0]);
+        load_scales(sm.list[0]);
+      }
 #pragma unroll 1
-        for (int j = 0; j < x.tiles && !failed; ++j) {
-          const unsigned n = done_tiles + j, scale_slot = n % kScaleSlots;
-          const int page0 = __shfl_sync(0xffffffffu, page, 2 * j), page1 = __shfl_sync(0xffffffffu, page, 2 * j + 1);
-          const int place0 = __shfl_sync(0xffffffffu, place, 2 * j), place1 = place0 + 16;
+      for (int it = 0; it < items && !failed; ++it) {
+        const int page = next_page, place = next_place, tiles = sm.list[it].tiles, heads_at = sm.list[it].unit * 128;
+        float4 scales[kHeads];                                            // as the softmax takes them
+        bool wide = false;
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+          // a scale that is no positive number within 2^-100 .. 2^100 is brought there: codes of a page of scale 0 then add nothing
+          const float v = fminf(fmaxf(next_value[h], 7.8886090522101181e-31f), 1.2676506002282294e30f);
+          const int e = (__float_as_int(v) >> 23) - 127;
+          const float significand = __int_as_float((__float_as_int(v) & 0x007fffff) | 0x3f800000);        // 1 for powers of two: exact then
+          const float exponent = static_cast<float>(e) + __log2f(significand);
+          scales[h] = make_float4(next_key[h], exponent, power_of_two(-e) * __frcp_rn(significand), 0.0f);
+          wide |= fabsf(exponent) > kWide;
+        }
+        const bool more = it + 1 < items;
+        const Item& next = sm.list[more ? it + 1 : it];
+        if (more) look(next);
+#pragma unroll 1
+        for (int j = 0; j < tiles; ++j) {
+          const int page0 = __shfl_sync(0xffffffffu, page, kOwn * j), place0 = __shfl_sync(0xffffffffu, place, kOwn * j);
+          const int page1 = __shfl_sync(0xffffffffu, page, kOwn * j + kOwn - 1), place1 = place0 + 16 == c.block ? 0 : place0 + 16;      // (in a page of 16 tokens the second piece starts the next page)
           const bool copy0 = leads0 && page0 != kUnseen, copy1 = leads1 && page1 != kUnseen;
-          // (in a page of 16 tokens the second piece starts the next page)
-          const int in_page1 = place1 == c.block ? 0 : place1;
           const uint32_t bytes = static_cast<uint32_t>((copy0 ? 1 : 0) + (copy1 ? 1 : 0)) * box * 128;
 #pragma unroll 1
           for (int values = 0; values < 2; ++values) {
-            const unsigned h = 2 * n + values, slot = h % kSlots;
-            if (h >= kSlots && !wait_for(smem_u32(&sm.empty[slot]), (h / kSlots - 1) & 1)) { failed = true; break; }
+            if (!wait_for(smem_u32(&sm.empty[slot]), turn ^ 1)) { failed = true; break; }                 // (at first the phase before a barrier's first: over)
             if (values == 0) {
               // The slots of the tile kScaleSlots before are free: its values gave theirs back before this tile's keys could be copied.
-              bool wide = false;
-              if ((lane >> 1) == j) {
+              if (lane / kOwn == j) {
 #pragma unroll
-                for (int k = 0; k < kHeads; ++k) {
-                  wide |= scales[k].w != 0.0f;
-                  sm.scales[scale_slot][k][2 * quarter + (lane & 1)] = scales[k];
-                }
+                for (int h = 0; h < kHeads; ++h) sm.scales[scale_slot][h][piece] = scales[h];
+                sm.wide[scale_slot][piece] = wide;
               }
-              wide = __any_sync(0xffffffffu, wide);
-              if (lane == 0) reinterpret_cast<int*>(&sm.wide[scale_slot])[quarter] = wide;
               __syncwarp();                                                // the scales are written
             }
             if (lane == 0) {
-              const uint32_t bar = smem_u32(&sm.full[slot]), dst = smem_u32(sm.ring[slot]) + quarter * 4096;
+              const uint32_t bar = smem_u32(&sm.full[slot]), dst = smem_u32(sm.ring[slot]) + piece0 * 2048;
               const CUtensorMap* map = values ? &value_map : &key_map;
               mbar_expect_tx(bar, bytes);
-              if (copy0) tma_box(dst, map, x.unit * 128, place0, page0, bar, policy);
-              if (copy1) tma_box(dst + 2048, map, x.unit * 128, in_page1, page1, bar, policy);
+              if (copy0) tma_box(dst, map, heads_at, place0, page0, bar, policy);
+              if (copy1) tma_box(dst + 2048, map, heads_at, place1, page1, bar, policy);
             }
             __syncwarp();
+            if (++slot == kSlots) { slot = 0; turn ^= 1; }
           }
+          if (failed) break;
+          scale_slot = (scale_slot + 1) % kScaleSlots;
+          if (j == 0 && more) load_scales(next);
         }
-        if (more) {
-          page = next_page;
-          place = next_place;
-#pragma unroll
-          for (int h = 0; h < kHeads; ++h) {
-            const int head = min(next.unit * kHeads + h, c.kv_heads - 1);
-            // a page outside the cache reads as zeros, which is what the copies of it bring too
-            const bool there = next_page >= 0 && next_page < c.num_pages;
-            const float key = there ? c.key_scale[next_page * c.scale_stride + head] : 0.0f, value = there ? c.value_scale[next_page * c.scale_stride + head] : 1.0f;
-            // a scale that is no positive number within 2^-100 .. 2^100 is brought there: codes of a page of scale 0 then add nothing
-            const float v = fminf(fmaxf(value, 7.8886090522101181e-31f), 1.2676506002282294e30f);
-            const int e = (__float_as_int(v) >> 23) - 127;
-            const float significand = __int_as_float((__float_as_int(v) & 0x007fffff) | 0x3f800000);      // 1 for powers of two: exact then
-            const float exponent = static_cast<float>(e) + __log2f(significand);
-            scales[h] = make_float4(key, exponent, power_of_two(-e) * __frcp_rn(significand), fabsf(exponent) > kWide ? 1.0f : 0.0f);
-          }
-        }
-        done_tiles += x.tiles;
-        if (!more) break;
-        x = next;
+        if (tiles == 0 && more) load_scales(next);
+        done_tiles += tiles;
       }
     } else if (warp == kScoreWarp) {
       // ---- S^T of a tile, once its keys and the item's queries are there and its group has read the scores of the tile before ----
       constexpr uint32_t kIdesc = (1u << 4) | (static_cast<uint32_t>(kN >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
 #pragma unroll 1
-      for (int i = blockIdx.x; i < total && !failed; i += gridDim.x) {
+      for (int it = 0; it < items && !failed; ++it) {
         const unsigned at = buffer();
         bool ok = wait_for(smem_u32(&sm.q_full[at]), phase());
-        const Item x = sm.item[at];
+        const Item x = sm.list[it];
         {
           const uint64_t q_desc = umma_desc(smem_u32(sm.q[at]), 16, 1024);
           unsigned of[kGroups] = {done_of[0], done_of[1]};
@@ -537,10 +562,10 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       // ---- O^T of a tile, once its group's weights are there; its completion gives the stage back ----
       constexpr uint32_t kIdesc = (1u << 4) | (1u << 15) | (static_cast<uint32_t>(kN >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
 #pragma unroll 1
-      for (int i = blockIdx.x; i < total && !failed; i += gridDim.x) {
+      for (int it = 0; it < items && !failed; ++it) {
         const unsigned at = buffer();
         if (!__all_sync(0xffffffffu, wait_for(smem_u32(&sm.q_full[at]), phase()))) { failed = true; break; }
-        const Item x = sm.item[at];
+        const Item x = sm.list[it];
 #pragma unroll 1
         for (int j = 0; j < x.tiles; ++j) {
           const int group = group_of(x, j);
@@ -566,8 +591,8 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       // ---- the queries of an item in three parts, half of the rows each; what its rows see ----
       const int first_row = (warp - kQueryWarp) * (kRows / kQueryWarps);
 #pragma unroll 1
-      for (int i = blockIdx.x; i < total && !failed; i += gridDim.x) {
-        const Item x = item_at(batch, i);
+      for (int it = 0; it < items && !failed; ++it) {
+        const Item x = sm.list[it];
         const unsigned buf = buffer();
         if (done_items >= kDeep && !__all_sync(0xffffffffu, wait_for(smem_u32(&sm.q_empty[buf]), phase() ^ 1))) { failed = true; break; }
         constexpr int kMine = kDim / 32;            // elements of a lane
@@ -591,18 +616,16 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             uint32_t raw[kMine / 2];
 #pragma unroll
             for (int w = 0; w < kMine / 2; ++w) raw[w] = sm.raw_q[r][lane * (kMine / 2) + w];
-            float v[kMine], largest = 0.0f;
-            bool odd = false;                       // a row with an element that is not finite has no scores that are: its references, and so its output, become NaN
+            float v[kMine];
+            uint32_t top = 0;
 #pragma unroll
             for (int w = 0; w < kMine; ++w) {
               v[w] = Elem<T>::to_float(reinterpret_cast<const T*>(raw)[w]);
-              largest = fmaxf(largest, fabsf(v[w]));
-              odd |= !(fabsf(v[w]) < INFINITY);
+              top = max(top, static_cast<uint32_t>(__float_as_int(v[w])) & 0x7fffffffu);
             }
-#pragma unroll
-            for (int y = 16; y > 0; y >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, y));
-            odd = __any_sync(0xffffffffu, odd);
-            const int e = largest > 0.0f && !odd ? max((__float_as_int(largest) >> 23) - 127 - 7, -126) : 0;
+            top = __reduce_max_sync(0xffffffffu, top);
+            const bool odd = top >= 0x7f800000u;    // a row with an element that is not finite has no scores that are: its references, and so its output, become NaN
+            const int e = top > 0 && !odd ? max(static_cast<int>(top >> 23) - 127 - 7, -126) : 0;
             const float up = odd ? 0.0f : power_of_two(-e);
             if (lane == 0) sm.row_scale[buf][r] = odd ? NAN : scale_log2 * power_of_two(e);
             uint32_t codes[kMine / 2][3];
@@ -633,7 +656,6 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           sm.kind[buf][lane] = kind;
           sm.to[buf][lane] = kind == kPartial ? ((at_row * a.q_heads + head) * a.parts + x.part - first_part) * partial_stride(kDim) : at_row * a.out_stride + head * kDim;
         }
-        if (first_row == 0 && lane == 0) sm.item[buf] = x;
         fence_async_proxy();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sm.q_full[buf]));
@@ -644,12 +666,12 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       const int own = threadIdx.x & (kTile - 1), row = lane % kRows;
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
 #pragma unroll 1
-      for (int i = blockIdx.x; i < total; i += gridDim.x) {
+      for (int it = 0; it < items; ++it) {
         const unsigned buf = buffer();
         if (!failed && !wait_for(smem_u32(&sm.done[buf]), phase())) failed = true;
         failed = __any_sync(0xffffffffu, failed);
         tcgen05_after_sync();
-        const Item x = sm.item[buf];
+        const Item x = sm.list[it];
         const bool has0 = tiles_of(x, 0) > 0, has1 = tiles_of(x, 1) > 0;
         // a lane has a row's factors: 2^(R - max R) of each group, over the joined sum where this is the row's only part
         const int kind = sm.kind[buf][row];
@@ -710,8 +732,12 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Role::kSoftmaxRegisters));
 #pragma unroll 1
-    for (int batch = 0; batch < a.step.sequences; batch += kBatch) {
-      const int total = lay_out(batch);
+    for (int batch = 0, base = 0, total = 0; batch < a.step.sequences; base += kList) {
+      if (base == 0) total = lay_out(batch);
+      else block_sync();
+      const int items = items_of(base, total);
+      block_sync();
+      if (items < kList) { batch += kBatch; base = -kList; }
       // ---- softmax: a thread has a token and all or half of the rows (of two heads then: one head's) ----
       constexpr int kMine = Role::kMine, kOfHead = kHeads == 2 && kHalves == 1 ? kEach : kMine;       // rows of a thread that share a head's scales
       const int group = warp / kGroupWarps, half = kHalves == 2 ? (warp >> 2) & 1 : 0, own = threadIdx.x & (kTile - 1), row0 = half * kMine;
@@ -723,10 +749,10 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       const int folded_row = row0 + row_after_fold<kMine>(lane);
       const bool folds = lane % (32 / kMine) == 0;
 #pragma unroll 1
-      for (int i = blockIdx.x; i < total; i += gridDim.x) {
+      for (int it = 0; it < items; ++it) {
         const unsigned buf = buffer();
         failed = group_any(group, failed || (leads && !wait_for(smem_u32(&sm.q_full[buf]), phase())));
-        const Item x = sm.item[buf];
+        const Item x = sm.list[it];
         const uint32_t outputs_at = tmem + lanes + kOutputs + buf * kGroups * 64;
         const int mine = tiles_of(x, group);
         const unsigned before = group ? done_of[1] : done_of[0];
@@ -758,8 +784,8 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           float4 scale_of[kMine / kOfHead];
 #pragma unroll
           for (int h = 0; h < kMine / kOfHead; ++h) scale_of[h] = load_shared16f(smem_u32(&sm.scales[scale_slot][kHeads == 2 && kHalves == 2 ? half : h][own >> 4]));
-          const int4 any_wide = sm.wide[scale_slot];
-          wide |= (any_wide.x | any_wide.y | any_wide.z | any_wide.w) != 0;
+          const uint2 any_wide = *reinterpret_cast<const uint2*>(sm.wide[scale_slot]);
+          wide |= (any_wide.x | any_wide.y) != 0;
           tmem_load_wait();
           tcgen05_before_sync();
           __syncwarp();
@@ -916,7 +942,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     }
   }
   // a wait that gave up left NaN (a result warp's own, at the latest); copies still in flight land before the shared memory is given back
-  if (failed && warp >= kCopyWarp && warp < kCopyWarp + kCopyWarps)
+  if (failed && warp >= kCopyWarp && warp < kScoreWarp)
     for (int i = 0; i < kSlots; ++i)
       if (!wait_for(smem_u32(&sm.full[i]), 0) && !wait_for(smem_u32(&sm.full[i]), 1)) break;
   tcgen05_before_sync();
