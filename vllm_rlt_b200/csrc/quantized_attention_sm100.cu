@@ -40,7 +40,8 @@ template <int kRows>
 struct Roles {
   static constexpr int kMine = kRows < 8 ? kRows : 8, kHalves = kRows / kMine;
   static constexpr int kGroupWarps = 4 * kHalves, kGroupThreads = 32 * kGroupWarps;
-  static constexpr int kCopyWarps = kHalves == 2 ? 4 : 8;                                    // each copies the same pieces of every tile
+  static constexpr bool kSplit = kHalves == 1;                                               // half of eight warps copy keys, half values; else four copy both
+  static constexpr int kCopyWarps = kSplit ? 8 : 4;
   static constexpr int kCopy = kGroups * kGroupWarps, kScore = kCopy + kCopyWarps, kValue = kScore + 1, kQuery = kScore + 2, kResult = kScore + 4;
   static constexpr int kControl = kCopyWarps + 8;
   static constexpr int kThreads = 32 * (kResult + 4);
@@ -51,6 +52,7 @@ struct Roles {
 constexpr int kDeep = 3;                // items between their queries and their results
 constexpr int kTile = 128;              // tokens
 constexpr int kTileBytes = kTile * 128; // of keys, or of values
+static_assert(kPieces * 16 == kTile);
 constexpr int kSlots = 10;              // tiles of keys or of values in the ring, in turn
 constexpr int kScaleSlots = 8;          // tiles' scales; see the copies
 constexpr int kBatch = 256;             // sequences whose items are laid out at a time
@@ -307,7 +309,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kSlots; ++i) { mbar_init(smem_u32(&sm.full[i]), Role::kCopyWarps); mbar_init(smem_u32(&sm.empty[i]), 1); }
+    for (int i = 0; i < kSlots; ++i) { mbar_init(smem_u32(&sm.full[i]), 4); mbar_init(smem_u32(&sm.empty[i]), 1); }
     for (int i = 0; i < kDeep; ++i) {
       mbar_init(smem_u32(&sm.q_full[i]), kQueryWarps);
       mbar_init(smem_u32(&sm.q_empty[i]), 4);                              // the result warps
@@ -438,23 +440,22 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     if (items < kList) { batch += kBatch; base = -kList; }
     if (warp >= kCopyWarp && warp < kScoreWarp) {
       static_assert(2 * kScaleSlots >= kSlots + 2, "tile n + kScaleSlots is copied after the values of tile n are done with");
-      // ---- copies: a warp has one or two pieces of every tile, its lane for tile j of an item (a part has up to sixteen) and piece their pages
-      // and scales ----
-      // What a copy costs is its issue, at four or five cycles for each of a warp's instructions: one warp alone took 2600 cycles a tile, of 1440 that the
-      // memory gives it.  Nothing that waits for the memory stands between the copies of two items: a next item's pages are read when an item's copies
-      // begin, and its scales when a tile of them has gone out.
-      constexpr int kOwn = kPieces / Role::kCopyWarps;
+      // ---- copies: a warp has two pieces of every tile, its lane 2j + i pages and scales of piece i of tile j of an item (a part has up to sixteen) ----
+      // What a copy costs is its issue: a warp alone has an instruction in four or five cycles, a box takes about 200 and the wait in front 270, of 1440
+      // that the memory gives a tile.  So nothing that waits for the memory stands between the copies of two items (a next item's pages are read when
+      // an item's copies begin, and its scales when a tile of them has gone out), and pieces that no row sees are copied too, as zeros from a page that
+      // does not exist.
+      constexpr bool kSplit = Role::kSplit;
       const uint64_t policy = policy_evict_first();
-      constexpr int kUnseen = static_cast<int>(0x80000000);               // a piece of a box that no row sees
-      const int piece0 = kOwn * (warp - kCopyWarp), piece = piece0 + lane % kOwn;
-      const bool leads0 = ((16 * piece0) & (box - 1)) == 0, leads1 = kOwn == 2 && box == 16;      // the pieces that a box starts with
-      int next_page = kUnseen, next_place = 0;
+      const int which = kSplit ? (warp - kCopyWarp) / 4 : 0, piece0 = (warp - kCopyWarp) % 4 * 2, piece = piece0 + (lane & 1);
+      const int boxes = box == 16 ? 2 : ((16 * piece0) % box == 0 ? 1 : 0);      // that start with this warp's pieces
+      int next_page = -1, next_place = 0;
       float next_key[kHeads], next_value[kHeads];
       auto look = [&](const Item& next) {
-        const int token = next.begin + lane / kOwn * kTile + 16 * piece, entry = token / c.block;
-        const bool seen = lane < kOwn * next.tiles && (token & -box) < next.end && (token | (box - 1)) >= next.from;      // (a box lies in one page)
+        const int token = next.begin + (lane >> 1) * kTile + 16 * piece, entry = token / c.block;
+        const bool seen = lane < 2 * next.tiles && (token & -box) < next.end && (token | (box - 1)) >= next.from;      // (a box lies in one page)
         next_place = token - entry * c.block;
-        next_page = seen ? a.step.tables[static_cast<int64_t>(next.s) * a.step.width + entry] : kUnseen;
+        next_page = seen ? a.step.tables[static_cast<int64_t>(next.s) * a.step.width + entry] : -1;
       };
       auto load_scales = [&](const Item& next) {
 #pragma unroll
@@ -466,62 +467,63 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           next_value[h] = there ? c.value_scale[at] : 1.0f;
         }
       };
-      unsigned slot = 2 * done_tiles % kSlots, turn = 2 * done_tiles / kSlots & 1, scale_slot = done_tiles % kScaleSlots;
+      unsigned slot = (2 * done_tiles + which) % kSlots, turn = (2 * done_tiles + which) / kSlots & 1, scale_slot = done_tiles % kScaleSlots;
       if (items > 0) {
         look(sm.list[0]);
-        load_scales(sm.list[0]);
+        if (!kSplit || which == 1) load_scales(sm.list[0]);
       }
 #pragma unroll 1
       for (int it = 0; it < items && !failed; ++it) {
         const int page = next_page, place = next_place, tiles = sm.list[it].tiles, heads_at = sm.list[it].unit * 128;
         float4 scales[kHeads];                                            // as the softmax takes them
         bool wide = false;
+        if (!kSplit || which == 1) {
 #pragma unroll
-        for (int h = 0; h < kHeads; ++h) {
-          // a scale that is no positive number within 2^-100 .. 2^100 is brought there: codes of a page of scale 0 then add nothing
-          const float v = fminf(fmaxf(next_value[h], 7.8886090522101181e-31f), 1.2676506002282294e30f);
-          const int e = (__float_as_int(v) >> 23) - 127;
-          const float significand = __int_as_float((__float_as_int(v) & 0x007fffff) | 0x3f800000);        // 1 for powers of two: exact then
-          const float exponent = static_cast<float>(e) + __log2f(significand);
-          scales[h] = make_float4(next_key[h], exponent, power_of_two(-e) * __frcp_rn(significand), 0.0f);
-          wide |= fabsf(exponent) > kWide;
+          for (int h = 0; h < kHeads; ++h) {
+            // a scale that is no positive number within 2^-100 .. 2^100 is brought there: codes of a page of scale 0 then add nothing
+            const float v = fminf(fmaxf(next_value[h], 7.8886090522101181e-31f), 1.2676506002282294e30f);
+            const int e = (__float_as_int(v) >> 23) - 127;
+            const float significand = __int_as_float((__float_as_int(v) & 0x007fffff) | 0x3f800000);      // 1 for powers of two: exact then
+            const float exponent = static_cast<float>(e) + __log2f(significand);
+            scales[h] = make_float4(next_key[h], exponent, power_of_two(-e) * __frcp_rn(significand), 0.0f);
+            wide |= fabsf(exponent) > kWide;
+          }
         }
         const bool more = it + 1 < items;
         const Item& next = sm.list[more ? it + 1 : it];
         if (more) look(next);
 #pragma unroll 1
-        for (int j = 0; j < tiles; ++j) {
-          const int page0 = __shfl_sync(0xffffffffu, page, kOwn * j), place0 = __shfl_sync(0xffffffffu, place, kOwn * j);
-          const int page1 = __shfl_sync(0xffffffffu, page, kOwn * j + kOwn - 1), place1 = place0 + 16 == c.block ? 0 : place0 + 16;      // (in a page of 16 tokens the second piece starts the next page)
-          const bool copy0 = leads0 && page0 != kUnseen, copy1 = leads1 && page1 != kUnseen;
-          const uint32_t bytes = static_cast<uint32_t>((copy0 ? 1 : 0) + (copy1 ? 1 : 0)) * box * 128;
+        for (int j = 0; j < tiles && !failed; ++j) {
+          const int page0 = __shfl_sync(0xffffffffu, page, 2 * j), place0 = __shfl_sync(0xffffffffu, place, 2 * j);
+          const int page1 = __shfl_sync(0xffffffffu, page, 2 * j + 1), place1 = place0 + 16 == c.block ? 0 : place0 + 16;      // (of a box of its own: in this page or the next)
 #pragma unroll 1
-          for (int values = 0; values < 2; ++values) {
+          for (int values = which; values <= (kSplit ? which : 1); ++values) {
             if (!wait_for(smem_u32(&sm.empty[slot]), turn ^ 1)) { failed = true; break; }                 // (at first the phase before a barrier's first: over)
-            if (values == 0) {
-              // The slots of the tile kScaleSlots before are free: its values gave theirs back before this tile's keys could be copied.
-              if (lane / kOwn == j) {
+            if (values) {
+              // The slots of the tile kScaleSlots before are free: its values gave theirs back before this tile's could be copied.
+              if ((lane >> 1) == j) {
 #pragma unroll
                 for (int h = 0; h < kHeads; ++h) sm.scales[scale_slot][h][piece] = scales[h];
                 sm.wide[scale_slot][piece] = wide;
               }
+              scale_slot = (scale_slot + 1) % kScaleSlots;
               __syncwarp();                                                // the scales are written
             }
             if (lane == 0) {
               const uint32_t bar = smem_u32(&sm.full[slot]), dst = smem_u32(sm.ring[slot]) + piece0 * 2048;
               const CUtensorMap* map = values ? &value_map : &key_map;
-              mbar_expect_tx(bar, bytes);
-              if (copy0) tma_box(dst, map, heads_at, place0, page0, bar, policy);
-              if (copy1) tma_box(dst + 2048, map, heads_at, place1, page1, bar, policy);
+              mbar_expect_tx(bar, static_cast<uint32_t>(boxes * box) * 128);
+              if (boxes > 0) {
+                tma_box(dst, map, heads_at, place0, page0, bar, policy);
+                if (boxes > 1) tma_box(dst + 2048, map, heads_at, place1, page1, bar, policy);
+              }
             }
-            __syncwarp();
-            if (++slot == kSlots) { slot = 0; turn ^= 1; }
+            slot += kSplit ? 2 : 1;
+            if (slot >= kSlots) { slot -= kSlots; turn ^= 1; }
           }
-          if (failed) break;
-          scale_slot = (scale_slot + 1) % kScaleSlots;
-          if (j == 0 && more) load_scales(next);
+          if (j == 0 && more && (!kSplit || which == 1)) load_scales(next);
         }
-        if (tiles == 0 && more) load_scales(next);
+        if (tiles == 0 && more && (!kSplit || which == 1)) load_scales(next);
         done_tiles += tiles;
       }
     } else if (warp == kScoreWarp) {
