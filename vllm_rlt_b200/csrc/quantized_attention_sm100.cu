@@ -57,7 +57,6 @@ constexpr int kSlots = 10;              // tiles of keys or of values in the rin
 constexpr int kScaleSlots = 8;          // tiles' scales; see the copies
 constexpr int kBatch = 256;             // sequences whose items are laid out at a time
 constexpr int kList = 48;               // items of this CTA that are looked up at a time
-constexpr int kClasses = kLongPart / kTile + 1;
 constexpr float kHighest = 8.0f, kFresh = 6.0f;
 constexpr float kFaint = -100.0f;       // log2 of a weight whose product with 1 / scale_v may leave fp32
 constexpr float kWide = 30.0f;          // log2 of a value scale that makes that possible
@@ -79,8 +78,7 @@ enum { kNowhere, kOutput, kZero, kPartial };
 // The work of a batch of sequences: cells (part, row tile) of whole parts in front of a sequence; then the last parts, largest first.
 struct Work {
   int whole_before[kBatch + 1], last_before[kBatch + 1], order[kBatch];
-  int in_class[kClasses];
-  unsigned char size_class[kBatch];
+  int whole[kBatch], last[kBatch];                    // a sequence's cells of whole parts; the tiles of its last part, then its row tiles
   int first[kBatch], count[kBatch], base[kBatch];     // a sequence's rows, and the keys its first row sees (below 1: none)
 };
 
@@ -308,6 +306,8 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(kColumns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if (warp == kCopyWarp && lane < 2)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane ? &value_map : &key_map)) : "memory");
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSlots; ++i) { mbar_init(smem_u32(&sm.full[i]), 4); mbar_init(smem_u32(&sm.empty[i]), 1); }
     for (int i = 0; i < kDeep; ++i) {
@@ -339,25 +339,6 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   bool failed = false;
   int sequences = 0, whole = 0;      // of the batch: sequences, cells of whole parts
 
-  // Exclusive sums of value(i), i < n, into out[0 .. n], by one warp.
-  auto scan = [&](int n, int* out, auto value) {
-    int before = 0;
-#pragma unroll 1
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      const int mine = i0 + lane < n ? value(i0 + lane) : 0;
-      int sum = mine;
-#pragma unroll
-      for (int y = 1; y < 32; y <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, sum, y);
-        if (lane >= y) sum += o;
-      }
-      if (i0 + lane < n) out[i0 + lane] = before + sum - mine;
-      before += __shfl_sync(0xffffffffu, sum, 31);
-    }
-    if (lane == 0) out[n] = before;
-  };
-  auto row_tiles = [&](int i) { return (sm.work.count[i] * group_heads + kEach - 1) / kEach; };
-
   // The items of sequences batch .., by all threads; their number.  Cells of whole parts come first, then every sequence's last part, those with the
   // most tiles first: dealt in this order, one CTA has about as many tiles as another.  The heads of a cell go to neighbouring CTAs at a time.
   auto lay_out = [&](int batch) {
@@ -372,33 +353,32 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       sm.work.count[i] = count;
       sm.work.base[i] = static_cast<int>(base < -0x20000000 ? -0x20000000 : (base > 0x20000000 ? 0x20000000 : base));
       const Spread x = spread_of(kEach, count, sm.work.base[i], group_heads, a.window, capacity);
-      sm.work.whole_before[i] = count > 0 ? (x.parts - 1) * x.tiles : 0;
       const int top = clamp_keys(sm.work.base[i] + count - 1, capacity);
-      sm.work.size_class[i] = static_cast<unsigned char>(top > 0 ? (top - 1 - part_begin(part_of(top - 1))) / kTile + 1 : 0);
+      sm.work.whole[i] = count > 0 ? (x.parts - 1) * x.tiles : 0;
+      sm.work.last[i] = (top > 0 ? (top - 1 - part_begin(part_of(top - 1))) / kTile + 1 : 0) << 24 | x.tiles;
     }
     block_sync();
-    if (warp < kClasses) {
-      int n = 0;
+    // A sequence's place, and what lies in front of it, by comparing it with all the others (a warp's 32 at a time); the sum of all behind the last.
 #pragma unroll 1
-      for (int i0 = 0; i0 < sequences; i0 += 32) n += __popc(__ballot_sync(0xffffffffu, i0 + lane < sequences && sm.work.size_class[i0 + lane] == warp));
-      if (lane == 0) sm.work.in_class[warp] = n;
-    } else if (warp == kClasses) {
-      scan(sequences, sm.work.whole_before, [&](int i) { return sm.work.whole_before[i]; });
-    }
-    block_sync();
-    if (warp < kClasses) {
-      int at = 0;
+    for (int i = warp; i <= sequences; i += kThreads / 32) {
+      const int mine = i < sequences ? sm.work.last[i] >> 24 : -1;
+      int place = 0, whole_before = 0, last_before = 0;
 #pragma unroll 1
-      for (int k = kClasses - 1; k > warp; --k) at += sm.work.in_class[k];
-#pragma unroll 1
-      for (int i0 = 0; i0 < sequences; i0 += 32) {
-        const unsigned mine = __ballot_sync(0xffffffffu, i0 + lane < sequences && sm.work.size_class[i0 + lane] == warp);
-        if ((mine >> lane) & 1) sm.work.order[at + __popc(mine & ((1u << lane) - 1))] = i0 + lane;
-        at += __popc(mine);
+      for (int k = lane; k < sequences; k += 32) {
+        const int last = sm.work.last[k];
+        const bool in_front = last >> 24 > mine || (last >> 24 == mine && k < i);
+        if (k < i) whole_before += sm.work.whole[k];
+        if (in_front) { ++place; last_before += last & 0xffffff; }
+      }
+      place = __reduce_add_sync(0xffffffffu, place);
+      whole_before = __reduce_add_sync(0xffffffffu, whole_before);
+      last_before = __reduce_add_sync(0xffffffffu, last_before);
+      if (lane == 0) {
+        sm.work.whole_before[i] = whole_before;
+        sm.work.last_before[place] = last_before;
+        if (i < sequences) sm.work.order[place] = i;
       }
     }
-    block_sync();
-    if (warp == 0) scan(sequences, sm.work.last_before, [&](int k) { return row_tiles(sm.work.order[k]); });
     block_sync();
     whole = sm.work.whole_before[sequences];
     return (whole + sm.work.last_before[sequences]) * units;
@@ -443,7 +423,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       // ---- copies: a warp has two pieces of every tile, its lane 2j + i pages and scales of piece i of tile j of an item (a part has up to sixteen) ----
       // What a copy costs is its issue: a warp alone has an instruction in four or five cycles, a box takes about 200 and the wait in front 270, of 1440
       // that the memory gives a tile.  So nothing that waits for the memory stands between the copies of two items (a next item's pages are read when
-      // an item's copies begin, and its scales when a tile of them has gone out), and pieces that no row sees are copied too, as zeros from a page that
+      // an item's copies begin, and its scales when its first keys have gone out), and pieces that no row sees are copied too, as zeros from a page that
       // does not exist.
       constexpr bool kSplit = Role::kSplit;
       const uint64_t policy = policy_evict_first();
@@ -477,7 +457,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         const int page = next_page, place = next_place, tiles = sm.list[it].tiles, heads_at = sm.list[it].unit * 128;
         float4 scales[kHeads];                                            // as the softmax takes them
         bool wide = false;
-        if (!kSplit || which == 1) {
+        auto convert = [&] {
 #pragma unroll
           for (int h = 0; h < kHeads; ++h) {
             // a scale that is no positive number within 2^-100 .. 2^100 is brought there: codes of a page of scale 0 then add nothing
@@ -488,7 +468,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             scales[h] = make_float4(next_key[h], exponent, power_of_two(-e) * __frcp_rn(significand), 0.0f);
             wide |= fabsf(exponent) > kWide;
           }
-        }
+        };
         const bool more = it + 1 < items;
         const Item& next = sm.list[more ? it + 1 : it];
         if (more) look(next);
@@ -500,6 +480,10 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           for (int values = which; values <= (kSplit ? which : 1); ++values) {
             if (!wait_for(smem_u32(&sm.empty[slot]), turn ^ 1)) { failed = true; break; }                 // (at first the phase before a barrier's first: over)
             if (values) {
+              if (j == 0) {                                                // (the first item's are still on their way when its keys are copied)
+                convert();
+                if (more) load_scales(next);
+              }
               // The slots of the tile kScaleSlots before are free: its values gave theirs back before this tile's could be copied.
               if ((lane >> 1) == j) {
 #pragma unroll
@@ -521,7 +505,6 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             slot += kSplit ? 2 : 1;
             if (slot >= kSlots) { slot -= kSlots; turn ^= 1; }
           }
-          if (j == 0 && more && (!kSplit || which == 1)) load_scales(next);
         }
         if (tiles == 0 && more && (!kSplit || which == 1)) load_scales(next);
         done_tiles += tiles;
@@ -743,7 +726,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       // ---- softmax: a thread has a token and all or half of the rows (of two heads then: one head's) ----
       constexpr int kMine = Role::kMine, kOfHead = kHeads == 2 && kHalves == 1 ? kEach : kMine;       // rows of a thread that share a head's scales
       const int group = warp / kGroupWarps, half = kHalves == 2 ? (warp >> 2) & 1 : 0, own = threadIdx.x & (kTile - 1), row0 = half * kMine;
-      const bool leads = warp % kGroupWarps == 0;
+      const int waits = warp % kGroupWarps;        // what this warp waits for in its group
       const uint32_t lanes = (static_cast<uint32_t>((warp & 3) * 32) << 16) + group * 64 + row0;      // and columns
       const uint32_t scores_at = tmem + lanes + kScores;
       // where this thread's weights go: rows of 128 tokens, 16-byte pieces swizzled by the row (a half's first row is a multiple of its rows)
@@ -753,7 +736,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
 #pragma unroll 1
       for (int it = 0; it < items; ++it) {
         const unsigned buf = buffer();
-        failed = group_any(group, failed || (leads && !wait_for(smem_u32(&sm.q_full[buf]), phase())));
+        failed = group_any(group, failed || (waits == 0 && !wait_for(smem_u32(&sm.q_full[buf]), phase())));
         const Item x = sm.list[it];
         const uint32_t outputs_at = tmem + lanes + kOutputs + buf * kGroups * 64;
         const int mine = tiles_of(x, group);
@@ -771,12 +754,13 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           const int token0 = x.begin + j * kTile, token = token0 + own;
           // The tile's scales are there with its keys and its values.  Only the values can be waited for: they keep their place until this group's
           // weights have met them, while that of the keys may have been filled again (and its barrier be a whole turn on).
-          // One warp waits, for the product of the tile before the last as well (it has read the weights that this tile's replace); the others wait for
-          // it at the group's barrier, which costs no issue slots.
+          // The product of the tile before the last is waited for as well (it has read the weights that this tile's replace).  A warp each waits for the
+          // three, and all at the group's barrier, which costs no issue slots.
           bool ok = true;
-          if (leads && !failed)
-            ok = wait_for(smem_u32(&sm.s_ready[group]), turn & 1) && wait_for(smem_u32(&sm.full[h % kSlots]), (h / kSlots) & 1) &&
-                 (turn < 2 || wait_for(smem_u32(&sm.o_done[group][turn & 1]), ((turn >> 1) - 1) & 1));
+          if (waits < 3 && !failed) {
+            const uint32_t bar = waits == 0 ? smem_u32(&sm.s_ready[group]) : (waits == 1 ? smem_u32(&sm.full[h % kSlots]) : smem_u32(&sm.o_done[group][turn & 1]));
+            ok = wait_for(bar, waits == 0 ? turn & 1 : (waits == 1 ? (h / kSlots) & 1 : ((turn >> 1) & 1) ^ 1));      // (before the first product: over)
+          }
           if (group_any(group, !ok)) failed = true;
           tcgen05_after_sync();
           float s[kMine], m[kMine], rest[kMine];
