@@ -87,7 +87,7 @@ struct __align__(1024) Shared {
   static constexpr int kN = (3 * kRows + 15) / 16 * 16;         // three parts of every row, in whole sixteens
   unsigned char ring[kSlots][kTileBytes];             // [token][128 bytes], swizzled by the copy: keys of a tile, its values, the next tile's keys ..
   unsigned char q[kDeep][kN * 128];                   // [item][part of a row][128 elements]
-  unsigned char p[kGroups][2][kN * 128];              // of a group's tiles in turn: [part of a row][128 tokens]
+  unsigned char p[kGroups][2][kN * 128];              // of a group's tiles in turn: [16 parts of rows][128 tokens][16 bytes]
   uint32_t raw_q[kRows][64];                          // the next item's queries as they are
   float4 scales[kScaleSlots][2][kPieces];             // by head and 16 tokens: key scale, log2 of the value scale, its inverse
   alignas(8) unsigned char wide[kScaleSlots][kPieces];      // a value scale of the piece is beyond 2^+-kWide
@@ -190,6 +190,11 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, %4}], [%5], %6;"
                ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(token), "r"(page), "r"(bar), "l"(policy) : "memory");
 }
+// An operand of 16-byte pieces of its rows with the columns 16 bytes apart: `rows` bytes between pieces of 16 rows, `columns` between groups of eight
+// columns; no swizzle.
+__device__ __forceinline__ uint64_t piece_desc(uint32_t addr, uint32_t columns, uint32_t rows) {
+  return static_cast<uint64_t>((addr & 0x3ffff) >> 4) | static_cast<uint64_t>(columns >> 4) << 16 | static_cast<uint64_t>(rows >> 4) << 32 | 1ull << 46;
+}
 // D[tmem] (+)= A[smem] * B[smem] of e4m3 codes, one elected thread; 32 codes of K.
 __device__ __forceinline__ void code_product(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
@@ -244,8 +249,9 @@ __device__ __forceinline__ void three_parts(float x0, float x1, uint32_t (&codes
     }
   }
 }
-__device__ __forceinline__ void store_shared1(uint32_t at, uint32_t x) {
-  asm volatile("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %1;\nst.shared.u8 [%0], lo;\n}\n" ::"r"(at), "r"(x) : "memory");
+__device__ __forceinline__ void store_shared8(uint32_t at, uint2 x) { asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(x.x), "r"(x.y) : "memory"); }
+__device__ __forceinline__ void store_shared16(uint32_t at, uint4 x) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
 }
 __device__ __forceinline__ float4 load_shared16f(uint32_t at) {
   float4 v;
@@ -545,7 +551,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       }
     } else if (warp == kValueWarp) {
       // ---- O^T of a tile, once its group's weights are there; its completion gives the stage back ----
-      constexpr uint32_t kIdesc = (1u << 4) | (1u << 15) | (static_cast<uint32_t>(kN >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
+      constexpr uint32_t kIdesc = (1u << 4) | (1u << 15) | (1u << 16) | (static_cast<uint32_t>(kN >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
 #pragma unroll 1
       for (int it = 0; it < items && !failed; ++it) {
         const unsigned at = buffer();
@@ -557,11 +563,11 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           const unsigned h = 2 * (done_tiles + j) + 1, slot = h % kSlots, mine = (group ? done_of[1] : done_of[0]) + j / 2;
           if (!__all_sync(0xffffffffu, wait_for(smem_u32(&sm.full[slot]), (h / kSlots) & 1) && wait_for(smem_u32(&sm.p_ready[group][mine & 1]), (mine >> 1) & 1))) { failed = true; break; }
           tcgen05_after_sync();
-          const uint64_t v_desc = umma_desc(smem_u32(sm.ring[slot]), kTileBytes, 1024), p_desc = umma_desc(smem_u32(sm.p[group][mine & 1]), 16, 1024);
+          const uint64_t v_desc = umma_desc(smem_u32(sm.ring[slot]), kTileBytes, 1024), p_desc = piece_desc(smem_u32(sm.p[group][mine & 1]), 128, kTile * 16);
           if (elect_one()) {
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
-              code_product(tmem + kOutputs + (at * kGroups + group) * 64, v_desc + static_cast<uint64_t>(ks * 4096 >> 4), p_desc + static_cast<uint64_t>(ks * 2), kIdesc,
+              code_product(tmem + kOutputs + (at * kGroups + group) * 64, v_desc + static_cast<uint64_t>(ks * 4096 >> 4), p_desc + static_cast<uint64_t>(ks * 32 * 16 >> 4), kIdesc,
                            (j >= 2 || ks > 0) ? 1u : 0u);
             umma_commit(smem_u32(&sm.o_done[group][mine & 1]));
             umma_commit(smem_u32(&sm.empty[slot]));
@@ -729,8 +735,8 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       const int waits = warp % kGroupWarps;        // what this warp waits for in its group
       const uint32_t lanes = (static_cast<uint32_t>((warp & 3) * 32) << 16) + group * 64 + row0;      // and columns
       const uint32_t scores_at = tmem + lanes + kScores;
-      // where this thread's weights go: rows of 128 tokens, 16-byte pieces swizzled by the row (a half's first row is a multiple of its rows)
-      const uint32_t first_weights = smem_u32(sm.p[group][0]) + row0 * 128 + (own & 15), piece = static_cast<uint32_t>((own >> 4) ^ (row0 & 7)) << 4;
+      // where this thread's weights go: its token's line of 16 bytes, a half's eight of them
+      const uint32_t first_weights = smem_u32(sm.p[group][0]) + own * 16 + half * 8;
       const int folded_row = row0 + row_after_fold<kMine>(lane);
       const bool folds = lane % (32 / kMine) == 0;
 #pragma unroll 1
@@ -869,15 +875,20 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             }
             three_parts(p.x, p.y, codes[r / 2]);
           }
+          // a part of this thread's rows: 4 or 8 bytes; of four rows all parts share a line, of eight rows two do
+          uint32_t words[3][kMine / 4];
 #pragma unroll
-          for (int r = 0; r < kMine; r += 2) {
-            const uint32_t at0 = weights + (piece ^ (r << 4)), at1 = weights + (piece ^ ((r + 1) << 4));
+          for (int k3 = 0; k3 < 3; ++k3)
 #pragma unroll
-            for (int k3 = 0; k3 < 3; ++k3) {
-              constexpr uint32_t kTurn[3] = {0u, (kRows & 7) << 4, (2 * kRows & 7) << 4};      // of the swizzle: parts of four rows start inside eight
-              store_shared1((at0 ^ kTurn[k3]) + (k3 * kRows + r) * 128, codes[r / 2][k3]);
-              store_shared1((at1 ^ kTurn[k3]) + (k3 * kRows + r + 1) * 128, codes[r / 2][k3] >> 8);
-            }
+            for (int w = 0; w < kMine / 4; ++w) words[k3][w] = __byte_perm(codes[2 * w][k3], codes[2 * w + 1][k3], 0x5410);
+          if constexpr (kRows == 4) {
+            store_shared16(weights, make_uint4(words[0][0], words[1][0], words[2][0], 0u));
+          } else if constexpr (kRows == 8) {
+            store_shared16(weights, make_uint4(words[0][0], words[0][1], words[1][0], words[1][1]));
+            store_shared8(weights + kTile * 16, make_uint2(words[2][0], words[2][1]));
+          } else {
+#pragma unroll
+            for (int k3 = 0; k3 < 3; ++k3) store_shared8(weights + k3 * (kTile * 16), make_uint2(words[k3][0], words[k3][1]));
           }
           if (ragged) {
             // Slots that no row of the item sees may hold anything, and a weight of zero times NaN is NaN: they are cleared.  NaN in a token that some
