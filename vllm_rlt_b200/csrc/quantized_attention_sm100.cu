@@ -97,7 +97,8 @@ struct __align__(1024) Shared {
   int keys[kDeep][kRows], low[kDeep][kRows];          // what a row sees of the part
   int64_t to[kDeep][kRows];                           // where its result goes: elements into the output, or floats into the partials
   int kind[kDeep][kRows];                             // kNowhere, kOutput, kZero, kPartial
-  float ref[kDeep][kGroups][kRows], l[kDeep][kGroups][4][kRows];        // of each group; l of each quarter of its tokens
+  alignas(16) float ref[kDeep][kGroups][kRows];
+  float l[kDeep][kGroups][4][kRows];        // of each group; l of each quarter of its tokens
   alignas(16) uint32_t nan_value[kDeep][kGroups][kRows][4];      // elements that a row gets NaN in
   int marked[kDeep][kGroups];                         // there are some
   // of a group's tile
@@ -106,7 +107,7 @@ struct __align__(1024) Shared {
   alignas(16) float root[kGroups][kRows];       // of a move of references: added to them (by); the root of what O and l are multiplied by
   uint32_t fresh[kGroups][2];                         // rows of a half without a reference yet
   unsigned moved[kGroups][2];                         // the turn of a half's last move of a reference that had been there
-  float4 result[4][kRows];                            // of each result warp: the groups' factors and where a row goes
+  float4 result[4][kRows];                            // of each result warp: the groups' factors and the address that a row goes to
   // A waiter may be a phase of a barrier behind, never two (a phase and the one after the next look alike): what has two buffers has two barriers.
   unsigned long long full[kSlots], empty[kSlots], q_full[kDeep], q_empty[kDeep], done[kDeep], s_ready[kGroups], s_free[kGroups], p_ready[kGroups][2], o_done[kGroups][2];
   uint32_t tmem_base;
@@ -482,7 +483,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         for (int j = 0; j < tiles && !failed; ++j) {
           const int page0 = __shfl_sync(0xffffffffu, page, 2 * j), place0 = __shfl_sync(0xffffffffu, place, 2 * j);
           const int page1 = __shfl_sync(0xffffffffu, page, 2 * j + 1), place1 = place0 + 16 == c.block ? 0 : place0 + 16;      // (of a box of its own: in this page or the next)
-#pragma unroll 1
+#pragma unroll
           for (int values = which; values <= (kSplit ? which : 1); ++values) {
             if (!wait_for(smem_u32(&sm.empty[slot]), turn ^ 1)) { failed = true; break; }                 // (at first the phase before a barrier's first: over)
             if (values) {
@@ -675,7 +676,9 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           if (has0) sum = ((sm.l[buf][0][0][row] + sm.l[buf][0][1][row]) + (sm.l[buf][0][2][row] + sm.l[buf][0][3][row])) * root0 * root0;
           if (has1) sum += ((sm.l[buf][1][0][row] + sm.l[buf][1][1][row]) + (sm.l[buf][1][2][row] + sm.l[buf][1][3][row])) * root1 * root1;
           const float scale = failed ? NAN : (kind == kPartial ? 1.0f : (kind == kOutput ? __frcp_rn(sum) : 0.0f));
-          if (lane < kRows) sm.result[warp & 3][row] = make_float4(root0 * root0 * scale, root1 * root1 * scale, __int_as_float(static_cast<int>(to)), __int_as_float(static_cast<int>(to >> 32)));
+          const uint64_t at = kind == kPartial ? reinterpret_cast<uint64_t>(a.partials + to) : reinterpret_cast<uint64_t>(static_cast<T*>(a.out) + to);
+          if (lane < kRows)
+            sm.result[warp & 3][row] = make_float4(root0 * root0 * scale, root1 * root1 * scale, __uint_as_float(static_cast<uint32_t>(at)), __uint_as_float(static_cast<uint32_t>(at >> 32)));
           if (kind == kPartial && lane < kRows && (warp & 3) == 0) *reinterpret_cast<float2*>(a.partials + to + kDim) = make_float2(big, sum);
         }
         const uint32_t partial = __ballot_sync(0xffffffffu, kind == kPartial), nowhere = __ballot_sync(0xffffffffu, kind == kNowhere);
@@ -684,6 +687,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         const uint32_t outputs0 = tmem + lanes + kOutputs + (buf * kGroups) * 64, outputs1 = outputs0 + 64;
 #pragma unroll 1
         for (int r0 = 0; r0 < kRows; r0 += 4) {
+          if (((nowhere >> r0) & 15) == 15) continue;
           const int d = kHeads == 2 ? own - 64 * (r0 / kEach) : own;      // of two heads, a thread's element may be the other one's
           float acc0[4], m0[4], rest0[4], acc1[4], m1[4], rest1[4];
           load_columns<4>(outputs0 + r0, acc0);
@@ -693,18 +697,18 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           load_columns<4>(outputs1 + kRows + r0, m1);
           load_columns<4>(outputs1 + 2 * kRows + r0, rest1);
           tmem_load_wait();
+          if (kHeads == 2 && (d < 0 || d >= kDim)) continue;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int r = r0 + k;
-            const float4 of = sm.result[warp & 3][r];
-            float o0 = fmaf(fmaf(rest0[k], 0.03125f, m0[k]), 0.03125f, acc0[k]), o1 = fmaf(fmaf(rest1[k], 0.03125f, m1[k]), 0.03125f, acc1[k]);
+            const float4 of = load_shared16f(smem_u32(&sm.result[warp & 3][r]));
+            const float o0 = fmaf(fmaf(rest0[k], 0.03125f, m0[k]), 0.03125f, acc0[k]), o1 = fmaf(fmaf(rest1[k], 0.03125f, m1[k]), 0.03125f, acc1[k]);
             float value = has0 ? o0 * of.x : 0.0f;                         // (a group without tiles has left nothing there)
             if (has1) value = fmaf(o1, of.y, value);
             if (marked && ((sm.nan_value[buf][0][r][own >> 5] | sm.nan_value[buf][1][r][own >> 5]) >> (own & 31)) & 1) value = NAN;
-            if (((nowhere >> r) & 1) || d < 0 || d >= kDim) continue;
-            const int64_t at = static_cast<int64_t>(static_cast<uint32_t>(__float_as_int(of.z)) | static_cast<uint64_t>(static_cast<uint32_t>(__float_as_int(of.w))) << 32) + d;
-            if ((partial >> r) & 1) a.partials[at] = value;
-            else static_cast<T*>(a.out)[at] = Elem<T>::from_float(value);
+            const uint64_t at = static_cast<uint64_t>(__float_as_uint(of.z)) | static_cast<uint64_t>(__float_as_uint(of.w)) << 32;
+            if ((partial >> r) & 1) reinterpret_cast<float*>(at)[d] = value;
+            else if (!((nowhere >> r) & 1)) reinterpret_cast<T*>(at)[d] = Elem<T>::from_float(value);
           }
         }
         tcgen05_before_sync();
@@ -929,7 +933,10 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           if (folds) sm.l[buf][group][warp & 3][folded_row] = failed ? NAN : total;
           if (own == 0) {
 #pragma unroll
-            for (int r = 0; r < kMine; ++r) sm.ref[buf][group][row0 + r] = (fresh >> r) & 1 ? -INFINITY : ref[r];
+            for (int r = 0; r < kMine; ++r)
+              if ((fresh >> r) & 1) ref[r] = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < kMine; r += 4) *reinterpret_cast<float4*>(&sm.ref[buf][group][row0 + r]) = make_float4(ref[r], ref[r + 1], ref[r + 2], ref[r + 3]);
           }
         }
         __syncwarp();
