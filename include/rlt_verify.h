@@ -800,7 +800,7 @@ RLT_API int rlt_return_pages(const int32_t* lengths, int requests, const int32_t
  *
  * rlt_quantized_attention: out[r, h] = sum_t softmax_t(scale * q[r, h] . K[t, h / g]) V[t, h / g], row i of the n_s of a sequence over
  * t < lengths[s] - n_s + i + 1, with window > 0 the last `window` of those; a row that sees no key gives zeros, rows behind
- * cu_rows[sequences] are left alone.  A length beyond table_width * block_size (at most 2^26) is cut to it; a page outside the cache reads as zeros.  q, out:
+ * cu_rows[sequences] are left alone, and out shares no memory with q.  A length beyond table_width * block_size (at most 2^26) is cut to it; a page outside the cache reads as zeros.  q, out:
  * [rows][q_heads][head_dim] with row strides.  max_new: the longest portion.  It, the numbers of rows and sequences and the shape choose the
  * kernels; among calls that they choose the same ones for, a row's bits depend on its own query, keys and values only.  bf16 portions of
  * more than 16 rows, long enough on average, are scored over an expansion of the pages in the workspace.  workspace:

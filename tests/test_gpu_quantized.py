@@ -285,6 +285,29 @@ def test_attention_matches_the_plain_form(dtype, heads, kv_heads, dim, block, le
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads, kv_heads, dim, block", [(2, 1, 128, 16), (2, 2, 64, 32), (2, 2, 40, 8)])
+def test_parts_of_long_contexts(dtype, heads, kv_heads, dim, block):
+    check_attention(heads, kv_heads, dim, block, [4096, 4097, 6144, 6145, 9000], [1, 2, 1, 1, 3], dtype)
+    check_attention(heads, kv_heads, dim, block, [4096, 6150, 8200], [2, 1, 3], dtype, window=4100)
+
+
+@pytest.mark.parametrize("dim, kv_heads, counts", [(128, 32, 1), (64, 5, 3)])
+def test_many_sequences(dim, kv_heads, counts):
+    """More sequences than are laid out at a time, with more items for a CTA than it looks up at a time."""
+    g = torch.Generator().manual_seed(dim)
+    lengths = torch.randint(0, 60, (300,), generator=g).tolist()
+    check_attention(kv_heads, kv_heads, dim, 16, lengths, torch.randint(0, counts + 1, (300,), generator=g).tolist(), torch.bfloat16)
+    lengths[290] = 1500
+    check_attention(kv_heads, kv_heads, dim, 16, lengths, [min(i % 7, 1) for i in range(300)], torch.float16, window=33)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_tables_for_the_longest_contexts(dtype):
+    """A row of a table of 2^26 tokens can have 32770 parts: three rows' partials fit in the workspace, and the rows are done in turns."""
+    check_attention(32, 8, 128, 16, [3000, 40, 2500], [5, 1, 2], dtype, width=1 << 22)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim, block", [(128, 16), (64, 32), (48, 5)])
 @pytest.mark.parametrize("window", [1, 2, 15, 16, 17, 40, 1000, 1024, 1025, 5000])
 def test_windows(dtype, dim, block, window):
@@ -396,6 +419,7 @@ LONG = [
     (16, 1, 64, 16, [1000], [1000], dict(strided=True)),
     (32, 16, 128, 48, [200, 31], [128, 64], dict(scale=0.3, spare=0)),            # rows at negative positions
     (32, 8, 128, 16, [64, 17], [64, 64], dict(width=100)),
+    (24, 3, 64, 16, [100, 70, 65, 200], [64, 70, 65, 64], {}),                    # an odd number of 64-wide heads
 ]
 
 
@@ -463,6 +487,30 @@ def test_long_portions_that_an_expansion_cannot_hold(dim):
     assert bool(((got.cpu().double() - want).abs() <= tol).all())
 
 
+def test_long_portions_from_a_graph():
+    """A captured call over expanded pages, replayed with other lengths, rows and codes, one of them a value that is NaN."""
+    heads, kv_heads, dim, block = 32, 4, 128, 16
+    call, _, _, _ = attention_case(heads, kv_heads, dim, block, [300, 200], [130, 130], torch.bfloat16, spare=0, width=30)
+    q, cache, tables, lengths, cu, most = call
+    assert is_expanded(call, {})
+    rlt.quantized_attention(*call)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = rlt.quantized_attention(*call)
+    codes = cache.value.view(torch.uint8)
+    for step in range(3):
+        if step == 1:
+            lengths.copy_(plain.words([140, 190]).cuda())
+            cu.copy_(plain.words([0, 135, 260]).cuda())
+            q.neg_()
+        if step == 2:
+            codes[int(tables[1, 3]), 5, 1, 7] = 0x7f                # token 53 of the second
+        graph.replay()
+        assert torch.equal(out.nan_to_num(9.0), rlt.quantized_attention(*call).nan_to_num(9.0)), step
+        assert bool(out.isnan().any()) == (step == 2)
+
+
 def test_rows_of_extreme_size():
     """Queries near the largest and smallest numbers of their type, beside ordinary ones."""
     for dtype, sizes in ((torch.bfloat16, [1e30, 1e-30, 0.0, 1.0]), (torch.float16, [60000.0, 1e-6, 0.0, 1.0]), (torch.float32, [1e30, 1e-38, 0.0, 1.0])):
@@ -494,8 +542,9 @@ def test_empty_calls():
     assert (out == 5.0).all()
     with pytest.raises(ValueError, match="page"):
         rlt.quantized_attention(q, cache, tables[:, :0].contiguous(), lengths, cu, 1)
-    with pytest.raises(ValueError, match="out must"):
-        rlt.quantized_attention(q, cache, tables, lengths, cu, 1, out=out.float())
+    for other in (out.float(), q):
+        with pytest.raises(ValueError, match="out must"):
+            rlt.quantized_attention(q, cache, tables, lengths, cu, 1, out=other)
     with pytest.raises(ValueError, match="CUDA"):
         rlt.quantized_attention(q, cache, tables.cpu(), lengths, cu, 1)
 

@@ -139,7 +139,8 @@ def test_the_c_entries_refuse_without_a_launch():
         assert bytes_of(**given) == 4 * given["rows"] * given["heads"] * 10 * (given.get("dim", 64) + 4), short
     assert bytes_of(**long, window=5) == 4 * 256 * 32 * 2 * (64 + 4)
     wide = dict(long, width=1 << 22, heads=64, kv=1, dim=128)         # 2^26 tokens are not expanded
-    assert bytes_of(**wide) == 4 * 256 * 64 * (4 + (1 << 15) - 2) * 132
+    a_row = 4 * 64 * (4 + (1 << 15) - 2) * 132
+    assert bytes_of(**wide) == (2 << 30) // a_row * a_row             # rows whose parts fit in 2 GB are done at a time
     assert attend(width=1000, nbytes=need - 1) == _capi.ERR_WORKSPACE
     assert attend(width=1000, nbytes=need, ws=p + 4) == _capi.ERR_WORKSPACE
     assert attend(width=1000, nbytes=need, ws=null) == _capi.ERR_WORKSPACE

@@ -27,12 +27,12 @@ quantized_rows_kernel(QuantizedAttentionArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int part = static_cast<int>(blockIdx.x % a.parts);
   const int64_t pair = blockIdx.x / a.parts;
-  const int row = static_cast<int>(pair / a.q_heads), head = static_cast<int>(pair % a.q_heads), kv_head = head / (a.q_heads / c.kv_heads);
+  const int row = a.step.row0 + static_cast<int>(pair / a.q_heads), head = static_cast<int>(pair % a.q_heads), kv_head = head / (a.q_heads / c.kv_heads);
   const int s = sequence_at(a.step.cu, a.step.sequences, row);
-  int first, count, low, keys;
-  rows_of(a.step, s, &first, &count);
+  int first, count, length, low, keys;
+  rows_of(a.step, s, &first, &count, &length);
   if (row < first || row >= first + count) return;                    // in no sequence: left as it was
-  keys_of(a.step, c.block, a.window, s, first, count, row, &low, &keys);
+  keys_of(a.step, c.block, a.window, length, first, count, row, &low, &keys);
   const int first_part = part_of(low), last_part = keys > 0 ? part_of(keys - 1) : first_part;
   if (first_part + part > last_part) return;
   const int begin = max(low, part_begin(first_part + part)), end = min(keys, part_begin(first_part + part + 1));
@@ -118,13 +118,13 @@ quantized_merge_kernel(QuantizedAttentionArgs a) {
   const QuantizedCache& c = a.cache;
   const int lane = threadIdx.x & 31;
   const int64_t pair = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  if (pair >= static_cast<int64_t>(a.step.rows) * a.q_heads) return;
-  const int row = static_cast<int>(pair / a.q_heads);
+  if (pair >= static_cast<int64_t>(a.step.rows - a.step.row0) * a.q_heads) return;
+  const int at = static_cast<int>(pair / a.q_heads), row = a.step.row0 + at;
   const int s = sequence_at(a.step.cu, a.step.sequences, row);
-  int first, count, low, keys;
-  rows_of(a.step, s, &first, &count);
+  int first, count, length, low, keys;
+  rows_of(a.step, s, &first, &count, &length);
   if (row < first || row >= first + count) return;
-  keys_of(a.step, c.block, a.window, s, first, count, row, &low, &keys);
+  keys_of(a.step, c.block, a.window, length, first, count, row, &low, &keys);
   const int parts = keys > 0 ? part_of(keys - 1) - part_of(low) + 1 : 1;
   if (parts < 2) return;
   const int stride = partial_stride(c.dim), quads = (stride - 4) / 4;
@@ -165,7 +165,7 @@ quantized_merge_kernel(QuantizedAttentionArgs a) {
       }
     }
   }
-  T* out = static_cast<T*>(a.out) + row * a.out_stride + (pair - static_cast<int64_t>(row) * a.q_heads) * c.dim;
+  T* out = static_cast<T*>(a.out) + row * a.out_stride + (pair - static_cast<int64_t>(at) * a.q_heads) * c.dim;
   const float inverse = 1.0f / total;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -179,7 +179,7 @@ quantized_merge_kernel(QuantizedAttentionArgs a) {
 
 template <typename T>
 int launch_rows(const QuantizedAttentionArgs& a, cudaStream_t stream) {
-  const int64_t pairs = static_cast<int64_t>(a.step.rows) * a.q_heads;
+  const int64_t pairs = static_cast<int64_t>(a.step.rows - a.step.row0) * a.q_heads;
   if (pairs * a.parts > 0x7fffffffll) {
     set_last_error_text("quantized_attention: too many rows, heads and parts of a context for one launch");
     return RLT_ERR_UNSUPPORTED;
@@ -193,7 +193,7 @@ int launch_rows(const QuantizedAttentionArgs& a, cudaStream_t stream) {
 
 template <typename T>
 int launch_merge(const QuantizedAttentionArgs& a, cudaStream_t stream) {
-  const int64_t pairs = static_cast<int64_t>(a.step.rows) * a.q_heads;
+  const int64_t pairs = static_cast<int64_t>(a.step.rows - a.step.row0) * a.q_heads;
   return launch_dependent("quantized_merge_kernel", quantized_merge_kernel<T>, dim3(static_cast<unsigned>((pairs + kWarps - 1) / kWarps)), dim3(kWarps * 32), 0,
                           stream, a);
 }
@@ -234,7 +234,7 @@ quantized_expand_kernel(QuantizedCache c, PackedRows step, Expanded x) {
     // bounds inside the rows that never fall, whatever stands in cu: the prompt kernel's list of tiles has room for those
     __shared__ int s_most[8];
     int most = 0;
-    for (int i = threadIdx.x; i <= s; i += 256) most = max(most, min(step.cu[i], step.rows));
+    for (int i = threadIdx.x; i <= s; i += 256) most = max(most, min(step.cu[i], step.total));
     most = static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<unsigned>(max(most, 0))));
     if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = most;
     __syncthreads();
@@ -242,7 +242,7 @@ quantized_expand_kernel(QuantizedCache c, PackedRows step, Expanded x) {
       for (int i = 1; i < 8; ++i) most = max(most, s_most[i]);
       x.cu[s] = most;
       x.lengths[s] = tokens;
-      if (s == step.sequences - 1) x.cu[s + 1] = max(most, min(step.cu[s + 1], step.rows));
+      if (s == step.sequences - 1) x.cu[s + 1] = max(most, min(step.cu[s + 1], step.total));
     }
   }
   const int row = c.kv_heads * c.dim, per_row = row / 16;
@@ -278,6 +278,14 @@ quantized_expand_kernel(QuantizedCache c, PackedRows step, Expanded x) {
     }
   }
   if (__syncthreads_or(marks) && threadIdx.x == 0) x.marked[s] = x.marked[step.sequences] = 1;
+}
+
+// Rows whose partials are written and joined at a time: tables are as wide as the longest context may become, so their room goes by that.
+constexpr size_t kMostPartials = size_t{2} << 30;
+size_t partial_bytes(int q_heads, int parts, int dim) { return parts < 2 ? 0 : sizeof(float) * static_cast<size_t>(q_heads) * parts * partial_stride(dim); }
+int rows_at_a_time(int rows, int q_heads, int parts, int dim) {
+  const size_t each = partial_bytes(q_heads, parts, dim), fit = each == 0 ? static_cast<size_t>(rows) : (kMostPartials > each ? kMostPartials / each : 1);
+  return static_cast<size_t>(rows) < fit ? rows : static_cast<int>(fit);
 }
 
 constexpr size_t kMostExpanded = size_t{4} << 30;      // bytes of expanded pages: tables are as wide as the longest context may become
@@ -325,7 +333,7 @@ int launch_expanded(const QuantizedAttentionArgs& a, const Expansion& e, unsigne
   p.q = a.q; p.out = a.out; p.key_cache = x.key; p.value_cache = x.value;
   p.token_stride = static_cast<int64_t>(c.kv_heads) * c.dim; p.block_stride = 16 * p.token_stride; p.num_blocks = static_cast<int64_t>(a.step.sequences) * e.width16;
   p.block_size = 16; p.q_heads = a.q_heads; p.kv_heads = c.kv_heads; p.head_dim = c.dim; p.dtype = a.dtype; p.block_tables = x.tables;
-  p.table_rows = a.step.sequences; p.table_width = e.width16; p.context_lengths = x.lengths; p.cu_seqlens_q = x.cu; p.rows = a.step.rows;
+  p.table_rows = a.step.sequences; p.table_width = e.width16; p.context_lengths = x.lengths; p.cu_seqlens_q = x.cu; p.rows = a.step.total;
   p.value_dim = c.dim; p.v_block_stride = p.block_stride; p.v_token_stride = p.token_stride; p.q_stride = a.q_stride; p.out_stride = a.out_stride;
   p.terms.scale = a.scale;
   if (!(a.scale > 0.0f) || !prefill_sm100_supported(p)) return RLT_OK;      // (there a scale of 0 means the usual one, and the largest score is taken before it)
@@ -349,7 +357,7 @@ int read_args(QuantizedAttentionArgs& a, const void* key_cache, const void* valu
   c.block_stride = block_stride; c.token_stride = token_stride; c.scale_stride = scale_stride; c.num_pages = num_blocks; c.block = block_size;
   c.kv_heads = kv_heads; c.dim = head_dim;
   a.dtype = dtype;
-  a.step.tables = block_tables; a.step.lengths = lengths; a.step.cu = cu_rows; a.step.sequences = sequences; a.step.width = table_width; a.step.rows = rows;
+  a.step.tables = block_tables; a.step.lengths = lengths; a.step.cu = cu_rows; a.step.sequences = sequences; a.step.width = table_width; a.step.total = a.step.rows = rows; a.step.row0 = 0;
   RLT_REQUIRE(dtype_valid(dtype), "quantized_attention: dtype must be float32, float16 or bfloat16");
   RLT_REQUIRE(quantized_cache_valid(c), "quantized_attention: cache must be [pages, block, kv_heads, dim <= 256] with a contiguous [kv_heads, dim] tail");
   RLT_REQUIRE(sequences >= 0 && rows >= 0 && table_width >= 0, "quantized_attention: invalid shape");
@@ -367,7 +375,7 @@ extern "C" RLT_API size_t rlt_quantized_attention_workspace_bytes(int rows, int 
   if (rows <= 0 || sequences <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || block_size <= 0 || table_width <= 0) return 0;
   const int parts = parts_of(static_cast<int64_t>(table_width) * block_size, window);
   const Expansion e = expansion_of(rows, sequences, max_new, q_heads, kv_heads, head_dim, block_size, table_width, window, dtype);
-  return e.partials + (parts < 2 ? 0 : sizeof(float) * static_cast<size_t>(rows) * q_heads * parts * partial_stride(head_dim));
+  return e.partials + static_cast<size_t>(rows_at_a_time(rows, q_heads, parts, head_dim)) * partial_bytes(q_heads, parts, head_dim);
 }
 
 extern "C" RLT_API int rlt_quantized_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const void* key_cache,
@@ -406,8 +414,15 @@ extern "C" RLT_API int rlt_quantized_attention(const void* q, int64_t q_stride, 
     if (status != RLT_OK) return status;
     if (scored) a.step.only = reinterpret_cast<const int32_t*>(static_cast<unsigned char*>(workspace) + e.marked);
   }
-  status = quantized_tiles_supported(a) ? launch_quantized_tiles(a, max_new, s) : RLT_ERR_UNSUPPORTED;
-  if (status == RLT_ERR_UNSUPPORTED) RLT_DISPATCH_DTYPE(dtype, T, status = launch_rows<T>(a, s));
-  if (status != RLT_OK || a.parts < 2) return status;
-  RLT_DISPATCH_DTYPE(dtype, T, return launch_merge<T>(a, s));
+  const bool tiles = quantized_tiles_supported(a);
+  const int each = rows_at_a_time(rows, q_heads, a.parts, head_dim);
+  for (int64_t row = 0; row < rows; row += each) {
+    a.step.row0 = static_cast<int>(row);
+    a.step.rows = static_cast<int>(rows - row < each ? rows : row + each);
+    status = tiles ? launch_quantized_tiles(a, max_new, s) : RLT_ERR_UNSUPPORTED;
+    if (status == RLT_ERR_UNSUPPORTED) RLT_DISPATCH_DTYPE(dtype, T, status = launch_rows<T>(a, s));
+    if (status == RLT_OK && a.parts > 1) RLT_DISPATCH_DTYPE(dtype, T, status = launch_merge<T>(a, s));
+    if (status != RLT_OK) return status;
+  }
+  return RLT_OK;
 }

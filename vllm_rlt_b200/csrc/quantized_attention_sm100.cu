@@ -17,12 +17,18 @@
 // that the largest is 2^kFresh.  Rounding p to three parts leaves 2^-12 of it, and below 2^-20 nothing: 2^-26 of a row's largest weight.
 // Scores, R, l and O are fp32.
 //
-// Roles.  Two groups of eight warps take tiles of 128 tokens in turn, each with scores, weights, references and sums of its own; one warp issues
-// S^T products, one O^T products, one the copies (a ring of tiles that runs on across items; keys give their place back before their values),
-// two prepare the queries of the next items.  Which group a tile belongs to goes by its
-// position, so a row's bits do not depend on the batch or on the other rows of its item.  Four warps write the results; three items are under way.
+// Roles.  Two groups of four or eight warps take tiles of 128 tokens in turn, each with scores, weights, references and sums of its own; one warp
+// issues S^T products, one O^T products, four or eight the copies (a ring of tiles that runs on across items; keys give their place back before
+// their values), two prepare the queries of the next items, four write the results; three items are under way.  Which group a tile belongs to
+// goes by its position, so a row's bits do not depend on the batch or on the other rows of its item.
 //
-// Bound by the bytes of keys and values.
+// What bounds it.  The bytes of keys and values would take 1440 cycles a tile (32 KB) of an SM; with sixteen rows an item the warps issue about 4700
+// instructions for one (half of them the softmax's, a quarter what an item costs at its ends), at 2.4 a cycle.  Measured, heads of 128, bf16:
+//   64 requests, 16 rows of 16 heads each, contexts of 512 to 4096        156 us, 4.0 TB/s of keys and values
+//   128 requests, a row of 32 heads over 8, contexts of 100 to 2048        68 us, 4.4 TB/s (items of four rows: the chain of a tile's waits)
+//   4 requests, 5 rows of 32 heads over 8, contexts of 65000 to 131072    263 us, 3.1 TB/s (20 rows are two items: every tile is scored twice)
+// The same with half as many copy warps, items found by every warp for itself and weights stored byte by byte: 189, 78 and 315 us.  With the
+// codes converted to half precision and multiplied by the warps (mma.sync): 342, 176 and 642 us.
 #include <cuda.h>
 
 #include "quantized_kv.cuh"
@@ -353,9 +359,9 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     block_sync();              // the batch before is done with
 #pragma unroll 1
     for (int i = threadIdx.x; i < sequences; i += kThreads) {
-      int first, count;
-      rows_of(a.step, batch + i, &first, &count);
-      const int64_t base = static_cast<int64_t>(a.step.lengths[batch + i]) - count + 1;
+      int first, count, length;
+      rows_of(a.step, batch + i, &first, &count, &length);
+      const int64_t base = static_cast<int64_t>(length) - count + 1;
       sm.work.first[i] = first;
       sm.work.count[i] = count;
       sm.work.base[i] = static_cast<int>(base < -0x20000000 ? -0x20000000 : (base > 0x20000000 ? 0x20000000 : base));
@@ -646,7 +652,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           int kind = kNowhere;
           if (my_live && x.part >= first_part && x.part <= last_part) kind = first_part < last_part ? kPartial : (sees > low ? kOutput : kZero);
           sm.kind[buf][lane] = kind;
-          sm.to[buf][lane] = kind == kPartial ? ((at_row * a.q_heads + head) * a.parts + x.part - first_part) * partial_stride(kDim) : at_row * a.out_stride + head * kDim;
+          sm.to[buf][lane] = kind == kPartial ? (((at_row - a.step.row0) * a.q_heads + head) * a.parts + x.part - first_part) * partial_stride(kDim) : at_row * a.out_stride + head * kDim;
         }
         fence_async_proxy();
         __syncwarp();
@@ -1000,8 +1006,8 @@ bool quantized_tiles_supported(const QuantizedAttentionArgs& a) {
   if (a.dtype == RLT_F32 || (c.dim != 64 && c.dim != 128) || c.block % 16 != 0 || c.num_pages < 1 || c.num_pages > 0x7fffffff) return false;
   if (c.token_stride % 16 != 0 || c.block_stride % 16 != 0 || !aligned16(c.key) || !aligned16(c.value)) return false;
   if (a.q_stride % 4 != 0 || (reinterpret_cast<uintptr_t>(a.q) & 7u) != 0) return false;
-  const int64_t group = a.q_heads / c.kv_heads, tiles = (static_cast<int64_t>(a.step.rows) * group + 3) / 4 + a.step.sequences;
-  return tiles * c.kv_heads * a.parts <= 0x7fffffff && static_cast<int64_t>(a.step.rows) * group <= 0x7fffffff;     // items are counted in 32 bits
+  const int64_t group = a.q_heads / c.kv_heads, tiles = (static_cast<int64_t>(a.step.total) * group + 3) / 4 + a.step.sequences;
+  return tiles * c.kv_heads * a.parts <= 0x7fffffff && static_cast<int64_t>(a.step.total) * group < (1 << 26);     // items are counted in 32 bits
 }
 
 int launch_quantized_tiles(const QuantizedAttentionArgs& a, int max_new, cudaStream_t stream) {

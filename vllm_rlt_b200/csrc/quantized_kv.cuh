@@ -45,7 +45,8 @@ struct PackedRows {
   const int32_t* cu;            // [sequences + 1]
   int sequences;
   int width;
-  int rows;
+  int total;                    // rows of the step
+  int row0, rows;               // of which a launch does rows row0 .. rows - 1
   const int32_t* only = nullptr;        // [sequences + 1]: where 0 the sequence has no rows, the last one 0: none has; nullptr: all have theirs
 };
 
@@ -74,11 +75,13 @@ inline int parts_of(int64_t capacity, int window) {
   return static_cast<int>(seen < all ? seen : all);
 }
 
-// The rows of sequence s, kept inside the step's.
-__device__ __forceinline__ void rows_of(const PackedRows& p, int s, int* first, int* count) {
-  const int begin = min(max(p.cu[s], 0), p.rows), end = min(max(p.cu[s + 1], begin), p.rows);
-  *first = begin;
-  *count = p.only == nullptr || p.only[s] != 0 ? end - begin : 0;
+// The rows of sequence s that a launch does, kept inside the step's, and the sequence's length with the last of them.
+__device__ __forceinline__ void rows_of(const PackedRows& p, int s, int* first, int* count, int* length) {
+  const int begin = min(max(p.cu[s], 0), p.total), end = min(max(p.cu[s + 1], begin), p.total), last = min(end, p.rows);
+  *first = max(begin, p.row0);
+  *count = p.only == nullptr || p.only[s] != 0 ? max(last - *first, 0) : 0;
+  const int64_t tokens = static_cast<int64_t>(p.lengths[s]) - (end - last);
+  *length = static_cast<int>(tokens < -0x7fffffff ? -0x7fffffff : tokens);
 }
 
 // The sequence of a row: the last one that starts at or before it (a row behind the last sequence is in none of them).
@@ -95,8 +98,8 @@ __device__ __forceinline__ int sequence_at(const int32_t* cu, int sequences, int
 __device__ __forceinline__ int table_tokens(const PackedRows& p, int block) { return p.width * block; }
 
 // Keys that a row sees: positions low .. keys - 1.  A length that its table cannot address is cut to what it can.
-__device__ __forceinline__ void keys_of(const PackedRows& p, int block, int window, int s, int first, int count, int row, int* low, int* keys) {
-  const int64_t seen = static_cast<int64_t>(p.lengths[s]) - count + (row - first) + 1;
+__device__ __forceinline__ void keys_of(const PackedRows& p, int block, int window, int length, int first, int count, int row, int* low, int* keys) {
+  const int64_t seen = static_cast<int64_t>(length) - count + (row - first) + 1;
   *keys = static_cast<int>(seen < 0 ? 0 : (seen < table_tokens(p, block) ? seen : table_tokens(p, block)));
   *low = window > 0 ? max(*keys - window, 0) : 0;
 }

@@ -125,9 +125,9 @@ quantized_write_kernel(QuantizedCache c, PackedRows step, const T* __restrict__ 
   const int row = blockIdx.x * kWindow + threadIdx.x;
   if (threadIdx.x < kWindow && row < step.rows) {
     const int s = sequence_at(staged ? s_cu : step.cu, step.sequences, row);
-    int first, count;
-    rows_of(step, s, &first, &count);
-    const int64_t position = static_cast<int64_t>(step.lengths[s]) - count + (row - first);
+    int first, count, length;
+    rows_of(step, s, &first, &count, &length);
+    const int64_t position = static_cast<int64_t>(length) - count + (row - first);
     if (row >= first && row < first + count && position >= 0 && position < table_tokens(step, c.block)) {
       const int entry = static_cast<int>(position) / c.block, offset = static_cast<int>(position) - entry * c.block;
       if (row == first || offset == 0) {
@@ -258,7 +258,8 @@ extern "C" RLT_API int rlt_quantized_kv_write(void* key_cache, void* value_cache
   const int64_t row = static_cast<int64_t>(kv_heads) * head_dim;
   RLT_REQUIRE(k_stride >= row && v_stride >= row, "quantized_kv_write: rows must be [rows, kv_heads, head_dim] with a contiguous tail");
   PackedRows step;
-  step.tables = block_tables; step.lengths = lengths; step.cu = cu_rows; step.sequences = sequences; step.width = table_width; step.rows = rows;
+  step.tables = block_tables; step.lengths = lengths; step.cu = cu_rows; step.sequences = sequences; step.width = table_width;
+  step.total = step.rows = rows; step.row0 = 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   RLT_DISPATCH_DTYPE(dtype, T, return launch<T>(c, step, k, k_stride, v, v_stride, s));
 }

@@ -215,9 +215,10 @@ def quantized_attention(q, cache: QuantizedKV, tables, lengths, cu, max_new: int
 
     Row i of the n_s rows of sequence s sees lengths[s] - n_s + i + 1 keys, with `window` the last so many of them; a row that sees none gives
     zeros, a length that its table cannot address is cut to what it can, and rows behind the last sequence are left as they are in `out`
-    (undefined where `out` is not given).  scale: 1 / sqrt(dim) unless given.  max_new: the longest portion of the step, which decides on the
-    kernels; results do not depend on the other sequences of a call.  Heads are whole groups over the cache's.  Slots that no token was
-    stored in may hold anything."""
+    (undefined where `out` is not given; it may not share memory with q).  scale: 1 / sqrt(dim) unless given.  max_new: the longest portion of
+    the step.  It, the shapes and the numbers of rows and sequences decide on the kernels: up to 16 rows, a row's bits are its own, whatever
+    else is in the call; long portions in bfloat16 (64 rows and more on average) are scored over an expansion of their pages, with weights
+    rounded to bfloat16.  Heads are whole groups over the cache's.  Slots that no token was stored in may hold anything."""
     cache.check()
     _check_step(tables, lengths, cu)
     pages, block, kv_heads, dim = cache.key.shape
@@ -228,8 +229,8 @@ def quantized_attention(q, cache: QuantizedKV, tables, lengths, cu, max_new: int
     index = _device_of(q, cache.key, cache.value, cache.key_scale, cache.value_scale, tables, lengths, cu)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != q.shape or out.dtype != q.dtype:
-        raise ValueError("out must have q's shape and dtype")
+    elif out.shape != q.shape or out.dtype != q.dtype or out.data_ptr() == q.data_ptr() != 0:
+        raise ValueError("out must have q's shape and dtype, and memory of its own")
     else:
         _device_of(q, out)
     rows, heads, _ = q.shape
