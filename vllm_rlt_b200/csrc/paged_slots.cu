@@ -9,8 +9,8 @@
 // second launch or a pass through global memory); the cluster's barrier then stands between the last read of the state and its first
 // write, so the state is updated in place without a copy.  Entries and rows are dealt to all threads of the cluster, which find their
 // request by a search in shared memory.  What bounds it is latency: two dependent reads, two block-wide barriers and one search.  The launch
-// for a full house (1024 requests, 1 to 37 rows each, 19514 rows) takes 9.9 us, giving the pages back 4.8; a step of 64 single rows and its way
-// back are under 8 us together, and a Python call of either is 19 us.
+// for a full house (1024 requests, 1 to 37 rows each, about 19500 rows) takes 9.3 us, giving the pages back 4.6; a step of 64 single rows 4.7 and
+// 3.3.  A Python call of either is 19 us.
 #include <cooperative_groups.h>
 
 #include "common.cuh"

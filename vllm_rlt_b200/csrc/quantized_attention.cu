@@ -16,7 +16,8 @@ constexpr float kToLog2 = 1.4426950408889634f;
 // ---- any shape: one CTA per (row, query head, part) ---------------------------------------------------
 // A lane scores a key of its own (32 at a time: five shuffles per 32 keys instead of per key), then the warp adds up the 32 values with its
 // lanes across the head.  kDims: elements of a head per lane.  In fp32 throughout: this is the kernel of 32-bit queries, and of head sizes,
-// page sizes and layouts that the tiles do not take.
+// page sizes and layouts that the tiles do not take.  Bound by its loads of single codes: 64 contexts of 512 to 4096 tokens, 16 rows of 16 heads
+// each, take 10 ms here and 0.15 ms in the tiles.
 template <typename T, int kDims>
 __global__ void __launch_bounds__(kWarps * 32)
 quantized_rows_kernel(QuantizedAttentionArgs a) {
@@ -109,7 +110,8 @@ quantized_rows_kernel(QuantizedAttentionArgs a) {
 
 // ---- joining parts -----------------------------------------------------------------------------------
 // out = sum_c O_c 2^(M_c - M) / sum_c l_c 2^(M_c - M), M the largest M_c.  One warp per (row, query head), parts in order; eight parts'
-// loads are in flight together.
+// loads are in flight together.  Bound by latency: a search, the bounds and length it gives, the parts.  With a binary search instead of 32
+// candidates at a time it took 6 us more behind 1024 rows of 64 sequences.
 template <typename T>
 __global__ void __launch_bounds__(kWarps * 32)
 quantized_merge_kernel(QuantizedAttentionArgs a) {
@@ -120,7 +122,14 @@ quantized_merge_kernel(QuantizedAttentionArgs a) {
   const int64_t pair = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
   if (pair >= static_cast<int64_t>(a.step.rows - a.step.row0) * a.q_heads) return;
   const int at = static_cast<int>(pair / a.q_heads), row = a.step.row0 + at;
-  const int s = sequence_at(a.step.cu, a.step.sequences, row);
+  // the row's sequence, 32 candidates at a time: what a warp waits for is dependent reads
+  int s = 0, past = a.step.sequences;
+  while (past - s > 1) {
+    const int step = (past - s + 31) / 32, at = s + lane * step;
+    const unsigned below = __ballot_sync(0xffffffffu, lane == 0 || (at < past && a.step.cu[at] <= row));
+    s += (31 - __clz(below)) * step;
+    past = min(s + step, past);
+  }
   int first, count, length, low, keys;
   rows_of(a.step, s, &first, &count, &length);
   if (row < first || row >= first + count) return;
@@ -206,7 +215,8 @@ int launch_merge(const QuantizedAttentionArgs& a, cudaStream_t stream) {
 // two (its values would be rounded), or with a length beyond its table (rows are cut one by one here) is marked, and scored behind it.
 //
 // A CTA takes pages of 16 tokens of one sequence: sequence s in pages s * width16 .. of `key` and `value`, and the tables, lengths and row
-// bounds that say so.  Bound by its traffic: a byte read, two written.
+// bounds that say so.  Bound by its traffic, a byte read and two written: 4 contexts of 5117 tokens, 8 heads of 128, 126 MB in 19.2 us (6.5 TB/s),
+// before 78 us of the prompt kernel for 1021 rows of 16 heads each; the tiles took 431 us for all of it.
 struct Expanded {
   __nv_bfloat16* key;
   __nv_bfloat16* value;
