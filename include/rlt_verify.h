@@ -772,7 +772,7 @@ RLT_API int rlt_step_metadata(int32_t* words, const int64_t* at, const int64_t* 
  * beyond table_width * block_size, held below zero or beyond table_width, free_count below zero or beyond free_capacity.
  * lengths, counts, new_lengths, held: int32 [requests], at most 8192.  tables: int32 [requests][table_width].  free_pages: int32
  * [free_capacity].  cu: int32 [requests + 1].  positions, row_seq: int32 [rows].  write_blocks, write_offsets: int64 [rows].  free_count,
- * active_rows, status: one int32.  held may be NULL (with free_pages and free_count): the tables are complete.
+ * active_rows, status: one int32.  held may be NULL (with free_pages and free_count): the tables are complete.  No two arguments share memory.
  *
  * rlt_return_pages: request s keeps the pages of its first lengths[s] tokens.  Page k of those given back goes to place
  * free_count + total - 1 - k, so that the call undoes the claims of the step before it.  status 1 and nothing changed where free_capacity
@@ -803,7 +803,7 @@ RLT_API int rlt_return_pages(const int32_t* lengths, int requests, const int32_t
  * cu_rows[sequences] are left alone, and out shares no memory with q.  A length beyond table_width * block_size (at most 2^26) is cut to it; a page outside the cache reads as zeros.  q, out:
  * [rows][q_heads][head_dim] with row strides.  max_new: the longest portion.  It, the numbers of rows and sequences and the shape choose the
  * kernels; among calls that they choose the same ones for, a row's bits depend on its own query, keys and values only.  bf16 portions of
- * more than 16 rows, long enough on average, are scored over an expansion of the pages in the workspace.  workspace:
+ * more than 16 rows, long enough on average and without a window, are scored over an expansion of the pages in the workspace.  workspace:
  * rlt_quantized_attention_workspace_bytes(...) bytes, 256-byte aligned, private to the call until its work on `stream` completes. */
 RLT_API int rlt_quantized_kv_write(void* key_cache, void* value_cache, float* key_scale, float* value_scale, int64_t block_stride,
                            int64_t token_stride, int64_t scale_stride, int64_t num_blocks, int block_size, int kv_heads, int head_dim,

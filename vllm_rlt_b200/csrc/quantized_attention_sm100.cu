@@ -24,9 +24,9 @@
 //
 // What bounds it.  The bytes of keys and values would take 1440 cycles a tile (32 KB) of an SM; with sixteen rows an item the warps issue about 4700
 // instructions for one (half of them the softmax's, a quarter what an item costs at its ends), at 2.4 a cycle.  Measured, heads of 128, bf16:
-//   64 requests, 16 rows of 16 heads each, contexts of 512 to 4096        151 us, 4.1 TB/s of keys and values
-//   128 requests, a row of 32 heads over 8, contexts of 100 to 2048        67 us, 4.5 TB/s (items of four rows: the chain of a tile's waits)
-//   4 requests, 5 rows of 32 heads over 8, contexts of 65000 to 131072    255 us, 3.2 TB/s (20 rows are two items: every tile is scored twice)
+//   64 requests, 16 rows of 16 heads each, contexts of 512 to 4096        156 us, 4.0 TB/s of keys and values
+//   128 requests, a row of 32 heads over 8, contexts of 100 to 2048        66 us, 4.5 TB/s (items of four rows: the chain of a tile's waits)
+//   4 requests, 5 rows of 32 heads over 8, contexts of 65000 to 131072    262 us, 3.2 TB/s (20 rows are two items: every tile is scored twice)
 // (a call's time with the joining of its parts, 5 to 10 us of it).  With items found by every warp for itself, four copy warps at all sizes and
 // weights stored byte by byte: 189, 78 and 315 us.  With the codes converted to half precision and multiplied by the warps (mma.sync): 342,
 // 176 and 642 us.
@@ -53,7 +53,8 @@ struct Roles {
   static constexpr int kControl = kCopyWarps + 8;
   static constexpr int kThreads = 32 * (kResult + 4);
   static constexpr int kLaunched = 65536 / kThreads / 8 * 8;                               // registers of a thread
-  static constexpr int kControlRegisters = 48;
+  // The softmax gets what the others leave of the launch's.  With 48 for them the copies and the results spilled: 1 to 2 % slower; with 40, 9 %.
+  static constexpr int kControlRegisters = kHalves == 2 ? 56 : 72;
   static constexpr int kSoftmaxRegisters = (kThreads * kLaunched - 32 * kControl * kControlRegisters) / (kGroups * kGroupThreads) / 8 * 8;
 };
 constexpr int kDeep = 3;                // items between their queries and their results
@@ -85,7 +86,7 @@ enum { kNowhere, kOutput, kZero, kPartial };
 // The work of a batch of sequences: cells (part, row tile) of whole parts in front of a sequence; then the last parts, largest first.
 struct Work {
   int whole_before[kBatch + 1], last_before[kBatch + 1], order[kBatch];
-  int whole[kBatch], last[kBatch];                    // a sequence's cells of whole parts; the tiles of its last part, then its row tiles
+  alignas(8) int2 size[kBatch];                       // a sequence's cells of whole parts; the tiles of its last part and, in the low 24 bits, its row tiles
   int first[kBatch], count[kBatch], base[kBatch];     // a sequence's rows, and the keys its first row sees (below 1: none)
 };
 
@@ -356,6 +357,8 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   // The items of sequences batch .., by all threads; their number.  Cells of whole parts come first, then every sequence's last part, those with the
   // most tiles first: dealt in this order, one CTA has about as many tiles as another.  The heads of a cell go to neighbouring CTAs at a time.
   auto lay_out = [&](int batch) {
+    static_assert(2 * (kBatch + 1) * sizeof(int) <= sizeof(sm.list), "the list is not in use meanwhile");
+    int *const places = reinterpret_cast<int*>(sm.list), *const last_sums = places + kBatch + 1;      // among the last parts, and the cells in front there
     sequences = min(a.step.sequences - batch, kBatch);
     block_sync();              // the batch before is done with
 #pragma unroll 1
@@ -368,30 +371,33 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       sm.work.base[i] = static_cast<int>(base < -0x20000000 ? -0x20000000 : (base > 0x20000000 ? 0x20000000 : base));
       const Spread x = spread_of(kEach, count, sm.work.base[i], group_heads, a.window, capacity);
       const int top = clamp_keys(sm.work.base[i] + count - 1, capacity);
-      sm.work.whole[i] = count > 0 ? (x.parts - 1) * x.tiles : 0;
-      sm.work.last[i] = (top > 0 ? (top - 1 - part_begin(part_of(top - 1))) / kTile + 1 : 0) << 24 | x.tiles;
+      sm.work.size[i] = make_int2(count > 0 ? (x.parts - 1) * x.tiles : 0, (top > 0 ? (top - 1 - part_begin(part_of(top - 1))) / kTile + 1 : 0) << 24 | x.tiles);
+    }
+#pragma unroll 1
+    for (int i = threadIdx.x; i <= sequences; i += kThreads) sm.work.whole_before[i] = places[i] = last_sums[i] = 0;
+    block_sync();
+    // A sequence's place, and what lies in front of it, by comparing it with all the others: a lane has a sequence, and the warps a share of the others
+    // each.  The sum of all stands behind the last.
+    const int blocks = sequences / 32 + 1, shares = kThreads / 32 / blocks, share = warp / blocks, i = warp % blocks * 32 + lane;
+    if (share < shares && i <= sequences) {
+      const int each = (sequences + shares - 1) / shares, mine = i < sequences ? sm.work.size[i].y >> 24 : -1;
+      int place = 0, whole_before = 0, last_sum = 0;
+#pragma unroll 4
+      for (int k = share * each; k < min((share + 1) * each, sequences); ++k) {
+        const int2 other = sm.work.size[k];
+        if (k < i) whole_before += other.x;
+        if (other.y >> 24 > mine || (other.y >> 24 == mine && k < i)) { ++place; last_sum += other.y & 0xffffff; }
+      }
+      atomicAdd(&sm.work.whole_before[i], whole_before);
+      atomicAdd(&places[i], place);
+      atomicAdd(&last_sums[i], last_sum);
     }
     block_sync();
-    // A sequence's place, and what lies in front of it, by comparing it with all the others (a warp's 32 at a time); the sum of all behind the last.
 #pragma unroll 1
-    for (int i = warp; i <= sequences; i += kThreads / 32) {
-      const int mine = i < sequences ? sm.work.last[i] >> 24 : -1;
-      int place = 0, whole_before = 0, last_before = 0;
-#pragma unroll 1
-      for (int k = lane; k < sequences; k += 32) {
-        const int last = sm.work.last[k];
-        const bool in_front = last >> 24 > mine || (last >> 24 == mine && k < i);
-        if (k < i) whole_before += sm.work.whole[k];
-        if (in_front) { ++place; last_before += last & 0xffffff; }
-      }
-      place = __reduce_add_sync(0xffffffffu, place);
-      whole_before = __reduce_add_sync(0xffffffffu, whole_before);
-      last_before = __reduce_add_sync(0xffffffffu, last_before);
-      if (lane == 0) {
-        sm.work.whole_before[i] = whole_before;
-        sm.work.last_before[place] = last_before;
-        if (i < sequences) sm.work.order[place] = i;
-      }
+    for (int k = threadIdx.x; k <= sequences; k += kThreads) {
+      const int place = places[k];
+      sm.work.last_before[place] = last_sums[k];
+      if (k < sequences) sm.work.order[place] = k;
     }
     block_sync();
     whole = sm.work.whole_before[sequences];
