@@ -289,6 +289,7 @@ def test_attention_matches_the_plain_form(dtype, heads, kv_heads, dim, block, le
 def test_parts_of_long_contexts(dtype, heads, kv_heads, dim, block):
     check_attention(heads, kv_heads, dim, block, [4096, 4097, 6144, 6145, 9000], [1, 2, 1, 1, 3], dtype)
     check_attention(heads, kv_heads, dim, block, [4096, 6150, 8200], [2, 1, 3], dtype, window=4100)
+    check_attention(heads, kv_heads, dim, block, [4096, 6150, 8200, 2000], [2, 1, 20, 17], dtype, window=1900)      # from any place in a tile, in one part
 
 
 @pytest.mark.parametrize("dim, kv_heads, counts", [(128, 32, 1), (64, 5, 3)])
@@ -309,7 +310,7 @@ def test_tables_for_the_longest_contexts(dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim, block", [(128, 16), (64, 32), (48, 5)])
-@pytest.mark.parametrize("window", [1, 2, 15, 16, 17, 40, 1000, 1024, 1025, 5000])
+@pytest.mark.parametrize("window", [1, 2, 15, 16, 17, 40, 1000, 1024, 1025, 1900, 1901, 5000])
 def test_windows(dtype, dim, block, window):
     check_attention(4, 2, dim, block, [1, 50, 1040, 2100], [1, 4, 17 if window > 100 else 2, 3], dtype, window=window)
 

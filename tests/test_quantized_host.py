@@ -128,8 +128,8 @@ def test_the_c_entries_refuse_without_a_launch():
 
     need = bytes_of()
     assert need == 4 * 10 * 4 * (64 + 4)                              # four parts of 1024 tokens and six of 2048
-    assert bytes_of(width=64) == bytes_of(window=1) == bytes_of(rows=0) == bytes_of(sequences=0) == 0
-    assert bytes_of(window=2) == 4 * 2 * 4 * (64 + 4)
+    assert bytes_of(width=64) == bytes_of(window=1) == bytes_of(window=1900) == bytes_of(rows=0) == bytes_of(sequences=0) == 0
+    assert bytes_of(window=1901) == 4 * 3 * 4 * (64 + 4)
     long = dict(rows=256, max_new=256, heads=32)
     parts = 256 * 32 * 10 * 4 * (64 + 4)
     assert bytes_of(**long) > 2 * 16000 * 2 * 64 * 2 + parts          # and 16000 expanded tokens
@@ -137,7 +137,7 @@ def test_the_c_entries_refuse_without_a_launch():
                   dict(heads=30), dict(heads=32, kv=32, rows=127)):
         given = dict(long, **short)
         assert bytes_of(**given) == 4 * given["rows"] * given["heads"] * 10 * (given.get("dim", 64) + 4), short
-    assert bytes_of(**long, window=5) == 4 * 256 * 32 * 2 * (64 + 4)
+    assert bytes_of(**long, window=5) == 0 and bytes_of(**long, window=3000) == 4 * 256 * 32 * 4 * (64 + 4)
     wide = dict(long, width=1 << 22, heads=64, kv=1, dim=128)         # 2^26 tokens are not expanded
     a_row = 4 * 64 * (4 + (1 << 15) - 2) * 132
     assert bytes_of(**wide) == (2 << 30) // a_row * a_row             # rows whose parts fit in 2 GB are done at a time

@@ -34,9 +34,9 @@ quantized_rows_kernel(QuantizedAttentionArgs a) {
   rows_of(a.step, s, &first, &count, &length);
   if (row < first || row >= first + count) return;                    // in no sequence: left as it was
   keys_of(a.step, c.block, a.window, length, first, count, row, &low, &keys);
-  const int first_part = part_of(low), last_part = keys > 0 ? part_of(keys - 1) : first_part;
+  const int first_part = part_of(low, a.window), last_part = keys > 0 ? part_of(keys - 1, a.window) : first_part;
   if (first_part + part > last_part) return;
-  const int begin = max(low, part_begin(first_part + part)), end = min(keys, part_begin(first_part + part + 1));
+  const int begin = max(low, part_begin(first_part + part, a.window)), end = min(keys, part_begin(first_part + part + 1, a.window));
 
   const T* q = static_cast<const T*>(a.q) + row * a.q_stride + static_cast<int64_t>(head) * c.dim;
   for (int d = threadIdx.x; d < kDims * 32; d += kWarps * 32) s_q[d] = d < c.dim ? Elem<T>::to_float(q[d]) * (a.scale * kToLog2) : 0.0f;
@@ -134,7 +134,7 @@ quantized_merge_kernel(QuantizedAttentionArgs a) {
   rows_of(a.step, s, &first, &count, &length);
   if (row < first || row >= first + count) return;
   keys_of(a.step, c.block, a.window, length, first, count, row, &low, &keys);
-  const int parts = keys > 0 ? part_of(keys - 1) - part_of(low) + 1 : 1;
+  const int parts = keys > 0 ? part_of(keys - 1, a.window) - part_of(low, a.window) + 1 : 1;
   if (parts < 2) return;
   const int stride = partial_stride(c.dim), quads = (stride - 4) / 4;
   const float* part = a.partials + pair * a.parts * stride;

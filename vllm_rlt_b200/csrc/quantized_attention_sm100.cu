@@ -22,7 +22,7 @@
 // their values), two prepare the queries of the next items, four write the results; three items are under way.  Which group a tile belongs to
 // goes by its position, so a row's bits do not depend on the batch or on the other rows of its item.
 //
-// What bounds it.  The bytes of keys and values would take 1440 cycles a tile (32 KB) of an SM; with sixteen rows an item the warps issue about 4700
+// What bounds it.  The bytes of keys and values would take 1440 cycles a tile (32 KB) of an SM; with sixteen rows an item the warps issue about 4800
 // instructions for one (half of them the softmax's, a quarter what an item costs at its ends), at 2.4 a cycle.  Measured, heads of 128, bf16:
 //   64 requests, 16 rows of 16 heads each, contexts of 512 to 4096        156 us, 4.0 TB/s of keys and values
 //   128 requests, a row of 32 heads over 8, contexts of 100 to 2048        66 us, 4.5 TB/s (items of four rows: the chain of a tile's waits)
@@ -64,6 +64,7 @@ static_assert(kPieces * 16 == kTile);
 constexpr int kSlots = 10;              // tiles of keys or of values in the ring, in turn
 constexpr int kScaleSlots = 8;          // tiles' scales; see the copies
 constexpr int kBatch = 256;             // sequences whose items are laid out at a time
+static_assert(kWholeWindow + 16 - 1 + kTile - 1 <= kLongPart, "the window of an item's rows, from the start of a tile, is a part at most");
 constexpr int kList = 48;               // items of this CTA that are looked up at a time
 constexpr float kHighest = 8.0f, kFresh = 6.0f;
 constexpr float kFaint = -100.0f;       // log2 of a weight whose product with 1 / scale_v may leave fp32
@@ -145,8 +146,8 @@ struct Spread {
 __device__ __forceinline__ Spread spread_of(int each, int count, int base, int group, int window, int capacity) {
   Spread x;
   const int top = clamp_keys(base + count - 1, capacity), low = window > 0 ? max(clamp_keys(base, capacity) - window, 0) : 0;
-  x.first_part = part_of(low);
-  x.parts = top > 0 ? part_of(top - 1) - x.first_part + 1 : 1;
+  x.first_part = part_of(low, window);
+  x.parts = top > 0 ? part_of(top - 1, window) - x.first_part + 1 : 1;
   x.tiles = (count * group + each - 1) / each;
   return x;
 }
@@ -186,8 +187,8 @@ __device__ __noinline__ Item find_item(const Work* work, int batch, int sequence
   x.pair0 = (cell < whole ? local - chunk * spread.tiles : local) * each;
   x.pairs = min(x.count * group - x.pair0, each);
   const int least = clamp_keys(x.base + x.pair0 / group, capacity), top = clamp_keys(x.base + (x.pair0 + x.pairs - 1) / group, capacity);
-  x.from = max(window > 0 ? max(least - window, 0) : 0, part_begin(x.part));
-  x.end = min(top, part_begin(x.part + 1));
+  x.from = max(window > 0 ? max(least - window, 0) : 0, part_begin(x.part, window));
+  x.end = min(top, part_begin(x.part + 1, window));
   x.all_from = max(window > 0 ? max(top - window, 0) : 0, x.from);
   x.all_end = min(least, x.end);
   x.begin = x.from / kTile * kTile;
@@ -370,8 +371,9 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       sm.work.count[i] = count;
       sm.work.base[i] = static_cast<int>(base < -0x20000000 ? -0x20000000 : (base > 0x20000000 ? 0x20000000 : base));
       const Spread x = spread_of(kEach, count, sm.work.base[i], group_heads, a.window, capacity);
-      const int top = clamp_keys(sm.work.base[i] + count - 1, capacity);
-      sm.work.size[i] = make_int2(count > 0 ? (x.parts - 1) * x.tiles : 0, (top > 0 ? (top - 1 - part_begin(part_of(top - 1))) / kTile + 1 : 0) << 24 | x.tiles);
+      const int top = clamp_keys(sm.work.base[i] + count - 1, capacity), low = a.window > 0 ? max(clamp_keys(sm.work.base[i], capacity) - a.window, 0) : 0;
+      const int last_tiles = top > 0 ? (top - 1 - max(part_begin(part_of(top - 1, a.window), a.window), low / kTile * kTile)) / kTile + 1 : 0;
+      sm.work.size[i] = make_int2(count > 0 ? (x.parts - 1) * x.tiles : 0, min(last_tiles, 127) << 24 | x.tiles);
     }
 #pragma unroll 1
     for (int i = threadIdx.x; i <= sequences; i += kThreads) sm.work.whole_before[i] = places[i] = last_sums[i] = 0;
@@ -653,7 +655,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         }
         if (first_row == 0 && lane < kRows) {
           const int sees = clamp_keys(x.base + my_row, capacity), low = a.window > 0 ? max(sees - a.window, 0) : 0;
-          const int first_part = part_of(low), last_part = sees > 0 ? part_of(sees - 1) : first_part;
+          const int first_part = part_of(low, a.window), last_part = sees > 0 ? part_of(sees - 1, a.window) : first_part;
           sm.keys[buf][lane] = my_live ? min(sees, x.end) : x.end;          // of the part; rows that are none see all of it, and nothing is masked for them
           sm.low[buf][lane] = my_live ? max(low, x.from) : x.from;
           int kind = kNowhere;

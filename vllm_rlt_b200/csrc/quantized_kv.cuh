@@ -17,10 +17,16 @@ constexpr float kLargestCode = 448.0f;
 // A context is split at fixed positions, whatever the batch: a row's bits are its own.  1024 tokens at first, so that a few ordinary contexts make
 // enough parts for all SMs; 2048 from 4096 on, where a part's costs (references found anew, its sums written and joined) weigh more.
 constexpr int kShortPart = 1024, kShortParts = 4, kLongPart = 2048;
-__host__ __device__ __forceinline__ int part_of(int token) {
+// A window of up to kWholeWindow keys is one part wherever it lies: its rows need no joining, and an item's ends are paid once for it.  Split / whole,
+// us: 96 requests of three rows, 1000 keys, 64-wide heads 75.6 / 61.7; 16 of one row, 1000 keys, 8 heads of 128 21 / 15; one request, 1800 keys 16.5 / 16.7.
+constexpr int kWholeWindow = 1900;
+__host__ __device__ __forceinline__ bool whole_window(int window) { return window > 0 && window <= kWholeWindow; }
+__host__ __device__ __forceinline__ int part_of(int token, int window) {
+  if (whole_window(window)) return 0;
   return token < kShortParts * kShortPart ? token / kShortPart : kShortParts + (token - kShortParts * kShortPart) / kLongPart;
 }
-__host__ __device__ __forceinline__ int part_begin(int part) {
+__host__ __device__ __forceinline__ int part_begin(int part, int window) {
+  if (whole_window(window)) return part > 0 ? 0x7fffffff : 0;
   return part <= kShortParts ? part * kShortPart : kShortParts * kShortPart + (part - kShortParts) * kLongPart;
 }
 
@@ -70,7 +76,7 @@ __host__ __device__ inline int partial_stride(int dim) { return (dim + 3) / 4 * 
 
 // Parts that a row's keys can span in a table of so many tokens, behind a window: w keys lie in at most ceil((w - 1) / part) + 1 parts of one size.
 inline int parts_of(int64_t capacity, int window) {
-  const int all = part_of(static_cast<int>(capacity) - 1) + 1;
+  const int all = part_of(static_cast<int>(capacity) - 1, window) + 1;
   const int64_t seen = window > 0 ? (static_cast<int64_t>(window) + 2 * kShortPart - 2) / kShortPart : all;
   return static_cast<int>(seen < all ? seen : all);
 }
