@@ -1016,7 +1016,7 @@ bool quantized_tiles_supported(const QuantizedAttentionArgs& a) {
   if (c.token_stride % 16 != 0 || c.block_stride % 16 != 0 || !aligned16(c.key) || !aligned16(c.value)) return false;
   if (a.q_stride % 4 != 0 || (reinterpret_cast<uintptr_t>(a.q) & 7u) != 0) return false;
   const int64_t group = a.q_heads / c.kv_heads, tiles = (static_cast<int64_t>(a.step.total) * group + 3) / 4 + a.step.sequences;
-  return tiles * c.kv_heads * a.parts <= 0x7fffffff && static_cast<int64_t>(a.step.total) * group < (1 << 26);     // items are counted in 32 bits
+  return tiles * c.kv_heads * a.parts <= 0x7fffffff && static_cast<int64_t>(a.step.total) * group <= (1 << 25);     // items are counted in 32 bits, a sequence's row tiles in 24
 }
 
 int launch_quantized_tiles(const QuantizedAttentionArgs& a, int max_new, cudaStream_t stream) {
