@@ -679,3 +679,51 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(x, alone[i]) for x in got[i])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kv_heads, group, counts", [(2, 1, [1, 1, 1]), (2, 4, [5, 2, 3]), (3, 1, [4, 4, 4]), (3, 2, [9, 1, 2]), (5, 7, [3, 1, 2])])
+@pytest.mark.parametrize("window", [0, 90])
+def test_nan_in_one_head_stays_in_it(dtype, kv_heads, group, counts, window):
+    """64-wide heads share lines of the cache: a NaN key or value of one head changes no bit of another one's rows."""
+    lengths = [200, 33, 1160]
+    call, options, _, _ = attention_case(group * kv_heads, kv_heads, 64, 16, lengths, counts, dtype, window=window, spare=0)
+    q, cache, tables, _, cu, most = call
+    clean = rlt.quantized_attention(*call, **options)
+    starts = plain.starts_of(counts)
+    for which in ("key", "value"):
+        codes = getattr(cache, which).view(torch.uint8)
+        for head in range(kv_heads):
+            saved = codes.clone()
+            seen = torch.zeros(sum(counts), dtype=torch.bool)
+            for s, (a, n) in enumerate(zip(lengths, counts)):
+                for token in (a - n - 20, a - 1):                    # one that all rows of the sequence see, one that only the last does
+                    codes[int(tables[s, token // 16]), token % 16, head, 7] = 0x7f if token % 2 else 0xff
+                seen[starts[s]:starts[s + 1]] = True
+            got = rlt.quantized_attention(*call, **options)
+            mine = torch.arange(group * kv_heads) // group == head
+            assert torch.equal(got[:, ~mine.cuda()], clean[:, ~mine.cuda()]), (which, head)
+            hit = got[:, mine.cuda()].isnan()
+            assert bool(hit.all() if which == "key" else hit[..., 7].all()), (which, head)
+            for s, (a, n) in enumerate(zip(lengths, counts)):
+                one = rlt.quantized_attention(q[starts[s]:starts[s + 1]].contiguous(), cache, tables[s:s + 1].contiguous(), plain.words([a]).cuda(),
+                                              plain.words([0, n]).cuda(), n, **options)
+                assert torch.equal(one.nan_to_num(9.0), got[starts[s]:starts[s + 1]].nan_to_num(9.0)), (which, head, s)
+            codes.copy_(saved)
+
+
+def test_a_stored_infinity_stays_in_its_head():
+    """What is not finite is stored as NaN: the rows of its own head are NaN, the neighbour's are as they would be without it."""
+    g = torch.Generator().manual_seed(5)
+    n, kv_heads, dim = 21, 2, 64
+    k, v = (torch.randn(n, kv_heads, dim, generator=g).bfloat16().cuda() for _ in range(2))
+    q = torch.randn(2, 8, dim, generator=g).bfloat16().cuda()
+    tables, lengths, cu = plain.words([[1, 0]]).cuda(), plain.words([n]).cuda(), plain.words([0, n]).cuda()
+    outs = []
+    for bad in (False, True):
+        if bad:
+            k[4, 1, 9] = math.inf
+        cache = rlt.QuantizedKV.allocate(2, 16, kv_heads, dim)
+        rlt.quantized_kv_write(cache, k, v, tables, lengths, cu)
+        outs.append(rlt.quantized_attention(q, cache, tables, lengths, plain.words([0, 2]).cuda(), 2))
+    assert outs[0].isfinite().all() and torch.equal(outs[0][:, :4], outs[1][:, :4]) and outs[1][:, 4:].isnan().all()

@@ -8,6 +8,9 @@
 //
 // Products.  Keys and values are the M operands, so a handful of rows is the N and nothing is padded to a tensor tile:
 //   S^T = K Q^T        lanes = 128 tokens, columns = rows;       O^T += V^T P^T     lanes = 128 value elements, V^T read MN-major
+// Two 64-wide heads share the 128 bytes of a token.  Each has a product of its own over its half of K and of the queries' lines, into columns of its
+// own: over the whole line, zeros in a query's other half would meet what the other head holds there, and 0 * NaN is NaN.  (O^T needs no such split:
+// an output element comes from its own value element, and the others are not stored.)
 // Q and P have more bits than a code, so both are sums of three: x = h + m / 32 + l / 1024, each rounded to four significant bits, what is
 // left going to the next: the columns of an operand are the three parts of its rows, and the parts of a result are added in fp32.  A query row
 // is brought to its own power of two first (the largest element in 2^7 .. 2^8); bf16 and fp16 rows lose what is 2^-27 of that.
@@ -95,7 +98,7 @@ template <int kRows>
 struct __align__(1024) Shared {
   static constexpr int kN = (3 * kRows + 15) / 16 * 16;         // three parts of every row, in whole sixteens
   unsigned char ring[kSlots][kTileBytes];             // [token][128 bytes], swizzled by the copy: keys of a tile, its values, the next tile's keys ..
-  unsigned char q[kDeep][kN * 128];                   // [item][part of a row][128 elements]
+  unsigned char q[kDeep][kN * 128];                   // [item][part of a row][128 elements], of two heads [item][part of a head's row][64 elements of each]
   unsigned char p[kGroups][2][kN * 128];              // of a group's tiles in turn: [16 parts of rows][128 tokens][16 bytes]
   uint32_t raw_q[kRows][64];                          // the next item's queries as they are
   float4 scales[kScaleSlots][2][kPieces];             // by head and 16 tokens: key scale, log2 of the value scale, its inverse
@@ -210,8 +213,9 @@ __device__ __forceinline__ void code_product(uint32_t d, uint64_t a, uint64_t b,
   asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
                ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
-template <int kCount>
-__device__ __forceinline__ void load_columns(uint32_t at, float (&x)[kCount]) {
+// kCount columns into x[kFirst] ..
+template <int kCount, int kFirst = 0, int kSize>
+__device__ __forceinline__ void load_columns(uint32_t at, float (&x)[kSize]) {
   uint32_t r[kCount];
   if constexpr (kCount == 8) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -220,7 +224,7 @@ __device__ __forceinline__ void load_columns(uint32_t at, float (&x)[kCount]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
   }
 #pragma unroll
-  for (int i = 0; i < kCount; ++i) x[i] = __uint_as_float(r[i]);
+  for (int i = 0; i < kCount; ++i) x[kFirst + i] = __uint_as_float(r[i]);
 }
 template <int kCount>
 __device__ __forceinline__ void store_columns(uint32_t at, const float (&x)[kCount]) {
@@ -309,6 +313,8 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   const auto block_sync = [] { asm volatile("bar.sync 4, %0;" ::"n"(kThreads) : "memory"); };
   const auto group_any = [](int group, bool mine) { return any_of_group<Role::kGroupThreads>(group, mine); };
   constexpr int kHeads = 128 / kDim, kEach = kRows / kHeads, kN = Sm::kN;
+  constexpr int kHeadN = (3 * kEach + 15) / 16 * 16;         // columns of a head's scores: three parts of its rows, in whole sixteens
+  static_assert(kHeadN * kHeads <= 64 && kHeadN <= kN, "columns of a group's scores (a head's share of them is 64 / kHeads), lines of an item's queries");
   // tensor memory: 64 columns for the scores of each group, then for its outputs of the items under way
   constexpr uint32_t kScores = 0, kOutputs = kGroups * 64, kColumns = 512;
   static_assert(kOutputs + kGroups * kDeep * 64 <= kColumns, "tensor memory");
@@ -533,7 +539,8 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       }
     } else if (warp == kScoreWarp) {
       // ---- S^T of a tile, once its keys and the item's queries are there and its group has read the scores of the tile before ----
-      constexpr uint32_t kIdesc = (1u << 4) | (static_cast<uint32_t>(kN >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
+      constexpr uint32_t kIdesc = (1u << 4) | (static_cast<uint32_t>(kHeadN >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
+      constexpr int kSteps = 4 / kHeads;      // of 32 codes, in a head
 #pragma unroll 1
       for (int it = 0; it < items && !failed; ++it) {
         const unsigned at = buffer();
@@ -554,7 +561,8 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             if (elect_one()) {
 #pragma unroll
               for (int ks = 0; ks < 4; ++ks)
-                code_product(tmem + kScores + group * 64, k_desc + static_cast<uint64_t>(ks * 2), q_desc + static_cast<uint64_t>(ks * 2), kIdesc, ks > 0);
+                code_product(tmem + kScores + group * 64 + ks / kSteps * 32, k_desc + static_cast<uint64_t>(ks * 2), q_desc + static_cast<uint64_t>(ks * 2), kIdesc,
+                             ks % kSteps > 0);
               umma_commit(smem_u32(&sm.s_ready[group]));
               umma_commit(smem_u32(&sm.empty[slot]));
             }
@@ -638,17 +646,16 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             uint32_t codes[kMine / 2][3];
 #pragma unroll
             for (int w = 0; w < kMine / 2; ++w) three_parts(odd ? 0.0f : v[2 * w] * up, odd ? 0.0f : v[2 * w + 1] * up, codes[w]);
-            // element lane * kMine of a 128-byte line whose 16-byte pieces are swizzled by the row; of two heads, the other's half of the line is zero
-            const uint32_t line = smem_u32(sm.q[buf]) + r * 128;
-            const int byte = (kHeads == 2 ? (r / kEach) * 64 : 0) + lane * kMine;
+            // element lane * kMine of a 128-byte line whose 16-byte pieces are swizzled by the line; of two heads, each has a half of a line
+            const int byte = r / kEach * kDim + lane * kMine;
 #pragma unroll
             for (int part = 0; part < 3; ++part) {
-              const uint32_t at = line + (byte ^ (((part * kRows + r) & 7) << 4));
+              const int line = part * kEach + r % kEach;
+              const uint32_t at = smem_u32(sm.q[buf]) + line * 128 + (byte ^ ((line & 7) << 4));
               if constexpr (kDim == 128) {
-                asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + part * kRows * 128), "r"(codes[0][part] | codes[kMine / 2 - 1][part] << 16) : "memory");
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(codes[0][part] | codes[kMine / 2 - 1][part] << 16) : "memory");
               } else {
-                asm volatile("st.shared.u16 [%0], %1;" ::"r"(at + part * kRows * 128), "h"(static_cast<uint16_t>(codes[0][part])) : "memory");
-                asm volatile("st.shared.u16 [%0], %1;" ::"r"((at ^ 64u) + part * kRows * 128), "h"(static_cast<uint16_t>(0)) : "memory");
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(static_cast<uint16_t>(codes[0][part])) : "memory");
               }
             }
           }
@@ -752,8 +759,13 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       constexpr int kMine = Role::kMine, kOfHead = kHeads == 2 && kHalves == 1 ? kEach : kMine;       // rows of a thread that share a head's scales
       const int group = warp / kGroupWarps, half = kHalves == 2 ? (warp >> 2) & 1 : 0, own = threadIdx.x & (kTile - 1), row0 = half * kMine;
       const int waits = warp % kGroupWarps;        // what this warp waits for in its group
-      const uint32_t lanes = (static_cast<uint32_t>((warp & 3) * 32) << 16) + group * 64 + row0;      // and columns
-      const uint32_t scores_at = tmem + lanes + kScores;
+      const uint32_t lanes = (static_cast<uint32_t>((warp & 3) * 32) << 16) + group * 64;      // and columns
+      const uint32_t scores_at = tmem + lanes + kScores + (kHeads == 2 ? half * 32 : row0);
+      // a part of this thread's scores (of two heads' rows, half are the other head's)
+      auto load_scores = [&](int part, float (&x)[kMine]) {
+        load_columns<kOfHead>(scores_at + part * kEach, x);
+        if constexpr (kOfHead < kMine) load_columns<kOfHead, kOfHead>(scores_at + 32 + part * kEach, x);
+      };
       // where this thread's weights go: its token's line of 16 bytes, a half's eight of them
       const uint32_t first_weights = smem_u32(sm.p[group][0]) + own * 16 + half * 8;
       const int folded_row = row0 + row_after_fold<kMine>(lane);
@@ -763,7 +775,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         const unsigned buf = buffer();
         failed = group_any(group, failed || (waits == 0 && !wait_for(smem_u32(&sm.q_full[buf]), phase())));
         const Item x = sm.list[it];
-        const uint32_t outputs_at = tmem + lanes + kOutputs + buf * kGroups * 64;
+        const uint32_t outputs_at = tmem + lanes + kOutputs + buf * kGroups * 64 + row0;
         const int mine = tiles_of(x, group);
         const unsigned before = group ? done_of[1] : done_of[0];
         float ref[kMine], l[kMine];
@@ -789,9 +801,9 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           if (group_any(group, !ok)) failed = true;
           tcgen05_after_sync();
           float s[kMine], m[kMine], rest[kMine];
-          load_columns<kMine>(scores_at, s);
-          load_columns<kMine>(scores_at + kRows, m);
-          load_columns<kMine>(scores_at + 2 * kRows, rest);
+          load_scores(0, s);
+          load_scores(1, m);
+          load_scores(2, rest);
           float4 scale_of[kMine / kOfHead];
 #pragma unroll
           for (int h = 0; h < kMine / kOfHead; ++h) scale_of[h] = load_shared16f(smem_u32(&sm.scales[scale_slot][kHeads == 2 && kHalves == 2 ? half : h][own >> 4]));
