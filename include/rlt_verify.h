@@ -787,7 +787,8 @@ RLT_API int rlt_return_pages(const int32_t* lengths, int requests, const int32_t
 /* ------------------------------------------------------------------------
  * A paged cache in 8 bits: e4m3 codes [pages][block_size][kv_heads][head_dim <= 256] (block_stride and token_stride in BYTES, the
  * [kv_heads, head_dim] tail contiguous) and fp32 scales [pages][kv_heads] (row stride scale_stride, in elements), keys and values alike;
- * value = code * scale.  No counterpart in the reference, whose caches hold the model's dtype.
+ * value = code * scale.  A value scale is zero or within 2^-100 .. 2^100: readers take one beyond an end as that end, and a negative or NaN one
+ * as NaN.  No counterpart in the reference, whose caches hold the model's dtype.
  * Rows are packed: rows cu_rows[s] .. cu_rows[s + 1] - 1 (int32 [sequences + 1]) are the last ones of sequence s, whose length with them is
  * lengths[s] (int32 [sequences]); page p of sequence s is block_tables[s][p] (int32 [sequences][table_width]).
  *

@@ -727,3 +727,65 @@ def test_a_stored_infinity_stays_in_its_head():
         rlt.quantized_kv_write(cache, k, v, tables, lengths, cu)
         outs.append(rlt.quantized_attention(q, cache, tables, lengths, plain.words([0, 2]).cuda(), 2))
     assert outs[0].isfinite().all() and torch.equal(outs[0][:, :4], outs[1][:, :4]) and outs[1][:, 4:].isnan().all()
+
+
+def scale_in_range(scale):
+    """The value scale that is read: the nearer end of 2^-100 .. 2^100, zero for zero, NaN for what is negative or NaN."""
+    scale = scale.double()
+    inside = scale.clamp(2.0 ** -100, 2.0 ** 100)
+    return torch.where(scale == 0, 0.0, torch.where(scale >= 0, inside, math.nan))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim", [128, 64, 40])
+@pytest.mark.parametrize("value_scale", [0.0, -0.0, 2.0 ** -110, 1e-35, 1e-40, 2.0 ** -100, 2.0 ** 100, 2.0 ** 110, math.inf])
+def test_value_scales_at_and_beyond_their_range(dtype, dim, value_scale):
+    """One cache gives one result, whatever kernel reads it: everywhere such a scale, and in one page beside ordinary ones."""
+    lengths, counts = [70, 35], [2, 1]
+    call, options, _, _ = attention_case(4, 2, dim, 16, lengths, counts, dtype, spare=0)
+    q, cache, tables, _, cu, _ = call
+    codes = [torch.nan_to_num(t.cpu().double()) for t in (cache.key, cache.value)]
+    ordinary = torch.nan_to_num(cache.value_scale, nan=1.0)
+    for everywhere in (True, False):
+        cache.value_scale.copy_(ordinary)
+        if everywhere:
+            cache.value_scale.fill_(value_scale)
+        else:
+            cache.value_scale[int(tables[0, 2])] = value_scale
+        scales = [torch.nan_to_num(cache.key_scale.cpu().double()), scale_in_range(cache.value_scale.cpu())]
+        want, parts = plain.attention(q.cpu(), codes, scales, tables.cpu(), lengths, plain.starts_of(counts))
+        got = rlt.quantized_attention(*call, **options).cpu().double()
+        tol = plain.allowed(want, parts, dtype, dim, tiles=dtype != torch.float32)
+        err = (got - want).abs()
+        assert bool((err <= tol).all()), (everywhere, float((err / tol).max()))
+        if everywhere and value_scale == 0:
+            assert bool((got == 0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [128, 64, 40])
+@pytest.mark.parametrize("bad", [math.nan, -1.0, -math.inf])
+def test_value_scales_that_are_no_sizes(dtype, dim, bad):
+    """The rows that see a token of such a page are NaN in its head, the others what they were."""
+    lengths, counts = [70, 35], [9, 2]                               # positions 61 .. 69: of the last page's tokens five rows see some, page 3 ends at 63
+    call, options, _, _ = attention_case(4, 2, dim, 16, lengths, counts, dtype, spare=0)
+    q, cache, tables, _, cu, _ = call
+    cache.value_scale.copy_(torch.nan_to_num(cache.value_scale, nan=1.0))
+    clean = rlt.quantized_attention(*call, **options)
+    cache.value_scale[int(tables[0, 4]), 1] = bad                    # tokens 64 .. 69
+    got = rlt.quantized_attention(*call, **options)
+    hit = torch.zeros(11, 4, dtype=torch.bool)
+    hit[3:9, 2:] = True
+    assert bool(got[hit.cuda()].isnan().all()) and torch.equal(got[~hit.cuda()], clean[~hit.cuda()])
+
+
+@pytest.mark.parametrize("value_scale", [0.0, 1e-35, 2.0 ** 110, math.nan])
+def test_long_portions_over_scales_beyond_their_range(value_scale):
+    lengths, counts = [200, 160], [200, 160]
+    call, options, _, _ = attention_case(32, 4, 64, 16, lengths, counts, torch.bfloat16, spare=0)
+    assert is_expanded(call, options)
+    q, cache, tables, on, cu, most = call
+    cache.value_scale[int(tables[1, 3]), 2] = value_scale
+    long, short = (rlt.quantized_attention(q, cache, tables, on, cu, m) for m in (most, 16))
+    assert torch.equal(long[200:].nan_to_num(9.0), short[200:].nan_to_num(9.0))
+    assert bool(long[200 + 48:, 16:24].isnan().all()) == math.isnan(value_scale) and bool(long[:200 + 48].isfinite().all())

@@ -57,7 +57,7 @@ quantized_rows_kernel(QuantizedAttentionArgs a) {
         const int64_t at = page * c.block_stride + (token - entry * c.block) * c.token_stride + static_cast<int64_t>(kv_head) * c.dim;
         const uint8_t* key = c.key + at;
         value = c.value + at;
-        value_scale = c.value_scale[page * c.scale_stride + kv_head];
+        value_scale = value_scale_of(c.value_scale[page * c.scale_stride + kv_head]);
         for (int d = 0; d < c.dim; ++d) score = fmaf(decode_one(key[d]), s_q[d], score);
         score *= c.key_scale[page * c.scale_stride + kv_head];
       }

@@ -101,7 +101,7 @@ struct __align__(1024) Shared {
   unsigned char q[kDeep][kN * 128];                   // [item][part of a row][128 elements], of two heads [item][part of a head's row][64 elements of each]
   unsigned char p[kGroups][2][kN * 128];              // of a group's tiles in turn: [16 parts of rows][128 tokens][16 bytes]
   uint32_t raw_q[kRows][64];                          // the next item's queries as they are
-  float4 scales[kScaleSlots][2][kPieces];             // by head and 16 tokens: key scale, log2 of the value scale, its inverse
+  float4 scales[kScaleSlots][2][kPieces];             // by head and 16 tokens: key scale, log2 of the value scale, its inverse, 0 where it is 0 (and 1)
   alignas(8) unsigned char wide[kScaleSlots][kPieces];      // a value scale of the piece is beyond 2^+-kWide
   Item list[kList];
   // of an item
@@ -488,12 +488,12 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         auto convert = [&] {
 #pragma unroll
           for (int h = 0; h < kHeads; ++h) {
-            // a scale that is no positive number within 2^-100 .. 2^100 is brought there: codes of a page of scale 0 then add nothing
-            const float v = fminf(fmaxf(next_value[h], 7.8886090522101181e-31f), 1.2676506002282294e30f);
+            // a scale of 0 goes as the smallest one, its weights as nothing; one that is NaN makes the scores NaN for the rows that see its tokens
+            const float given = value_scale_of(next_value[h]), v = fmaxf(given, power_of_two(kMinScaleExponent));
             const int e = (__float_as_int(v) >> 23) - 127;
             const float significand = __int_as_float((__float_as_int(v) & 0x007fffff) | 0x3f800000);      // 1 for powers of two: exact then
-            const float exponent = static_cast<float>(e) + __log2f(significand);
-            scales[h] = make_float4(next_key[h], exponent, power_of_two(-e) * __frcp_rn(significand), 0.0f);
+            const float exponent = given >= 0.0f ? static_cast<float>(e) + __log2f(significand) : NAN;
+            scales[h] = make_float4(next_key[h], exponent, power_of_two(-e) * __frcp_rn(significand), given == 0.0f ? 0.0f : 1.0f);
             wide |= fabsf(exponent) > kWide;
           }
         };
@@ -901,8 +901,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
               p = make_float2(fast_exp2(faint0 ? s[r] - scale.y : s[r]), fast_exp2(faint1 ? s[r + 1] - scale.y : s[r + 1]));
               l[r] = fmaf(p.x, faint0 ? 1.0f : scale.z, l[r]);
               l[r + 1] = fmaf(p.y, faint1 ? 1.0f : scale.z, l[r + 1]);
-              if (faint0) p.x = 0.0f;
-              if (faint1) p.y = 0.0f;
+              p = make_float2(faint0 ? 0.0f : p.x * scale.w, faint1 ? 0.0f : p.y * scale.w);
             }
             three_parts(p.x, p.y, codes[r / 2]);
           }

@@ -2,7 +2,7 @@
 // and read it share: its argument block, its conversions and the rows of a packed step.
 //
 // Scales that the store kernel writes are powers of two, so that x / scale and a change of scale are exact in fp32 and every code is
-// rounded once; readers take any positive scale.
+// rounded once.  Readers take a key's scale as it is, and a value's inside the range of those (value_scale_of).
 #pragma once
 
 #include <cuda_fp8.h>
@@ -137,6 +137,13 @@ __device__ __forceinline__ int exponent_above(float scale) {
   if (!(scale > 0.0f)) return kMinScaleExponent;
   const int bits = __float_as_int(scale), e = (bits >> 23) - 127 + ((bits & 0x7fffff) != 0 ? 1 : 0);
   return min(max(e, kMinScaleExponent), kMaxScaleExponent);
+}
+
+// The scale of values that every reader goes by: zero, or 2^-100 .. 2^100 (one beyond an end counts as that end, which keeps weight / scale and its
+// sums over a context within fp32); what is negative or NaN is no size, and NaN.
+__device__ __forceinline__ float value_scale_of(float scale) {
+  if (scale == 0.0f) return 0.0f;
+  return scale > 0.0f ? fminf(fmaxf(scale, power_of_two(kMinScaleExponent)), power_of_two(kMaxScaleExponent)) : NAN;
 }
 
 inline bool quantized_cache_valid(const QuantizedCache& c) {

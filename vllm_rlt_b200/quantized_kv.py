@@ -27,7 +27,9 @@ class QuantizedKV:
     """One layer's keys and values in 8 bits: a value is its code times the scale of its page and head.
 
     key / value: float8_e4m3fn `[pages, block, kv_heads, dim]` of one layout, pages and tokens with any stride, the `[kv_heads, dim]` tail
-    contiguous; dim at most 256.  key_scale / value_scale: float32 `[pages, kv_heads]` of one layout, heads side by side."""
+    contiguous; dim at most 256.  key_scale / value_scale: float32 `[pages, kv_heads]` of one layout, heads side by side.  Scales that
+    `quantized_kv_write` makes are powers of two, 2^-100 .. 2^100.  Others may be read too: a value scale beyond that range counts as its nearer
+    end, zero as zero, and a negative or NaN one makes the rows that see its page NaN in its head."""
 
     key: torch.Tensor
     value: torch.Tensor
