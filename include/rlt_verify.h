@@ -805,7 +805,8 @@ RLT_API int rlt_return_pages(const int32_t* lengths, int requests, const int32_t
  * [rows][q_heads][head_dim] with row strides.  max_new: the longest portion.  It, the numbers of rows and sequences and the shape choose the
  * kernels; among calls that they choose the same ones for, a row's bits depend on its own query, keys and values only.  bf16 portions of
  * more than 16 rows, long enough on average and without a window, are scored over an expansion of the pages in the workspace.  workspace:
- * rlt_quantized_attention_workspace_bytes(...) bytes, 256-byte aligned, private to the call until its work on `stream` completes. */
+ * rlt_quantized_attention_workspace_bytes(...) bytes, 256-byte aligned, private to the call until its work on `stream` completes.  Waits on the
+ * device are bounded; rows whose scoring gave up on one are NaN. */
 RLT_API int rlt_quantized_kv_write(void* key_cache, void* value_cache, float* key_scale, float* value_scale, int64_t block_stride,
                            int64_t token_stride, int64_t scale_stride, int64_t num_blocks, int block_size, int kv_heads, int head_dim,
                            const void* k, int64_t k_stride, const void* v, int64_t v_stride, int dtype, const int32_t* block_tables,

@@ -116,7 +116,7 @@ template <typename T>
 __global__ void __launch_bounds__(kWarps * 32)
 quantized_merge_kernel(QuantizedAttentionArgs a) {
   grid_dependency_wait();
-  if (a.step.only != nullptr && a.step.only[a.step.sequences] == 0) return;
+  if (!has_rows(a.step, a.step.sequences)) return;
   const QuantizedCache& c = a.cache;
   const int lane = threadIdx.x & 31;
   const int64_t pair = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
@@ -422,7 +422,10 @@ extern "C" RLT_API int rlt_quantized_attention(const void* q, int64_t q_stride, 
     bool scored = false;
     status = launch_expanded(a, e, static_cast<unsigned char*>(workspace), info.sm_count, &scored, s);
     if (status != RLT_OK) return status;
-    if (scored) a.step.only = reinterpret_cast<const int32_t*>(static_cast<unsigned char*>(workspace) + e.marked);
+    if (scored) {
+      a.step.only = reinterpret_cast<const int32_t*>(static_cast<unsigned char*>(workspace) + e.marked);
+      a.step.gave_up = reinterpret_cast<const uint32_t*>(static_cast<unsigned char*>(workspace) + e.prompt) + 1;      // the prompt kernels' error word
+    }
   }
   const bool tiles = quantized_tiles_supported(a);
   const int each = rows_at_a_time(rows, q_heads, a.parts, head_dim);

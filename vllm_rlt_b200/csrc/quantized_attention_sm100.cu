@@ -598,7 +598,8 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           }
           __syncwarp();
         }
-        if (elect_one()) umma_commit(smem_u32(&sm.done[at]));
+        // (an item without all of its products is never done: the result warps give up on it and leave NaN)
+        if (!failed && elect_one()) umma_commit(smem_u32(&sm.done[at]));
         __syncwarp();
         pass(x);
       }
@@ -609,7 +610,9 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       for (int it = 0; it < items && !failed; ++it) {
         const Item x = sm.list[it];
         const unsigned buf = buffer();
-        if (done_items >= kDeep && !__all_sync(0xffffffffu, wait_for(smem_u32(&sm.q_empty[buf]), phase() ^ 1))) { failed = true; break; }
+        // Twice: result warps that are waiting give up themselves meanwhile and go on, so every item gets the places where their NaN goes.
+        const uint32_t empty = smem_u32(&sm.q_empty[buf]), before = phase() ^ 1;
+        if (done_items >= kDeep && !__all_sync(0xffffffffu, wait_for(empty, before) || wait_for(empty, before))) { failed = true; break; }
         constexpr int kMine = kDim / 32;            // elements of a lane
         // lane r has row r's place in the item
         const int my_head = x.unit * kHeads + lane % kRows / kEach, my_pair = x.pair0 + lane % kEach, my_row = my_pair / group_heads;
@@ -971,7 +974,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       }
     }
   }
-  // a wait that gave up left NaN (a result warp's own, at the latest); copies still in flight land before the shared memory is given back
+  // a wait that gave up left NaN in the rows of its item and of those behind it (a result warp's own, at the latest); copies still in flight land before the shared memory is given back
   if (failed && warp >= kCopyWarp && warp < kScoreWarp)
     for (int i = 0; i < kSlots; ++i)
       if (!wait_for(smem_u32(&sm.full[i]), 0) && !wait_for(smem_u32(&sm.full[i]), 1)) break;

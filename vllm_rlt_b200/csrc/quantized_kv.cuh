@@ -54,6 +54,7 @@ struct PackedRows {
   int total;                    // rows of the step
   int row0, rows;               // of which a launch does rows row0 .. rows - 1
   const int32_t* only = nullptr;        // [sequences + 1]: where 0 the sequence has no rows, the last one 0: none has; nullptr: all have theirs
+  const uint32_t* gave_up = nullptr;    // of the kernel that scored the others: where not 0 a wait of it ran out, and all sequences have their rows again
 };
 
 struct QuantizedAttentionArgs {
@@ -81,11 +82,13 @@ inline int parts_of(int64_t capacity, int window) {
   return static_cast<int>(seen < all ? seen : all);
 }
 
+__device__ __forceinline__ bool has_rows(const PackedRows& p, int s) { return p.only == nullptr || p.only[s] != 0 || *p.gave_up != 0; }
+
 // The rows of sequence s that a launch does, kept inside the step's, and the sequence's length with the last of them.
 __device__ __forceinline__ void rows_of(const PackedRows& p, int s, int* first, int* count, int* length) {
   const int begin = min(max(p.cu[s], 0), p.total), end = min(max(p.cu[s + 1], begin), p.total), last = min(end, p.rows);
   *first = max(begin, p.row0);
-  *count = p.only == nullptr || p.only[s] != 0 ? max(last - *first, 0) : 0;
+  *count = has_rows(p, s) ? max(last - *first, 0) : 0;
   const int64_t tokens = static_cast<int64_t>(p.lengths[s]) - (end - last);
   *length = static_cast<int>(tokens < -0x7fffffff ? -0x7fffffff : tokens);
 }
