@@ -789,3 +789,14 @@ def test_long_portions_over_scales_beyond_their_range(value_scale):
     long, short = (rlt.quantized_attention(q, cache, tables, on, cu, m) for m in (most, 16))
     assert torch.equal(long[200:].nan_to_num(9.0), short[200:].nan_to_num(9.0))
     assert bool(long[200 + 48:, 16:24].isnan().all()) == math.isnan(value_scale) and bool(long[:200 + 48].isfinite().all())
+
+
+@pytest.mark.parametrize("dim", [128, 64])
+def test_rows_that_see_no_key_in_front_of_others(dim):
+    """Hundreds of padding sequences, whose items have nothing to score, in front of sequences that have."""
+    n = 700
+    lengths, counts = [0] * n, [1] * n
+    for s in (3, 299, 300, 511, 512, 640, 699):
+        lengths[s] = 200 + s
+    for kv_heads in (64, 6):
+        check_attention(kv_heads, kv_heads, dim, 16, lengths, counts, torch.bfloat16)

@@ -335,7 +335,7 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     for (int i = 0; i < kDeep; ++i) {
       mbar_init(smem_u32(&sm.q_full[i]), kQueryWarps);
       mbar_init(smem_u32(&sm.q_empty[i]), 4);                              // the result warps
-      mbar_init(smem_u32(&sm.done[i]), 1 + kGroups * kGroupWarps);        // the last product's completion, and each softmax warp
+      mbar_init(smem_u32(&sm.done[i]), 2 + kGroups * kGroupWarps);        // the last product's completion, the warp of S^T and each softmax warp
     }
     for (int i = 0; i < kGroups; ++i) {
       mbar_init(smem_u32(&sm.s_ready[i]), 1);
@@ -571,6 +571,8 @@ quantized_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           }
         }
         if (!__all_sync(0xffffffffu, ok)) failed = true;
+        // (nothing else holds an item without tiles back until this warp has seen its queries' phase)
+        if (!failed && lane == 0) mbar_arrive(smem_u32(&sm.done[at]));
         pass(x);
       }
     } else if (warp == kValueWarp) {
