@@ -1,6 +1,11 @@
 """Pages and slots of a step, the 8-bit cache and the attention over it, against plain float64 forms."""
 
 import math
+import os
+import subprocess
+import sys
+import threading
+from pathlib import Path
 
 import pytest
 import torch
@@ -800,3 +805,55 @@ def test_rows_that_see_no_key_in_front_of_others(dim):
         lengths[s] = 200 + s
     for kv_heads in (64, 6):
         check_attention(kv_heads, kv_heads, dim, 16, lengths, counts, torch.bfloat16)
+
+
+def test_requests_whose_sums_nearly_fill_the_usual_shared_memory():
+    """Each in a process that has made no larger call before."""
+    code = """
+import plain_quantized as plain, torch, vllm_rlt_b200 as rlt
+for n in (4053, 4094):
+    lengths, counts = [i % 40 for i in range(n)], [1 + i % 2 for i in range(n)]
+    tables = torch.randint(0, 1000, (n, 3), generator=torch.Generator().manual_seed(n), dtype=torch.int32)
+    want = plain.step_slots(lengths, counts, tables.tolist(), 16, 3 * n)
+    got = rlt.step_slots(plain.words(lengths).cuda(), plain.words(counts).cuda(), tables.cuda(), 16, 3 * n)
+    for name, expected in zip(("cu", "lengths", "positions", "row_seq", "write_blocks", "write_offsets"), want):
+        assert getattr(got, name).tolist() == expected, (n, name)
+    assert int(got.status) == 0
+for n in (6079, 6142):
+    lengths, held, free, count = [16 * (i % 3) for i in range(n)], [3] * n, [-1] * (3 * n), [0]
+    tables = torch.arange(3 * n, dtype=torch.int32).view(n, 3)
+    state = dict(held=plain.words(held).cuda(), free_pages=plain.words(free).cuda(), free_count=plain.words(count).cuda())
+    status = rlt.return_pages(plain.words(lengths).cuda(), tables.cuda(), 16, **state)
+    assert plain.return_pages(lengths, tables.tolist(), 16, held, free, count) == int(status) == 0
+    assert state["held"].tolist() == held and state["free_pages"].tolist() == free and state["free_count"].tolist() == count, n
+"""
+    root = Path(__file__).resolve().parent
+    done = subprocess.run([sys.executable, "-c", code], cwd=root.parent, env=dict(os.environ, PYTHONPATH=f"{root.parent}:{root}"), capture_output=True, text=True,
+                          timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_threads_with_unlike_numbers_of_requests():
+    """Steps of 8192, 5000 and 6 requests at once, each from a thread of its own: one does not take another's shared memory away."""
+    lib, failed = rlt.load_library(), []
+    sizes = (8192, 5000, 8192, 6)
+    streams = [torch.cuda.Stream() for _ in sizes]
+    arrays = [[torch.zeros(n + 1, dtype=torch.int64, device="cuda") for _ in range(8)] for n in sizes]
+    torch.cuda.synchronize()
+
+    def work(n, stream, at):
+        torch.cuda.set_device(0)
+        for _ in range(4000):
+            code = lib.rlt_step_slots(at[0], at[0], n, at[1], 1, 16, None, None, 0, None, 0, at[2], at[3], None, None, None, None, at[4], at[5], stream)
+            code = code or lib.rlt_return_pages(at[0], n, at[1], 1, 16, at[0], None, 0, at[6], at[7], stream)
+            if code:
+                failed.append((n, code, lib.rlt_last_error()))
+                return
+
+    threads = [threading.Thread(target=work, args=(n, s.cuda_stream, [t.data_ptr() for t in a])) for n, s, a in zip(sizes, streams, arrays)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed[0]

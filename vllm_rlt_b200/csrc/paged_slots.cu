@@ -200,8 +200,12 @@ return_pages_kernel(SlotArgs a) {
   }
 }
 
-int launch(const char* what, void (*kernel)(SlotArgs), const SlotArgs& a, size_t smem, int64_t work, cudaStream_t stream) {
-  if (smem > 48 * 1024) RLT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+// words: of shared memory for each request.
+int launch(const char* what, void (*kernel)(SlotArgs), const SlotArgs& a, int words, int64_t work, cudaStream_t stream) {
+  // The limit is the process's: always that of the most requests, so that no thread's call lowers what another is about to launch with (and whatever the
+  // size, since without it the kernel's static memory counts against the usual 48 KB too).
+  RLT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, words * static_cast<int>(sizeof(int)) * kMaxRequests));
+  const size_t smem = static_cast<size_t>(words) * sizeof(int) * a.requests;
   // Few rows are one CTA's work; a cluster's barrier costs more than a second pass over them.
   const unsigned ctas = work <= 2 * kThreads ? 1 : 8;
   cudaLaunchConfig_t config = {};
@@ -239,7 +243,7 @@ extern "C" RLT_API int rlt_step_slots(const int32_t* lengths, const int32_t* cou
   a.free_pages = const_cast<int32_t*>(free_pages); a.free_capacity = free_capacity; a.free_count = free_count; a.rows = rows; a.cu = cu;
   a.new_lengths = new_lengths; a.positions = positions; a.row_seq = row_seq; a.write_blocks = write_blocks; a.write_offsets = write_offsets;
   a.active_rows = active_rows; a.status = status;
-  return launch("step_slots_kernel", step_slots_kernel, a, 3 * sizeof(int) * static_cast<size_t>(requests) + 16, rows, static_cast<cudaStream_t>(stream));
+  return launch("step_slots_kernel", step_slots_kernel, a, 3, rows, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" RLT_API int rlt_return_pages(const int32_t* lengths, int requests, const int32_t* tables, int table_width, int block_size, int32_t* held,
@@ -252,6 +256,5 @@ extern "C" RLT_API int rlt_return_pages(const int32_t* lengths, int requests, co
   SlotArgs a = {};
   a.lengths = lengths; a.requests = requests; a.tables = const_cast<int32_t*>(tables); a.width = table_width; a.block = block_size; a.held = held;
   a.free_pages = free_pages; a.free_capacity = free_capacity; a.free_count = free_count; a.status = status;
-  return launch("return_pages_kernel", return_pages_kernel, a, 2 * sizeof(int) * static_cast<size_t>(requests) + 16,
-                static_cast<int64_t>(requests) * 8, static_cast<cudaStream_t>(stream));
+  return launch("return_pages_kernel", return_pages_kernel, a, 2, static_cast<int64_t>(requests) * 8, static_cast<cudaStream_t>(stream));
 }
