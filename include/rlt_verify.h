@@ -803,8 +803,9 @@ RLT_API int rlt_return_pages(const int32_t* lengths, int requests, const int32_t
  * t < lengths[s] - n_s + i + 1, with window > 0 the last `window` of those; a row that sees no key gives zeros, rows behind
  * cu_rows[sequences] are left alone, and out shares no memory with q.  A length beyond table_width * block_size (at most 2^26) is cut to it; a page outside the cache reads as zeros.  q, out:
  * [rows][q_heads][head_dim] with row strides.  max_new: the longest portion.  It, the numbers of rows and sequences and the shape choose the
- * kernels; among calls that they choose the same ones for, a row's bits depend on its own query, keys and values only.  bf16 portions of
- * more than 16 rows, long enough on average and without a window, are scored over an expansion of the pages in the workspace.  workspace:
+ * kernels; among calls that they choose the same ones for, a row's bits depend on its own query, keys and values only.  In a step of bf16
+ * portions that are long on average and have no window, the long ones (64 rows and more, 128 where no heads share keys) are scored over an
+ * expansion of their pages in the workspace.  workspace:
  * rlt_quantized_attention_workspace_bytes(...) bytes, 256-byte aligned, private to the call until its work on `stream` completes.  Waits on the
  * device are bounded; rows whose scoring gave up on one are NaN. */
 RLT_API int rlt_quantized_kv_write(void* key_cache, void* value_cache, float* key_scale, float* value_scale, int64_t block_stride,

@@ -857,3 +857,18 @@ def test_threads_with_unlike_numbers_of_requests():
         t.join()
     torch.cuda.synchronize()
     assert not failed, failed[0]
+
+
+@pytest.mark.parametrize("heads, kv_heads, dim", [(32, 8, 128), (16, 2, 64)])
+def test_short_portions_beside_a_long_one(heads, kv_heads, dim):
+    """A prompt's portion beside single tokens and verification rows: the short ones keep the bits that they have without it."""
+    lengths, counts = [1500, 900, 3000, 40, 2100, 17, 33, 700], [1, 900, 16, 1, 5, 0, 17, 70]
+    call, options, got = check_attention(heads, kv_heads, dim, 16, lengths, counts, torch.bfloat16)
+    assert is_expanded(call, options)
+    q, cache, tables, _, _, _ = call
+    starts = plain.starts_of(counts)
+    for s, (a, n) in enumerate(zip(lengths, counts)):
+        if n:
+            one = rlt.quantized_attention(q[starts[s]:starts[s + 1]].contiguous(), cache, tables[s:s + 1].contiguous(), plain.words([a]).cuda(),
+                                          plain.words([0, n]).cuda(), min(n, 16))
+            assert torch.equal(one, got[starts[s]:starts[s + 1]]) == (n < 64), s

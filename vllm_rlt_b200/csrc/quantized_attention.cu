@@ -4,6 +4,8 @@
 //
 // Contexts are split at fixed positions.  A part leaves O = sum 2^(s_t - M) v_t, M and l = sum 2^(s_t - M) in fp32 (s in log2
 // units); rows whose keys lie in one part are finished by the kernel that scored them, the others by the merge.
+#include <algorithm>
+
 #include "attention.cuh"
 #include "quantized_kv.cuh"
 
@@ -212,7 +214,10 @@ int launch_merge(const QuantizedAttentionArgs& a, cudaStream_t stream) {
 // products.  So its pages are expanded into bf16 once, which has room for every code times 2^-100 .. 2^100 without a rounding, and the
 // prompt kernel of 16-bit caches scores them in tiles of 256 rows.  What that kernel would get wrong is left to the tiles of this one: a
 // sequence with a value that is NaN (its weight of 0 in rows that do not see it would make them NaN), with a page scale that is no power of
-// two (its values would be rounded), or with a length beyond its table (rows are cut one by one here) is marked, and scored behind it.
+// two (its values would be rounded), or with a length beyond its table (rows are cut one by one here) is marked, and scored behind it.  So is a
+// sequence with a short portion beside long ones, and its pages stay as they are: a single token's context would be expanded for one row, and walked by
+// one CTA a head.  With all of them expanded / with the long ones, us, 32 heads over 8 of 128: 1000 rows beside ten single tokens on 50000 keys each
+// 2855 / 248, on 2000 keys 158 / 90; 4000 rows beside forty on 4000 962 / 407; 2000 rows beside ten on 16 keys 115 / 131.
 //
 // A CTA takes pages of 16 tokens of one sequence: sequence s in pages s * width16 .. of `key` and `value`, and the tables, lengths and row
 // bounds that say so.  Bound by its traffic, a byte read and two written: 4 contexts of 5117 tokens, 8 heads of 128, 126 MB in 19.2 us (6.5 TB/s),
@@ -225,6 +230,7 @@ struct Expanded {
   int32_t* cu;                  // [sequences + 1]
   int32_t* marked;              // [sequences + 1], zero before; the last: some sequence is
   int width16;
+  int least;                    // rows of a portion that is long
 };
 
 // Of four codes in a word: the top bit of each that is NaN (all seven bits under its sign are set).
@@ -237,9 +243,12 @@ __device__ __forceinline__ bool plain_scale(float scale) {
 __global__ void __launch_bounds__(256)
 quantized_expand_kernel(QuantizedCache c, PackedRows step, Expanded x) {
   const int s = blockIdx.y, capacity = table_tokens(step, c.block);
-  const int tokens = min(max(step.lengths[s], 0), capacity);
+  int first, count, length;
+  rows_of(step, s, &first, &count, &length);
+  const bool expands = count >= x.least;
+  const int tokens = expands ? min(max(length, 0), capacity) : 0;       // (the prompt kernel gives a short portion's rows zeros, which do not stay)
   const int32_t* table = step.tables + static_cast<int64_t>(s) * step.width;
-  bool marks = step.lengths[s] > capacity;
+  bool marks = expands ? length > capacity : count > 0;
   if (blockIdx.x == 0) {
     // bounds inside the rows that never fall, whatever stands in cu: the prompt kernel's list of tiles has room for those
     __shared__ int s_most[8];
@@ -299,6 +308,7 @@ int rows_at_a_time(int rows, int q_heads, int parts, int dim) {
 }
 
 constexpr size_t kMostExpanded = size_t{4} << 30;      // bytes of expanded pages: tables are as wide as the longest context may become
+constexpr int kLongRows = 64, kLongPasses = 8;         // of a portion that is expanded: its rows, and passes of the tiles over its context
 
 // Whether a step's portions are long enough, and what the expansion takes of the workspace.
 struct Expansion {
@@ -315,7 +325,7 @@ Expansion expansion_of(int rows, int sequences, int max_new, int q_heads, int kv
   // heads 570 / 338, 4 such portions 153 / 128, 4 of 1021 rows on 5120 tokens 431 / 119; with fewer rows 16 of 64, 292 / 331, 16 of 32 in
   // groups of four heads 291 / 359; with few CTAs 1 of 256 on 512 tokens 25 / 31, 1 of 64 in groups of four on 131072 tokens 911 / 1990.
   const int64_t passes = static_cast<int64_t>(rows) * (q_heads / kv_heads) / 16;
-  const bool pays = passes >= 8ll * sequences && rows >= 64ll * sequences && (static_cast<int64_t>(rows) / 256 + sequences) * q_heads >= 64;
+  const bool pays = passes >= static_cast<int64_t>(kLongPasses) * sequences && rows >= static_cast<int64_t>(kLongRows) * sequences && (static_cast<int64_t>(rows) / 256 + sequences) * q_heads >= 64;
   e.width16 = static_cast<int>(static_cast<int64_t>(width) * block / 16);
   const size_t pages = static_cast<size_t>(sequences) * e.width16, bytes = pages * 16 * kv_heads * dim * 2;
   if (!pays || 2 * bytes > kMostExpanded || pages > 0x7fffffff) return e;
@@ -339,6 +349,8 @@ int launch_expanded(const QuantizedAttentionArgs& a, const Expansion& e, unsigne
   x.key = reinterpret_cast<__nv_bfloat16*>(workspace + e.key); x.value = reinterpret_cast<__nv_bfloat16*>(workspace + e.value);
   x.tables = reinterpret_cast<int32_t*>(workspace + e.tables); x.lengths = reinterpret_cast<int32_t*>(workspace + e.lengths);
   x.cu = reinterpret_cast<int32_t*>(workspace + e.cu); x.marked = reinterpret_cast<int32_t*>(workspace + e.marked); x.width16 = e.width16;
+  const int group = a.q_heads / c.kv_heads;
+  x.least = std::max(kLongRows, (16 * kLongPasses + group - 1) / group);
   AttentionArgs p;
   p.q = a.q; p.out = a.out; p.key_cache = x.key; p.value_cache = x.value;
   p.token_stride = static_cast<int64_t>(c.kv_heads) * c.dim; p.block_stride = 16 * p.token_stride; p.num_blocks = static_cast<int64_t>(a.step.sequences) * e.width16;

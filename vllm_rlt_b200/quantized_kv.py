@@ -218,9 +218,9 @@ def quantized_attention(q, cache: QuantizedKV, tables, lengths, cu, max_new: int
     Row i of the n_s rows of sequence s sees lengths[s] - n_s + i + 1 keys, with `window` the last so many of them; a row that sees none gives
     zeros, a length that its table cannot address is cut to what it can, and rows behind the last sequence are left as they are in `out`
     (undefined where `out` is not given; it may not share memory with q).  scale: 1 / sqrt(dim) unless given.  max_new: the longest portion of
-    the step.  It, the shapes and the numbers of rows and sequences decide on the kernels: up to 16 rows, a row's bits are its own, whatever
-    else is in the call; long portions in bfloat16 without a window (64 rows and more on average) are scored over an expansion of their pages, with weights
-    rounded to bfloat16.  Heads are whole groups over the cache's.  Slots that no token was stored in may hold anything."""
+    the step.  It, the shapes and the numbers of rows and sequences decide on the kernels: in portions of up to 16 rows, a row's bits are its own,
+    whatever else is in the call; in a step of long portions in bfloat16 without a window (64 rows and more on average), those of 64 rows and more
+    (128 where no heads share keys) are scored over an expansion of their pages, with weights rounded to bfloat16.  Heads are whole groups over the cache's.  Slots that no token was stored in may hold anything."""
     cache.check()
     _check_step(tables, lengths, cu)
     pages, block, kv_heads, dim = cache.key.shape
