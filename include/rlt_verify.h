@@ -775,8 +775,8 @@ RLT_API int rlt_step_metadata(int32_t* words, const int64_t* at, const int64_t* 
  * active_rows, status: one int32.  held may be NULL (with free_pages and free_count): the tables are complete.  No two arguments share memory.
  *
  * rlt_return_pages: request s keeps the pages of its first lengths[s] tokens.  Page k of those given back goes to place
- * free_count + total - 1 - k, so that the call undoes the claims of the step before it.  status 1 and nothing changed where free_capacity
- * would be passed or held is out of range. */
+ * free_count + total - 1 - k, so that the call undoes the claims of the step before it.  Holders of a page are not counted: pages that requests
+ * share must not be given back here.  status 1 and nothing changed where free_capacity would be passed or held is out of range. */
 RLT_API int rlt_step_slots(const int32_t* lengths, const int32_t* counts, int requests, int32_t* tables, int table_width, int block_size,
                    int32_t* held, const int32_t* free_pages, int free_capacity, int32_t* free_count, int rows, int32_t* cu,
                    int32_t* new_lengths, int32_t* positions, int32_t* row_seq, int64_t* write_blocks, int64_t* write_offsets,

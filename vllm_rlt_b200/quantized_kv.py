@@ -148,7 +148,8 @@ def step_slots(lengths, counts, tables, block: int, rows: int, *, held=None, fre
 
 def return_pages(lengths, tables, block: int, *, held, free_pages, free_count):
     """Request s keeps the pages of its first `lengths[s]` tokens (0: none) and gives the others back to the stack, so that what was claimed
-    last is claimed next; held, free_pages and free_count are updated in place, the tables stay.  Returns an int32 status on the device: 0, or
+    last is claimed next; held, free_pages and free_count are updated in place, the tables stay.  A page is one request's: holders are not
+    counted, and a page that stands in two requests' tables would be given back by each.  Returns an int32 status on the device: 0, or
     1 where the stack has no room (pages given back twice) or a number of held pages cannot be; then nothing has changed."""
     _check_tables(tables)
     n, width = tables.shape
