@@ -795,7 +795,8 @@ RLT_API int rlt_return_pages(const int32_t* lengths, int requests, const int32_t
  * rlt_quantized_kv_write: k, v [rows][kv_heads][head_dim] of `dtype`, row strides in elements.  Per page that gets rows and head, K and V
  * apart: e the smallest exponent in [-100, 100] with max |finite x| <= 448 * 2^e over the new rows; scale = 2^e where offset 0 is written,
  * else max(2^e, old scale rounded up to a power of two), and where that is larger than the old one the tokens in front of the new rows are
- * rounded again; code = e4m3(x / scale), to nearest even, saturating; what is not finite becomes NaN.  A page that is written belongs to one
+ * rounded again; code = e4m3(x / scale), to nearest even, saturating; what is not finite becomes NaN.  A scale never shrinks while its page is
+ * held, so codes depend on how rows were grouped into calls, and on rows that were rejected afterwards.  A page that is written belongs to one
  * sequence of the call.  Rows at negative positions, behind cu_rows[sequences], beyond their table row or in pages outside the cache are
  * not stored.
  *

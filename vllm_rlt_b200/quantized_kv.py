@@ -196,6 +196,10 @@ def quantized_kv_write(cache: QuantizedKV, k, v, tables, lengths, cu) -> None:
     are rounded again.  A page whose offset 0 is written starts anew: what it held behind the new rows means nothing any more.  Codes are
     rounded to the nearest, ties to even; elements that are not finite are stored as NaN and have no part in a scale.
 
+    So what a page holds depends on every row that was written to it, those that were rejected later among them: a scale that grew for one
+    stays, and the tokens in front were rounded for it.  Steps that speculate store other codes than steps of one token, and a prompt in one call
+    others than in several; tokens chosen over such a cache may differ by that.
+
     A page that is written belongs to one sequence of the call.  Rows at negative positions, behind the last sequence, behind the end of
     their table row or in a page that does not exist are not stored."""
     cache.check()
