@@ -12,7 +12,7 @@
 //
 // Bound by its traffic for prompts: 16 of 128 to 1024 rows, 16 heads of 128 in bf16, 105 MB, take 27.8 us (3.8 TB/s; 34.5 with keys and values in
 // one CTA, 60 when every run was read twice with one load in flight).  What is left is the start (the rows' sequences, their tables: four dependent
-// reads) and the tail of CTAs that are all resident at once.  One row of each of 128 requests, 8 heads: 4.6 us, a launch and those reads.
+// reads) and the tail of two waves of CTAs (1070 of them, four an SM).  One row of each of 128 requests, 8 heads: 4.6 us, a launch and those reads.
 #include <type_traits>
 
 #include "quantized_kv.cuh"

@@ -225,7 +225,11 @@ def quantized_attention(q, cache: QuantizedKV, tables, lengths, cu, max_new: int
     (undefined where `out` is not given; it may not share memory with q).  scale: 1 / sqrt(dim) unless given.  max_new: the longest portion of
     the step.  It, the shapes and the numbers of rows and sequences decide on the kernels: in portions of up to 16 rows, a row's bits are its own,
     whatever else is in the call; in a step of long portions in bfloat16 without a window (64 rows and more on average), those of 64 rows and more
-    (128 where no heads share keys) are scored over an expansion of their pages, with weights rounded to bfloat16.  Heads are whole groups over the cache's.  Slots that no token was stored in may hold anything."""
+    (128 where no heads share keys) are scored over an expansion of their pages, with weights rounded to bfloat16.  Otherwise weights have 11 bits
+    where 16-bit queries meet 64- or 128-wide heads in pages of whole 16-token tiles, fp32's elsewhere.  A call's scratch goes by the tables'
+    width: up to 2 GB for the parts of long contexts, and up to 4 GB for expanded pages (where they would take more, nothing is expanded).
+
+    Heads are whole groups over the cache's.  Slots that no token was stored in may hold anything."""
     cache.check()
     _check_step(tables, lengths, cu)
     pages, block, kv_heads, dim = cache.key.shape
