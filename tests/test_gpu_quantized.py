@@ -872,3 +872,34 @@ def test_short_portions_beside_a_long_one(heads, kv_heads, dim):
             one = rlt.quantized_attention(q[starts[s]:starts[s + 1]].contiguous(), cache, tables[s:s + 1].contiguous(), plain.words([a]).cuda(),
                                           plain.words([0, n]).cuda(), min(n, 16))
             assert torch.equal(one, got[starts[s]:starts[s + 1]]) == (n < 64), s
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads, kv_heads, dim, block", [(8, 2, 128, 16), (6, 3, 64, 32), (4, 2, 40, 8)])
+def test_keys_and_values_side_by_side_in_one_pool(dtype, heads, kv_heads, dim, block):
+    """A pool [pages, block, keys or values, kv_heads, dim]: tokens are two rows apart, pages further than their tokens."""
+    g = torch.Generator().manual_seed(dim)
+    lengths, counts = [70, 33, 130], [3, 33, 40]
+    tables, pages = pages_for(lengths, block, g)
+    raw, scales = plain.make_cache(pages, block, kv_heads, dim, g)                    # [2, pages, 1, block, heads, dim]
+    pool = torch.full((pages, block + 2, 2, kv_heads, dim), 0x7f, dtype=torch.uint8, device="cuda")
+    pool[:, :block] = raw[:, :, 0].permute(1, 2, 0, 3, 4).cuda()
+    before = pool.clone()
+    dev_scales = scales[:, :, 0].contiguous().cuda()
+    cache = rlt.QuantizedKV(pool[:, :block, 0].view(plain.CODE), pool[:, :block, 1].view(plain.CODE), dev_scales[0], dev_scales[1])
+    cu = plain.starts_of(counts)
+    k, v = (torch.randn(sum(counts), kv_heads, dim, generator=g).to(dtype) for _ in range(2))
+    rlt.quantized_kv_write(cache, k.cuda(), v.cuda(), tables.cuda(), plain.words(lengths).cuda(), plain.words(cu).cuda())
+    codes, want_scales = raw[:, :, 0].view(plain.CODE).double(), scales[:, :, 0].double()
+    for i, x in enumerate((k, v)):
+        plain.kv_write(codes[i], want_scales[i], x.double(), tables, lengths, cu)
+    assert torch.equal(dev_scales.cpu().double(), want_scales)
+    assert same_values(cache.key.cpu().double(), codes[0]) and same_values(cache.value.cpu().double(), codes[1])
+    assert torch.equal(pool[:, block:], before[:, block:])
+    for most, some in ((3, [3, 2, 1]), (40, [3, 33, 40])):
+        rows = plain.starts_of(some)
+        q = (torch.randn(sum(some), heads, dim, generator=g) * 0.1).to(dtype)
+        want, parts = plain.attention(q, codes, want_scales, tables, lengths, rows)
+        got = rlt.quantized_attention(q.cuda(), cache, tables.cuda(), plain.words(lengths).cuda(), plain.words(rows).cuda(), most).cpu().double()
+        tol = plain.allowed(want, parts, dtype, dim, tiles=dtype != torch.float32)
+        assert bool(((got - want).abs() <= tol).all()), most
