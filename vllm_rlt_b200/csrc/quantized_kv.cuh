@@ -82,7 +82,7 @@ inline int parts_of(int64_t capacity, int window) {
   return static_cast<int>(seen < all ? seen : all);
 }
 
-__device__ __forceinline__ bool has_rows(const PackedRows& p, int s) { return p.only == nullptr || p.only[s] != 0 || *p.gave_up != 0; }
+__device__ __forceinline__ bool has_rows(const PackedRows& p, int s) { return p.only == nullptr || (static_cast<uint32_t>(p.only[s]) | *p.gave_up) != 0; }
 
 // The rows of sequence s that a launch does, kept inside the step's, and the sequence's length with the last of them.
 __device__ __forceinline__ void rows_of(const PackedRows& p, int s, int* first, int* count, int* length) {
