@@ -28,8 +28,8 @@
 // What bounds it.  The bytes of keys and values would take 1440 cycles a tile (32 KB) of an SM; with sixteen rows an item the warps issue about 4800
 // instructions for one (half of them the softmax's, a quarter what an item costs at its ends), at 2.4 a cycle.  Measured, heads of 128, bf16:
 //   64 requests, 16 rows of 16 heads each, contexts of 512 to 4096        157 us, 4.0 TB/s of keys and values
-//   128 requests, a row of 32 heads over 8, contexts of 100 to 2048        65 us, 4.6 TB/s (items of four rows: the chain of a tile's waits)
-//   4 requests, 5 rows of 32 heads over 8, contexts of 65000 to 131072    264 us, 3.1 TB/s (20 rows are two items: every tile is scored twice)
+//   128 requests, a row of 32 heads over 8, contexts of 100 to 2048        66 us, 4.5 TB/s (items of four rows: the chain of a tile's waits)
+//   4 requests, 5 rows of 32 heads over 8, contexts of 65000 to 131072    265 us, 3.1 TB/s (20 rows are two items: every tile is scored twice)
 // (a call's time with the joining of its parts, 5 to 10 us of it).  With items found by every warp for itself, four copy warps at all sizes and
 // weights stored byte by byte: 189, 78 and 315 us.  With the codes converted to half precision and multiplied by the warps (mma.sync): 342,
 // 176 and 642 us.
