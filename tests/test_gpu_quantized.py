@@ -903,3 +903,30 @@ def test_keys_and_values_side_by_side_in_one_pool(dtype, heads, kv_heads, dim, b
         got = rlt.quantized_attention(q.cuda(), cache, tables.cuda(), plain.words(lengths).cuda(), plain.words(rows).cuda(), most).cpu().double()
         tol = plain.allowed(want, parts, dtype, dim, tiles=dtype != torch.float32)
         assert bool(((got - want).abs() <= tol).all()), most
+
+
+def test_portions_of_a_captured_step_become_short_and_long():
+    """A call captured with long portions, replayed with others of any length in the same rows: each portion goes where its rows say, and rows
+    behind the last sequence stay."""
+    lengths = [300, 500, 200]
+    call, _, _, _ = attention_case(32, 8, 128, 16, lengths, [100, 120, 80], torch.bfloat16, spare=0, width=40)
+    q, cache, tables, dev_lengths, cu, most = call
+    assert is_expanded(call, {})
+    out = torch.full_like(q, 7.0)
+    rlt.quantized_attention(*call, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rlt.quantized_attention(*call, out=out)
+    for counts in ([100, 120, 80], [1, 5, 16], [63, 64, 65], [0, 150, 1], [0, 0, 0], [200, 99, 1]):
+        starts = plain.starts_of(counts)
+        cu.copy_(plain.words(starts))
+        out.fill_(7.0)
+        graph.replay()
+        for s, n in enumerate(counts):
+            if n:
+                rows = q[starts[s]:starts[s + 1]].contiguous()
+                part = torch.cat((rows, rows.new_zeros(256 - n, *rows.shape[1:]))) if n >= 64 else rows        # (of a step long enough)
+                one = rlt.quantized_attention(part, cache, tables[s:s + 1].contiguous(), dev_lengths[s:s + 1], plain.words([0, n]).cuda(), len(part) if n >= 64 else 16)
+                assert torch.equal(one[:n], out[starts[s]:starts[s + 1]]), (counts, s)
+        assert bool((out[starts[3]:] == 7.0).all())
